@@ -7,10 +7,21 @@ written against the reference runs unchanged.
 """
 
 from nibble_amd.checkpoint import load_quantized_weight_checkpoint, save_quantized_weight_checkpoint
-from nibble_amd.cuda import cuda_extension_available, dequantize_cuda, linear_cuda
+from nibble_amd.cuda import (
+    cuda_extension_available,
+    dequantize_cuda,
+    kv_attention_cuda,
+    kv_read_cuda,
+    kv_write_cuda,
+    linear_cuda,
+    rotary_cuda,
+    rotary_kv_write_cuda,
+)
 from nibble_amd.integration import load_packed_state_dict, replace_linear_layers
+from nibble_amd.kv_cache import QuantizedKVCache
 from nibble_amd.linear import Int4Linear, QuantizedLinear
 from nibble_amd.quantization import pack_int4, quantize_and_pack_weights, quantize_groupwise, unpack_int4
+from nibble_amd.rotary import rope_frequencies, rope_tables, rotary
 
 __all__ = [
     "QuantizedLinear",
@@ -26,4 +37,13 @@ __all__ = [
     "linear_cuda",
     "dequantize_cuda",
     "cuda_extension_available",
+    "QuantizedKVCache",
+    "rope_frequencies",
+    "rope_tables",
+    "rotary",
+    "rotary_cuda",
+    "kv_write_cuda",
+    "rotary_kv_write_cuda",
+    "kv_read_cuda",
+    "kv_attention_cuda",
 ]

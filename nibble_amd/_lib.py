@@ -112,6 +112,48 @@ DECODE_SIGNATURES = {
                                                    _i64, _vp]),
 }
 
+# include/w4a16_kv.h
+FP16, BF16, FP32 = 0, 1, 2
+KV_INT8, KV_FP8 = 0, 1
+
+
+class KVRows(ctypes.Structure):
+    """w4a16_kv_rows"""
+
+    _fields_ = [("data", _vp), ("batch_stride", _i64), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class KVCodes(ctypes.Structure):
+    """w4a16_kv_codes"""
+
+    _fields_ = [("codes", _vp), ("scales", _vp), ("batch_stride", _i64), ("head_stride", _i64),
+                ("scale_batch_stride", _i64), ("scale_head_stride", _i64)]
+
+
+class KVCache(ctypes.Structure):
+    """w4a16_kv_cache"""
+
+    _fields_ = [("k", KVCodes), ("v", KVCodes), ("batch", _i64), ("kv_heads", _i64), ("slots", _i64),
+                ("head_dim", _i64), ("block", _i64), ("code_type", ctypes.c_int)]
+
+
+_rows_p = ctypes.POINTER(KVRows)
+_codes_p = ctypes.POINTER(KVCodes)
+_cache_p = ctypes.POINTER(KVCache)
+
+# every symbol declared in include/w4a16_kv.h
+KV_SIGNATURES = {
+    "w4a16_rotary": (ctypes.c_int, [_rows_p, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
+                                    ctypes.c_int, ctypes.c_int, _vp]),
+    "w4a16_kv_write": (ctypes.c_int, [_rows_p, _rows_p, _i64, _cache_p, _vp, _vp, ctypes.c_int, _vp]),
+    "w4a16_rotary_kv_write": (ctypes.c_int, [_rows_p, _vp, _i64, _rows_p, _rows_p, _i64, _vp, _vp, _i64, _i64,
+                                             ctypes.c_int, _cache_p, _vp, _vp, ctypes.c_int, _vp]),
+    "w4a16_kv_read": (ctypes.c_int, [_codes_p, _vp, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, _vp]),
+    "w4a16_kv_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "w4a16_kv_attention": (ctypes.c_int, [_rows_p, _vp, _i64, _i64, _cache_p, _vp, _vp, ctypes.c_float, ctypes.c_int,
+                                          _vp, _i64, _vp]),
+}
+
 _lib = None
 
 
@@ -130,7 +172,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`"
             )
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (restype, argtypes) in {**SIGNATURES, **DECODE_SIGNATURES}.items():
+        for name, (restype, argtypes) in {**SIGNATURES, **DECODE_SIGNATURES, **KV_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.restype = restype
             fn.argtypes = argtypes

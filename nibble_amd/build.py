@@ -52,7 +52,7 @@ def _run(cmd: list[str], verbose: bool) -> None:
 
 HIP_SOURCES = ["w4a16_hip.hip", "w4a16_decode.hip", "w4a16_pair.hip", "w4a16_stream.hip", "w4a16_gemm.hip",
                "w4a16_pair_ring.hip", "w4a16_quant.hip",
-               "w4a16_group.hip"]
+               "w4a16_group.hip", "w4a16_kv.hip", "w4a16_kv_attn.hip"]
 
 
 def build_hip(verbose: bool = False) -> str:

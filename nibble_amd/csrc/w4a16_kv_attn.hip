@@ -1,0 +1,830 @@
+// Attention over the 8-bit key/value cache (include/w4a16_kv.h).
+//
+// Mathematics. The query rows of one KV head, r = t group + g (token t, query
+// head g of the head's group), attend together, so that a key or value is
+// read once for all of them. With e_k, e_v the exponents of the scales of slot
+// j's blocks, the score in powers of two is
+//     s_j = (q . code_k,j) 2^e_k scale log2(e),
+// and the value's scale joins the softmax instead of the product:
+//     w_j = s_j + e_v,   R = max_j w_j,   P_j = 2^(w_j - R) in [0, 1],
+//     o = sum_j P_j code_v,j / sum_j 2^-e_v P_j.
+// Both products run on the matrix cores with fp16 operands: codes are exact in
+// fp16, q is exact too (bf16 rows are moved into fp16's range by a power of
+// two per row), and P is the only rounding: relative 2^-11, one for each
+// weight, whatever the scales of the values are, as the largest P is 1. Scores,
+// R, both sums and the outputs are fp32.
+//
+// S^T = K Q^T and O^T = V^T P^T: with keys in the rows of the first product a
+// lane receives weights of consecutive keys of its own query column, which are
+// the second product's right operand as they stand, if V^T's keys are taken in
+// the same order. Neither P nor, in the decode form, K and V pass through LDS.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+#include "w4a16_hip.h"
+#include "w4a16_kv_device.h"
+#include "w4a16_kv_host.h"
+
+namespace w4a16 {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnArgs {
+    const uint16_t* q;
+    uint16_t* out;
+    const uint8_t *k_codes, *v_codes;
+    const float *k_scales, *v_scales;
+    const int64_t *start, *counts;
+    float2* states;   // [batch tokens heads][splits] {R, l} and
+    float* partial;   // [batch tokens heads][splits][dim], with splits > 1
+    int64_t qb, qt, qh;
+    int64_t kb, kh, vb, vh, ksb, ksh, vsb, vsh;
+    int64_t slots;
+    float scale;
+    int tokens, heads, kv_heads, group, block_log, splits, row_tiles;
+    bool vec;
+};
+
+// What a workgroup's rows see: rows row0 .. of sequence b.
+struct Seen {
+    int64_t start;
+    int count;   // tokens that are no padding
+};
+
+__device__ __forceinline__ Seen seen_of(const AttnArgs& a, int b) {
+    Seen s;
+    s.start = min(a.start[b], a.slots);   // past the slots: no row is inside
+    s.count = a.tokens;
+    if (a.counts != nullptr) s.count = (int)min(max(a.counts[b], (int64_t)0), (int64_t)a.tokens);
+    return s;
+}
+
+// Slots that the rows row0 .. row0 + n - 1 see together: 0 .. end - 1.
+__device__ __forceinline__ int seen_end(const AttnArgs& a, const Seen& s, int row0, int n) {
+    const int last_row = min(row0 + n, a.tokens * a.group) - 1;
+    const int t = min(last_row / a.group, s.count - 1);
+    if (t < row0 / a.group) return 0;
+    const int64_t p = min(s.start + t, a.slots - 1);
+    return p < 0 ? 0 : (int)p + 1;
+}
+
+// A query row's 16-bit values -> fp16, with the power of two that was divided
+// out (bf16 only). The row's values are spread over the lanes that `rowmax`
+// joins.
+template <int TYPE, int N, typename F>
+__device__ __forceinline__ float query_to_f16(u32x4 (&q)[N], F rowmax) {
+    if constexpr (TYPE == W4A16_FP16) {
+        return 1.0f;
+    } else {
+        float amax = 0.0f;
+        float x[N][8];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            widen8<TYPE>(q[i], x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[i][e]));
+        }
+        amax = rowmax(amax);
+        // the largest magnitude to 2^14 .. 2^15; infinities and zeros keep a shift that a float holds
+        int shift = 14 - ((int)(__builtin_bit_cast(uint32_t, amax) >> 23) - 127);
+        shift = min(max(shift, -120), 120);
+        const float m = exp2_int(shift);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] *= m;
+            q[i] = narrow8<W4A16_FP16>(x[i]);
+        }
+        return exp2_int(-shift);
+    }
+}
+
+// 8 codes (two biased words) as a matrix operand.
+template <int CODES>
+__device__ __forceinline__ f16x8 decode8(uint32_t a, uint32_t b) {
+    a = kv_bias<CODES>(a);
+    b = kv_bias<CODES>(b);
+    const u32x4 v = {as_u32(decode2_f16<CODES, false>(a)), as_u32(decode2_f16<CODES, true>(a)),
+                     as_u32(decode2_f16<CODES, false>(b)), as_u32(decode2_f16<CODES, true>(b))};
+    return __builtin_bit_cast(f16x8, v);
+}
+
+// Words x[0..7] of 8 keys, 4 dims each -> for dim DD the 8 keys' values as a
+// matrix operand. Byte pairs of neighbouring keys come together by v_perm.
+template <int CODES>
+__device__ __forceinline__ void transpose8(const uint32_t (&x)[8], f16x8 (&out)[4]) {
+    u32x4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = kv_bias<CODES>(perm(x[2 * i + 1], x[2 * i], 0x05010400u));   // dims 0, 1
+        const uint32_t hi = kv_bias<CODES>(perm(x[2 * i + 1], x[2 * i], 0x07030602u));   // dims 2, 3
+        v[0][i] = as_u32(decode2_f16<CODES, false>(lo));
+        v[1][i] = as_u32(decode2_f16<CODES, true>(lo));
+        v[2][i] = as_u32(decode2_f16<CODES, false>(hi));
+        v[3][i] = as_u32(decode2_f16<CODES, true>(hi));
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) out[d] = __builtin_bit_cast(f16x8, v[d]);
+}
+
+// 4 consecutive outputs of a row.
+template <int TYPE>
+__device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(narrow16<TYPE>(a) | (narrow16<TYPE>(b) << 16),
+                                              narrow16<TYPE>(c) | (narrow16<TYPE>(d) << 16));
+}
+
+// ---------------------------------------------------------------------------
+// Decode form: up to 16 NT query rows of a KV head, every wavefront streaming
+// chunks of 32 slots.
+//
+// Bound: the cache's bytes. Lane (c, h) = (lane & 15, lane >> 4). Keys: 16
+// bytes of row c at 64 j + 16 h, so that two loads of 1 KiB read 16 rows of 64
+// (128, 256) bytes; values: dim / 16 bytes at dim / 16 c of the rows that the
+// lane's weights stand for (slots 4 h + i and 16 + 4 h + i), whole rows again.
+// The next chunk's keys are requested when the present ones are multiplied,
+// its values likewise. Wavefronts of a workgroup join through LDS; the slots
+// of a sequence are divided into `splits` shares, joined by merge_kernel.
+// ---------------------------------------------------------------------------
+constexpr int kDecodeWaves = 4;
+
+template <int D, int NT, int CODES, int TYPE>
+__global__ void __launch_bounds__(64 * kDecodeWaves)
+decode_kernel(const AttnArgs a) {
+    constexpr int W = kDecodeWaves;
+    constexpr int J = D / 64;                    // 16-byte loads of a key row's quarter; words of a value load
+    constexpr int PARTS = D > 128 ? D / 128 : 1;
+    constexpr int DP = D / PARTS;
+    __shared__ float row_max[W][16 * NT], row_sum[W][16 * NT];
+    __shared__ __align__(16) float joined[W][16][DP + 4];
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int c = lane & 15, h = lane >> 4;
+    int item = blockIdx.x;
+    const int split = item % a.splits;
+    item /= a.splits;
+    const int tile = item % a.row_tiles;
+    item /= a.row_tiles;
+    const int hk = item % a.kv_heads, b = item / a.kv_heads;
+    const int rows = a.tokens * a.group, row0 = tile * 16 * NT;
+
+    u32x4 qr[NT][2 * J];
+    float row_scale[NT];
+    int last[NT];
+    const Seen seen = seen_of(a, b);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = min(row0 + 16 * n + c, rows - 1);
+        const int t = r / a.group, g = r - t * a.group;
+        const uint16_t* q = a.q + b * a.qb + t * a.qt + (hk * a.group + g) * a.qh;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            qr[n][2 * j] = load8(q + 64 * j + 16 * h, a.vec);
+            qr[n][2 * j + 1] = load8(q + 64 * j + 16 * h + 8, a.vec);
+        }
+        const int64_t p = seen.start + t;
+        last[n] = t < seen.count && p >= 0 && p < a.slots ? (int)p : -1;
+    }
+    const int end = seen_end(a, seen, row0, 16 * NT);
+    const int last_slot = max(end - 1, 0);
+    const int chunks = (end + 31) >> 5;
+    const int share = (chunks + a.splits - 1) / a.splits;
+    const int first = split * share, stop = min(chunks, first + share);
+
+    const uint8_t* kc = a.k_codes + b * a.kb + hk * a.kh;
+    const uint8_t* vc = a.v_codes + b * a.vb + hk * a.vh;
+    const float* ks = a.k_scales + b * a.ksb + hk * a.ksh;
+    const float* vs = a.v_scales + b * a.vsb + hk * a.vsh;
+
+    u32x4 kr[2][J];
+    uint32_t vr[8][J];
+    float k_scale[2], v_scale[2];
+    auto load_keys = [&](int chunk) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const uint8_t* row = kc + (int64_t)min(32 * chunk + 16 * m + c, last_slot) * D + 16 * h;
+#pragma unroll
+            for (int j = 0; j < J; ++j) kr[m][j] = *reinterpret_cast<const u32x4*>(row + 64 * j);
+            const int at = min(32 * chunk + 16 * m, last_slot) >> a.block_log;
+            k_scale[m] = ks[at];
+            v_scale[m] = vs[at];
+        }
+    };
+    auto load_values = [&](int chunk) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int slot = 32 * chunk + 16 * (i >> 2) + 4 * h + (i & 3);
+            const uint8_t* row = vc + (int64_t)min(slot, last_slot) * D + (D / 16) * c;
+            if constexpr (J == 1) {
+                vr[i][0] = *reinterpret_cast<const uint32_t*>(row);
+            } else if constexpr (J == 2) {
+                const uint2 v = *reinterpret_cast<const uint2*>(row);
+                vr[i][0] = v.x;
+                vr[i][1] = v.y;
+            } else {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(row);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) vr[i][w] = v[w];
+            }
+        }
+    };
+
+    // the first chunk whether or not there is one (rows are clamped): registers
+    // that only one side of a branch defines have been miscompiled here
+    int chunk = first + wave;
+    load_keys(chunk);
+    load_values(chunk);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+        row_scale[n] = a.scale * kLog2e * query_to_f16<TYPE>(qr[n], row_pair_max);
+
+    float run_max[NT], run_sum[NT];
+    f32x4 acc[NT][D / 16];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        run_max[n] = -__builtin_inff();
+        run_sum[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) acc[n][i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    while (chunk < stop) {
+        const int slot0 = 32 * chunk;
+        f32x4 st[NT][2];
+        float ksc[2], vex[2], vinv[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            ksc[m] = k_scale[m];
+            const int e = exponent_of(v_scale[m]);
+            vex[m] = (float)e;
+            vinv[m] = exp2_int(-e);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) st[n][m] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const f16x8 key = decode8<CODES>(kr[m][j][2 * x], kr[m][j][2 * x + 1]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        st[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            key, __builtin_bit_cast(f16x8, qr[n][2 * j + x]), st[n][m], 0, 0, 0);
+                }
+        }
+        const bool more = chunk + W < stop;
+        if (more) load_keys(chunk + W);
+        f16x8 weights[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float w[2][4], mx = run_max[n];
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    w[m][e] = __builtin_fmaf(st[n][m][e], row_scale[n] * ksc[m], vex[m]);
+                    if (slot0 + 16 * m + 4 * h + e > last[n]) w[m][e] = -__builtin_inff();
+                    mx = fmaxf(mx, w[m][e]);
+                }
+            mx = row_pair_max(mx);
+            const float base = mx == -__builtin_inff() ? 0.0f : mx;   // no slot of the row seen yet
+            const float rescale = __builtin_amdgcn_exp2f(run_max[n] - base);
+            run_max[n] = mx;
+            float sum[2] = {0.0f, 0.0f};
+            u32x4 packed;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(w[m][e] - base);
+                    sum[m] += p[e];
+                }
+                packed[2 * m] = as_u32((f16x2){(f16)p[0], (f16)p[1]});
+                packed[2 * m + 1] = as_u32((f16x2){(f16)p[2], (f16)p[3]});
+            }
+            weights[n] = __builtin_bit_cast(f16x8, packed);
+            run_sum[n] = run_sum[n] * rescale + (sum[0] * vinv[0] + sum[1] * vinv[1]);
+            if (__any(rescale != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) acc[n][i] *= rescale;
+            }
+        }
+        if (slot0 + 32 > end) {   // rows behind the last slot may hold anything, NaN codes too
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (slot0 + 16 * (i >> 2) + 4 * h + (i & 3) >= end)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) vr[i][j] = 0;
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            uint32_t words[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) words[i] = vr[i][j];
+            f16x8 value[4];
+            transpose8<CODES>(words, value);
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    acc[n][4 * j + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[d], weights[n],
+                                                                               acc[n][4 * j + d], 0, 0, 0);
+        }
+        if (!more) break;
+        chunk += W;
+        load_values(chunk);
+    }
+
+    // the wavefronts' states joined: lane (c, h) holds row c's dims D / 16 (4 h + i) + j in acc[][j][i]
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        run_sum[n] = row_pair_sum(run_sum[n]);
+        if (h == 0) {
+            row_max[wave][16 * n + c] = run_max[n];
+            row_sum[wave][16 * n + c] = run_sum[n];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float top = row_max[0][16 * n + c];
+#pragma unroll
+        for (int w = 1; w < W; ++w) top = fmaxf(top, row_max[w][16 * n + c]);
+        const float own = run_max[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(run_max[n] - top);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+            if (n + part > 0) __syncthreads();   // the previous values are read
+#pragma unroll
+            for (int i = 0; i < 4 / PARTS; ++i)
+#pragma unroll
+                for (int j = 0; j < D / 16; j += 4) {
+                    const int e = part * (4 / PARTS) + i;
+                    *reinterpret_cast<f32x4*>(&joined[wave][c][(D / 16) * ((4 / PARTS) * h + i) + j]) =
+                        (f32x4){acc[n][j][e], acc[n][j + 1][e], acc[n][j + 2][e], acc[n][j + 3][e]} * own;
+                }
+            __syncthreads();
+            for (int x = threadIdx.x; x < 16 * DP / 4; x += 64 * W) {
+                const int row = x / (DP / 4), col = 4 * (x - row * (DP / 4));
+                const int r = row0 + 16 * n + row;
+                if (r >= rows) continue;
+                f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+                float t0 = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) t0 = fmaxf(t0, row_max[w][16 * n + row]);
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    o += *reinterpret_cast<const f32x4*>(&joined[w][row][col]);
+                    const float m = row_max[w][16 * n + row];
+                    l += m == -__builtin_inff() ? 0.0f : row_sum[w][16 * n + row] * __builtin_amdgcn_exp2f(m - t0);
+                }
+                // the column in `joined` -> the head's dim (256 dims come in two parts)
+                const int q = col / (D / 16), dim = PARTS == 1 ? col
+                    : (D / 16) * (4 * (q / (4 / PARTS)) + part * (4 / PARTS) + q % (4 / PARTS)) + col % (D / 16);
+                const int t = r / a.group, g = r - t * a.group;
+                const int64_t at = ((int64_t)b * a.tokens + t) * a.heads + hk * a.group + g;
+                if (a.splits > 1) {
+                    const int64_t sp = at * a.splits + split;
+                    *reinterpret_cast<f32x4*>(a.partial + sp * D + dim) = o;
+                    if (col == 0 && part == 0) a.states[sp] = make_float2(t0, l);
+                    continue;
+                }
+                const int64_t p = seen.start + t;
+                float inv = 1.0f / l;
+                if (t >= seen.count) {
+                    o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+                    inv = 0.0f;
+                } else if (p < 0 || p >= a.slots) {
+                    inv = __builtin_nanf("");
+                }
+                store4<TYPE>(a.out + at * D + dim, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+            }
+        }
+    }
+}
+
+// The shares of each output row joined, a wavefront a row: out = sum_s acc_s
+// 2^(R_s - R) / sum_s l_s 2^(R_s - R). Lane s holds share s's state (at most
+// 64 shares); a share without slots has R = -inf and drops out.
+template <int D, int TYPE>
+__global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, int64_t rows) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t bt = row / a.heads;
+    const int b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens);
+    const Seen seen = seen_of(a, b);
+    const int64_t p = seen.start + t;
+    constexpr int E = D / 64;   // dims a lane
+    float o[E] = {};
+    float inv = 0.0f;
+    if (t < seen.count && p >= 0 && p < a.slots) {
+        float2 state = make_float2(-__builtin_inff(), 0.0f);
+        if (lane < a.splits) state = a.states[row * a.splits + lane];
+        const float top = wave_max(state.x);
+        const float f = state.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.x - top);
+        inv = 1.0f / wave_sum(state.y * f);
+        const float* part = a.partial + row * a.splits * D + lane * E;
+        for (int s = 0; s < a.splits; ++s) {
+            const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
+            if (fs == 0.0f) continue;   // nothing was written there
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(part[(int64_t)s * D + e], fs, o[e]);
+        }
+    } else if (t < seen.count) {
+        inv = __builtin_nanf("");
+    }
+    uint16_t* out = a.out + row * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = (uint16_t)narrow16<TYPE>(o[e] * inv);
+}
+
+// ---------------------------------------------------------------------------
+// Prompt form: 128 query rows of a KV head a workgroup, 32 a wavefront.
+//
+// Bound: the matrix cores and the softmax's vector instructions (4 dim flops
+// a pair of row and slot). Tiles of 8192 / dim slots: their codes are
+// requested into registers while the tile before is multiplied, decoded to
+// fp16 once for the workgroup's rows and kept in LDS, keys row by row, values
+// transposed with their slots in the order of the score registers.
+// v_mfma_f32_32x32x16_f16: lane (n, h) = (lane & 31, lane >> 5) receives the
+// scores of row n for slots 8 (i >> 2) + 4 h + (i & 3) of each 32.
+// ---------------------------------------------------------------------------
+constexpr int kPromptWaves = 4;
+constexpr int kPromptRows = 32 * kPromptWaves;
+
+template <int D, int CODES, int TYPE>
+__global__ void __launch_bounds__(64 * kPromptWaves)
+prompt_kernel(const AttnArgs a) {
+    constexpr int KT = 8192 / D;        // slots of a tile
+    constexpr int KN = KT / 32;
+    constexpr int KROW = D + 8;         // fp16 values of a key row in LDS
+    constexpr int VROW = KT + 8;        // of a value dim's row
+    __shared__ __align__(16) f16 keys[KT * KROW];
+    __shared__ __align__(16) f16 values[D * VROW];
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int n = lane & 31, h = lane >> 5;
+    int item = blockIdx.x;
+    const int split = item % a.splits;
+    item /= a.splits;
+    const int hk = item % a.kv_heads;
+    item /= a.kv_heads;
+    // the last rows, which see the most slots, are dispatched first
+    const int tile = a.row_tiles - 1 - item % a.row_tiles, b = item / a.row_tiles;
+    const int rows = a.tokens * a.group, row0 = tile * kPromptRows;
+
+    const Seen seen = seen_of(a, b);
+    const int end = seen_end(a, seen, row0, kPromptRows);
+    const int last_slot = max(end - 1, 0);
+    const int tiles = (end + KT - 1) / KT;
+    const int share = (tiles + a.splits - 1) / a.splits;
+    const int first = split * share, stop = min(tiles, first + share);
+
+    const int r = min(row0 + 32 * wave + n, rows - 1);
+    const int t = r / a.group, g = r - t * a.group;
+    u32x4 qr[D / 16];
+    {
+        const uint16_t* q = a.q + b * a.qb + t * a.qt + (hk * a.group + g) * a.qh;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) qr[s] = load8(q + 16 * s + 8 * h, a.vec);
+    }
+    const int64_t p = seen.start + t;
+    const bool inside = t < seen.count && p >= 0 && p < a.slots;
+    const int last = inside ? (int)p : -1;
+    // slots past wave_end are hidden from all rows of the wavefront; up to wave_all no row needs a mask
+    const int wave_end = seen_end(a, seen, row0 + 32 * wave, 32);
+    const int first_t = min(row0 + 32 * wave, rows - 1) / a.group;
+    const int64_t p_first = seen.start + first_t;
+    const bool all_inside = row0 + 32 * wave + 32 <= rows && min(row0 + 32 * wave + 31, rows - 1) / a.group < seen.count &&
+                            p_first >= 0;
+    const int wave_all = all_inside ? (int)min(p_first, a.slots - 1) + 1 : 0;
+
+    const uint8_t* kc = a.k_codes + b * a.kb + hk * a.kh;
+    const uint8_t* vc = a.v_codes + b * a.vb + hk * a.vh;
+    const float* ks = a.k_scales + b * a.ksb + hk * a.ksh;
+    const float* vs = a.v_scales + b * a.vsb + hk * a.vsh;
+
+    u32x4 kr[2];
+    uint32_t vr[8];
+    const int vgroup = threadIdx.x / (D / 4), vdim = threadIdx.x % (D / 4);   // 8 slots, 4 dims of the values
+    auto load_tile = [&](int tile_at) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int u = threadIdx.x + 256 * i;
+            const int row = min(tile_at * KT + u / (D / 16), last_slot);
+            kr[i] = *reinterpret_cast<const u32x4*>(kc + (int64_t)row * D + 16 * (u % (D / 16)));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int slot = tile_at * KT + 16 * (vgroup >> 1) + 8 * (i >> 2) + 4 * (vgroup & 1) + (i & 3);
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(vc + (int64_t)min(slot, last_slot) * D + 4 * vdim);
+            vr[i] = slot < end ? v : 0u;   // rows behind the last slot may hold anything
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int u = threadIdx.x + 256 * i;
+            f16x8* dst = reinterpret_cast<f16x8*>(keys + (u / (D / 16)) * KROW + 16 * (u % (D / 16)));
+            dst[0] = decode8<CODES>(kr[i][0], kr[i][1]);
+            dst[1] = decode8<CODES>(kr[i][2], kr[i][3]);
+        }
+        f16x8 value[4];
+        transpose8<CODES>(vr, value);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+            *reinterpret_cast<f16x8*>(values + (4 * vdim + d) * VROW + 8 * vgroup) = value[d];
+    };
+    load_tile(first);   // rows are clamped: no register is left undefined where there is no tile
+    const float row_scale = a.scale * kLog2e * query_to_f16<TYPE>(qr, [](float v) {
+        const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
+                                                        __builtin_bit_cast(uint32_t, v), false, false);
+        return fmaxf(__builtin_bit_cast(float, (uint32_t)x[0]), __builtin_bit_cast(float, (uint32_t)x[1]));
+    });
+    float run_max = -__builtin_inff(), run_sum = 0.0f;
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+
+    for (int at = first; at < stop; ++at) {
+        const int slot0 = at * KT;
+        if (at > first) __syncthreads();   // the tile before is used
+        stage();
+        __syncthreads();
+        if (at + 1 < stop) load_tile(at + 1);
+        if (slot0 >= wave_end) continue;   // every wavefront meets the same barriers
+        f32x16 st[KN];
+        float mx = run_max;
+        float vinv[KN][2], vex[KN][2];
+#pragma unroll
+        for (int k = 0; k < KN; ++k) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st[k][i] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s)
+                st[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    *reinterpret_cast<const f16x8*>(keys + (32 * k + n) * KROW + 16 * s + 8 * h),
+                    __builtin_bit_cast(f16x8, qr[s]), st[k], 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < KN; ++k) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int blk = min(slot0 + 32 * k + 16 * x, last_slot) >> a.block_log;
+                const int e = exponent_of(vs[blk]);
+                const float mul = row_scale * ks[blk];
+                vex[k][x] = (float)e;
+                vinv[k][x] = exp2_int(-e);
+#pragma unroll
+                for (int i = 8 * x; i < 8 * x + 8; ++i) st[k][i] = __builtin_fmaf(st[k][i], mul, vex[k][x]);
+            }
+        }
+        if (slot0 + KT > wave_all) {
+#pragma unroll
+            for (int k = 0; k < KN; ++k)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (slot0 + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3) > last) st[k][i] = -__builtin_inff();
+        }
+#pragma unroll
+        for (int k = 0; k < KN; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[k][i]);
+        {
+            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
+                                                            __builtin_bit_cast(uint32_t, mx), false, false);
+            mx = fmaxf(__builtin_bit_cast(float, (uint32_t)x[0]), __builtin_bit_cast(float, (uint32_t)x[1]));
+        }
+        const float base = mx == -__builtin_inff() ? 0.0f : mx;
+        const float rescale = __builtin_amdgcn_exp2f(run_max - base);
+        run_max = mx;
+        f16x8 weights[KN][2];
+        float total = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KN; ++k)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float sum = 0.0f;
+                u32x4 packed;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float lo = __builtin_amdgcn_exp2f(st[k][8 * x + 2 * i] - base);
+                    const float hi = __builtin_amdgcn_exp2f(st[k][8 * x + 2 * i + 1] - base);
+                    sum += lo + hi;
+                    packed[i] = as_u32((f16x2){(f16)lo, (f16)hi});
+                }
+                weights[k][x] = __builtin_bit_cast(f16x8, packed);
+                total = __builtin_fmaf(sum, vinv[k][x], total);
+            }
+        run_sum = __builtin_fmaf(run_sum, rescale, total);
+        if (__any(rescale != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) acc[d] *= rescale;
+        }
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int k = 0; k < KN; ++k)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                        *reinterpret_cast<const f16x8*>(values + (32 * d + n) * VROW + 32 * k + 16 * x + 8 * h),
+                        weights[k][x], acc[d], 0, 0, 0);
+    }
+
+    if (row0 + 32 * wave + n >= rows) return;
+    {
+        const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, run_sum),
+                                                        __builtin_bit_cast(uint32_t, run_sum), false, false);
+        run_sum = __builtin_bit_cast(float, (uint32_t)x[0]) + __builtin_bit_cast(float, (uint32_t)x[1]);
+    }
+    const int64_t at = ((int64_t)b * a.tokens + t) * a.heads + hk * a.group + g;
+    if (a.splits > 1) {
+        const int64_t sp = at * a.splits + split;
+        if (h == 0) a.states[sp] = make_float2(run_max, run_sum);
+        float* o = a.partial + sp * D + 4 * h;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f32x4*>(o + 32 * d + 2 * i) =
+                    (f32x4){acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+        return;
+    }
+    const bool padding = t >= seen.count;
+    const float inv = padding ? 0.0f : inside ? 1.0f / run_sum : __builtin_nanf("");
+    uint16_t* o = a.out + at * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = padding ? 0.0f : acc[d][i + e] * inv;
+            store4<TYPE>(o + 32 * d + 2 * i, v[0], v[1], v[2], v[3]);
+        }
+}
+
+}  // namespace w4a16
+
+namespace {
+
+using namespace w4a16;
+using w4a16_internal::kv_fail;
+
+// How a call is launched: the form, the rows of a workgroup, the shares of the slots.
+struct AttnPlan {
+    bool prompt;
+    int column_tiles;   // NT of the decode form
+    int64_t row_tiles;
+    int splits;
+};
+
+constexpr int kMaxSplits = 64;
+
+AttnPlan plan_attention(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t slots, int64_t dim) {
+    AttnPlan p;
+    const int64_t rows = tokens * (heads / kv_heads);
+    p.prompt = rows > 64;
+    p.column_tiles = rows <= 16 ? 1 : rows <= 32 || dim == 256 ? 2 : 4;
+    const int64_t per = p.prompt ? kPromptRows : 16 * p.column_tiles;
+    p.row_tiles = (rows + per - 1) / per;
+    // shares: until the chip is full, and none of less than 256 slots
+    const int64_t wanted = p.prompt ? 512 : 1024;
+    const int64_t groups = batch * kv_heads * p.row_tiles;
+    int64_t splits = (wanted + groups - 1) / (groups > 0 ? groups : 1);
+    const int64_t most = (slots + 255) / 256;
+    if (splits > most) splits = most;
+    if (splits > kMaxSplits) splits = kMaxSplits;
+    p.splits = splits < 1 ? 1 : (int)splits;
+    return p;
+}
+
+template <int D, int CODES, int TYPE>
+void launch_attention(const AttnPlan& p, const AttnArgs& a, int64_t grid, hipStream_t st) {
+    const dim3 g((unsigned)grid);
+    if (p.prompt)
+        hipLaunchKernelGGL((prompt_kernel<D, CODES, TYPE>), g, dim3(64 * kPromptWaves), 0, st, a);
+    else if (p.column_tiles == 1)
+        hipLaunchKernelGGL((decode_kernel<D, 1, CODES, TYPE>), g, dim3(64 * kDecodeWaves), 0, st, a);
+    else if (p.column_tiles == 2)
+        hipLaunchKernelGGL((decode_kernel<D, 2, CODES, TYPE>), g, dim3(64 * kDecodeWaves), 0, st, a);
+    else if constexpr (D <= 128)
+        hipLaunchKernelGGL((decode_kernel<D, 4, CODES, TYPE>), g, dim3(64 * kDecodeWaves), 0, st, a);
+}
+
+template <int D, int TYPE>
+void launch_typed(const AttnPlan& p, const AttnArgs& a, int code_type, int64_t grid, int64_t rows, hipStream_t st) {
+    if (code_type == W4A16_KV_INT8)
+        launch_attention<D, W4A16_KV_INT8, TYPE>(p, a, grid, st);
+    else
+        launch_attention<D, W4A16_KV_FP8, TYPE>(p, a, grid, st);
+    if (a.splits > 1)
+        hipLaunchKernelGGL((merge_kernel<D, TYPE>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, rows);
+}
+
+template <int D>
+void launch_dim(const AttnPlan& p, const AttnArgs& a, int code_type, int type, int64_t grid, int64_t rows,
+                hipStream_t st) {
+    if (type == W4A16_FP16)
+        launch_typed<D, W4A16_FP16>(p, a, code_type, grid, rows, st);
+    else
+        launch_typed<D, W4A16_BF16>(p, a, code_type, grid, rows, st);
+}
+
+bool sizes_fit(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads) {
+    return batch >= 0 && tokens >= 0 && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && batch <= (1 << 24) &&
+           tokens <= (1 << 24) && heads <= (1 << 16) && tokens * (heads / kv_heads) <= (1 << 28);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t w4a16_kv_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                           int64_t slots, int64_t head_dim) {
+    if (!sizes_fit(batch, tokens, heads, kv_heads) || slots < 1 || batch == 0 || tokens == 0) return 0;
+    const AttnPlan p = plan_attention(batch, tokens, heads, kv_heads, slots, head_dim);
+    return p.splits > 1 ? batch * tokens * heads * p.splits * (4 * head_dim + 8) : 0;
+}
+
+int w4a16_kv_attention(const w4a16_kv_rows* q, void* out, int64_t tokens, int64_t heads, const w4a16_kv_cache* cache,
+                       const int64_t* start, const int64_t* counts, float scale, int type, void* workspace,
+                       int64_t workspace_bytes, void* stream) {
+    int rc = w4a16_internal::check_kv_cache(cache);
+    if (rc != W4A16_OK) return rc;
+    if (type != W4A16_FP16 && type != W4A16_BF16) return kv_fail(W4A16_ERR_CONFIG, "queries must be fp16 or bf16");
+    if (tokens < 0 || heads < 1 || heads % cache->kv_heads != 0)
+        return kv_fail(W4A16_ERR_SHAPE, "heads must be a positive multiple of the cache's KV heads");
+    if (!sizes_fit(cache->batch, tokens, heads, cache->kv_heads))
+        return kv_fail(W4A16_ERR_TOO_LARGE, "too many tokens or heads");
+    if (cache->batch == 0 || tokens == 0) return W4A16_OK;
+    if (q == nullptr || q->data == nullptr || out == nullptr || start == nullptr)
+        return kv_fail(W4A16_ERR_NULL, "q, out and start must be non-NULL");
+    if ((reinterpret_cast<uintptr_t>(q->data) & 1u) != 0 || (reinterpret_cast<uintptr_t>(out) & 15u) != 0)
+        return kv_fail(W4A16_ERR_ALIGNMENT, "q must be 2-byte and out 16-byte aligned");
+    const int64_t dim = cache->head_dim, batch = cache->batch;
+    const AttnPlan p = plan_attention(batch, tokens, heads, cache->kv_heads, cache->slots, dim);
+    const int64_t rows = batch * tokens * heads;
+    if (p.splits > 1) {
+        if (workspace == nullptr || workspace_bytes < rows * p.splits * (4 * dim + 8))
+            return kv_fail(W4A16_ERR_CONFIG, "the workspace is smaller than w4a16_kv_attention_workspace_bytes");
+        if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+            return kv_fail(W4A16_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
+    }
+    const int64_t grid = batch * cache->kv_heads * p.row_tiles * p.splits;
+    if (grid > 0x7FFFFFFF || rows / 4 > 0x7FFFFFFE) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
+    AttnArgs a{};
+    a.q = static_cast<const uint16_t*>(q->data);
+    a.out = static_cast<uint16_t*>(out);
+    a.k_codes = static_cast<const uint8_t*>(cache->k.codes);
+    a.v_codes = static_cast<const uint8_t*>(cache->v.codes);
+    a.k_scales = cache->k.scales;
+    a.v_scales = cache->v.scales;
+    a.start = start;
+    a.counts = counts;
+    // the outputs come first, so that both start on 16 bytes
+    a.partial = static_cast<float*>(workspace);
+    a.states = reinterpret_cast<float2*>(static_cast<float*>(workspace) + (p.splits > 1 ? rows * p.splits * dim : 0));
+    a.qb = q->batch_stride;
+    a.qt = q->token_stride;
+    a.qh = q->head_stride;
+    a.kb = cache->k.batch_stride;
+    a.kh = cache->k.head_stride;
+    a.vb = cache->v.batch_stride;
+    a.vh = cache->v.head_stride;
+    a.ksb = cache->k.scale_batch_stride;
+    a.ksh = cache->k.scale_head_stride;
+    a.vsb = cache->v.scale_batch_stride;
+    a.vsh = cache->v.scale_head_stride;
+    a.slots = cache->slots;
+    a.scale = scale;
+    a.tokens = (int)tokens;
+    a.heads = (int)heads;
+    a.kv_heads = (int)cache->kv_heads;
+    a.group = (int)(heads / cache->kv_heads);
+    a.block_log = cache->block == 16 ? 4 : cache->block == 32 ? 5 : cache->block == 64 ? 6 : 7;
+    a.splits = p.splits;
+    a.row_tiles = (int)p.row_tiles;
+    a.vec = (reinterpret_cast<uintptr_t>(q->data) & 15u) == 0 &&
+            ((q->batch_stride | q->token_stride | q->head_stride) & 7) == 0;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dim == 64)
+        launch_dim<64>(p, a, cache->code_type, type, grid, rows, st);
+    else if (dim == 128)
+        launch_dim<128>(p, a, cache->code_type, type, grid, rows, st);
+    else
+        launch_dim<256>(p, a, cache->code_type, type, grid, rows, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return kv_fail(W4A16_ERR_LAUNCH, std::string("kernel launch failed: ") + hipGetErrorString(e));
+    return W4A16_OK;
+}
+
+}  // extern "C"

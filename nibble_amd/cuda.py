@@ -1,5 +1,6 @@
-"""Python wrappers of the torch ops ``w4a16::linear``, ``w4a16::dequantize`` and
-``w4a16::quantize``.
+"""Python wrappers of the torch ops ``w4a16::linear``, ``w4a16::dequantize``,
+``w4a16::quantize`` and of the ops of the 8-bit key/value cache (``rotary``,
+``kv_write``, ``rotary_kv_write``, ``kv_read``, ``kv_attention``).
 
 Mirrors reference ``w4a16/cuda.py``: importing the compiled extension
 (``nibble_amd._C``, here a thin libtorch shim over the HIP C ABI) registers
@@ -43,6 +44,27 @@ if _EXTENSION_LOAD_ERROR is None:
             weights.new_empty((rows, cols // 2), dtype=torch.uint8),
             weights.new_empty((rows, cols // group_size), dtype=torch.float16),
         )
+
+    @torch.library.register_fake("w4a16::rotary")
+    def _rotary_fake(x, positions, cos, sin, interleaved=False):
+        return x.new_empty(x.shape)
+
+    @torch.library.register_fake("w4a16::kv_write")
+    def _kv_write_fake(k, v, k_codes, k_scales, v_codes, v_scales, start, counts=None):
+        return None
+
+    @torch.library.register_fake("w4a16::rotary_kv_write")
+    def _rotary_kv_write_fake(q, k, v, cos, sin, k_codes, k_scales, v_codes, v_scales, start, counts=None,
+                              interleaved=False):
+        return q.new_empty(q.shape)
+
+    @torch.library.register_fake("w4a16::kv_read")
+    def _kv_read_fake(codes, scales, dtype):
+        return codes.new_empty(codes.shape, dtype=dtype)
+
+    @torch.library.register_fake("w4a16::kv_attention")
+    def _kv_attention_fake(q, k_codes, k_scales, v_codes, v_scales, start, counts=None, scale=None):
+        return q.new_empty(q.shape)
 
 
 def cuda_extension_available() -> bool:
@@ -118,3 +140,88 @@ def quantize_cuda(weights: torch.Tensor, group_size: int = 128) -> tuple[torch.T
     two from 16 to 512, weights contiguous and 16-byte aligned."""
     _require_extension()
     return torch.ops.w4a16.quantize(weights, group_size)
+
+
+def rotary_cuda(
+    x: torch.Tensor,
+    positions: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    interleaved: bool = False,
+) -> torch.Tensor:
+    """Rotary positions on the GPU: x fp16 / bf16 [tokens, heads, head_dim] or
+    [batch, tokens, heads, head_dim] (any strides, the last dimension
+    contiguous) with its first 2 * cos.shape[1] dims rotated by the rows
+    ``positions`` (int64 [tokens] or [batch, tokens]) of the fp32 tables; the
+    other dims are copied. Pairs are dims (i, i + half), or (2i, 2i + 1) when
+    ``interleaved``. A position outside the tables gives NaN."""
+    _require_extension()
+    return torch.ops.w4a16.rotary.default(x, positions, cos, sin, interleaved)
+
+
+def kv_write_cuda(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_codes: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_codes: torch.Tensor,
+    v_scales: torch.Tensor,
+    start: torch.Tensor,
+    counts: torch.Tensor | None = None,
+) -> None:
+    """Quantizes k and v fp16 / bf16 [batch, tokens, kv_heads, head_dim] into
+    the slots start[b] .. of an 8-bit cache (codes int8 or float8_e4m3fn
+    [batch, kv_heads, slots, head_dim], power-of-two scales fp32 [batch,
+    kv_heads, blocks]; one scale for every 16, 32, 64 or 128 slots). The first
+    counts[b] tokens of a sequence are written (None: all). A block's scale
+    grows with its tokens, and its earlier codes are rescaled then."""
+    _require_extension()
+    torch.ops.w4a16.kv_write.default(k, v, k_codes, k_scales, v_codes, v_scales, start, counts)
+
+
+def rotary_kv_write_cuda(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    k_codes: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_codes: torch.Tensor,
+    v_scales: torch.Tensor,
+    start: torch.Tensor,
+    counts: torch.Tensor | None = None,
+    interleaved: bool = False,
+) -> torch.Tensor:
+    """``rotary_cuda`` of q and k at positions start[b] + t and
+    ``kv_write_cuda`` of the rotated k and of v, in one launch; returns the
+    rotated q (zeros in padding rows). The tables need a row for every slot and
+    a rotated part that is a multiple of 16."""
+    _require_extension()
+    return torch.ops.w4a16.rotary_kv_write.default(q, k, v, cos, sin, k_codes, k_scales, v_codes, v_scales, start,
+                                                   counts, interleaved)
+
+
+def kv_read_cuda(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """The values code * scale of an 8-bit cache's keys or values (or of a view
+    of its leading slots), rounded once to fp16, bf16 or fp32."""
+    _require_extension()
+    return torch.ops.w4a16.kv_read.default(codes, scales, dtype)
+
+
+def kv_attention_cuda(
+    q: torch.Tensor,
+    k_codes: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_codes: torch.Tensor,
+    v_scales: torch.Tensor,
+    start: torch.Tensor,
+    counts: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """Causal attention of q fp16 / bf16 [batch, tokens, heads, head_dim] over
+    an 8-bit cache that holds the tokens' own keys and values: token t of
+    sequence b sees the slots 0 .. start[b] + t. Rows at or past counts[b] are
+    padding and come out zero. ``scale`` defaults to head_dim ** -0.5."""
+    _require_extension()
+    return torch.ops.w4a16.kv_attention.default(q, k_codes, k_scales, v_codes, v_scales, start, counts, scale)
