@@ -30,6 +30,13 @@ a contiguous view of its rows, so state-dict keys and layouts are those of
 the per-layer modules. ``fused=False`` runs the same step as separate torch
 ops around ``QuantizedLinear`` (the reference-shaped decoder).
 
+``LlamaConfig.kv_cache`` "int8" or "fp8" keeps the keys and values in 8 bits
+(``QuantizedKVCache``): the step then rotates q and k, writes k and v
+(``rotary_kv_write``, one launch) and attends (``kv_attention``) between the
+q|k|v and the o GEMV, the prompt likewise. Half the bytes of the cache, and
+head dims 128 and 256 run the fused step, too. ``LlamaConfig.rope_scaling``
+(the Hugging Face dict) scales the rotary positions for long contexts.
+
 Prefill of a prompt runs the W4A16 op itself for every projection up to 1024
 tokens (q|k|v as one op; the op's W4A16 GEMM from 9 rows, its LDS-staged
 form from 128; up to 8 rows its small-batch kernels), gate|up as one GEMM
@@ -54,8 +61,10 @@ import torch.nn.functional as F
 
 from nibble_amd import _lib
 from nibble_amd.cuda import dequantize_cuda
+from nibble_amd.kv_cache import QuantizedKVCache
 from nibble_amd.linear import QuantizedLinear
 from nibble_amd.quantization import quantize_and_pack_weights
+from nibble_amd.rotary import rope_frequencies, rope_tables
 
 # Longest prompt the fused prefill takes where the prefill attention cannot
 # stream the caches (query heads per KV head not a power of two up to 64:
@@ -88,6 +97,9 @@ class LlamaConfig:
     max_seq_len: int = 64
     group_size: int = 128
     init_std: float = 0.02
+    kv_cache: str = "fp16"             # or "int8", "fp8": QuantizedKVCache
+    kv_block: int = 64                 # slots of a scale of an 8-bit cache
+    rope_scaling: dict | None = None   # as in Hugging Face configs (nibble_amd/rotary.py)
 
     @property
     def num_linear_layers(self) -> int:
@@ -149,9 +161,11 @@ class Block(torch.nn.Module):
             return torch.ops.w4a16.linear(x, mod.packed_weights, mod.scales, self.cfg.group_size)
         return mod(x)
 
-    def forward(self, x, cos, sin, positions, k_cache, v_cache, mask):
-        """x [T, H] fp16; positions [T] int64 (cache slots to write);
-        k_cache / v_cache [kv_heads, S, head_dim]; mask [T, S] additive fp32.
+    def forward(self, x, cos, sin, positions, k_cache, v_cache, mask, kv_cache=None):
+        """x [T, H] fp16; positions [T] int64 (cache slots to write,
+        consecutive); k_cache / v_cache [kv_heads, S, head_dim]; mask [T, S]
+        additive fp32. With kv_cache (a QuantizedKVCache) that holds the keys
+        and values, and cos / sin are the whole tables.
         With native_prefill on a GPU, prompts of up to NATIVE_PREFILL_MAX_ROWS
         tokens run q|k|v and gate|up as one W4A16 op each over the
         concatenated weights (and o, down as the op); otherwise every
@@ -169,6 +183,27 @@ class Block(torch.nn.Module):
             q = self.q_proj(h).view(t, cfg.num_heads, cfg.head_dim)
             k = self.k_proj(h).view(t, cfg.num_kv_heads, cfg.head_dim)
             v = self.v_proj(h).view(t, cfg.num_kv_heads, cfg.head_dim)
+        if kv_cache is not None:
+            q, k, v = (y.contiguous().unsqueeze(0) for y in (q, k, v))
+            start = positions[:1]
+            attn = kv_cache.attend(kv_cache.rotary_write(q, k, v, cos, sin, start), start)
+            attn = attn.reshape(t, cfg.hidden_size)
+        else:
+            attn = self._attend(q, k, v, cos, sin, positions, k_cache, v_cache, mask)
+        x = x + self._linear(self.o_proj, attn)
+        h = self.post_norm(x)
+        if self.gu_packed is not None and self._native(h, self.gu_packed):
+            gu = torch.ops.w4a16.linear(h, self.gu_packed, self.gu_scales, cfg.group_size)
+            mlp = F.silu(gu[:, : cfg.intermediate_size]) * gu[:, cfg.intermediate_size:]
+        else:
+            mlp = F.silu(self.gate_proj(h)) * self.up_proj(h)
+        x = x + self._linear(self.down_proj, mlp)
+        return x
+
+    def _attend(self, q, k, v, cos, sin, positions, k_cache, v_cache, mask):
+        """Rotary, cache write and attention over the fp16 cache, [T, H] fp16."""
+        cfg = self.cfg
+        t = q.shape[0]
         q = _rope(q, cos, sin)
         k = _rope(k, cos, sin)
         k_cache.index_copy_(1, positions, k.transpose(0, 1).contiguous())
@@ -180,16 +215,7 @@ class Block(torch.nn.Module):
         qf = q.float().transpose(0, 1).contiguous()                     # [heads, T, d]
         scores = torch.matmul(qf, kf.transpose(1, 2).contiguous()) / math.sqrt(cfg.head_dim) + mask
         attn = torch.matmul(torch.softmax(scores, dim=-1), vf)          # [heads, T, d]
-        attn = attn.transpose(0, 1).reshape(t, cfg.hidden_size).to(torch.float16)
-        x = x + self._linear(self.o_proj, attn)
-        h = self.post_norm(x)
-        if self.gu_packed is not None and self._native(h, self.gu_packed):
-            gu = torch.ops.w4a16.linear(h, self.gu_packed, self.gu_scales, cfg.group_size)
-            mlp = F.silu(gu[:, : cfg.intermediate_size]) * gu[:, cfg.intermediate_size:]
-        else:
-            mlp = F.silu(self.gate_proj(h)) * self.up_proj(h)
-        x = x + self._linear(self.down_proj, mlp)
-        return x
+        return attn.transpose(0, 1).reshape(t, cfg.hidden_size).to(torch.float16)
 
 
 def _concat_rows(modules: list[QuantizedLinear]) -> tuple[torch.Tensor, torch.Tensor]:
@@ -229,13 +255,21 @@ class LlamaDecoder(torch.nn.Module):
             raise ValueError("init must be 'random' or 'empty'")
         self.cfg = cfg
         device = torch.device(device)
+        if cfg.kv_cache not in ("fp16", "int8", "fp8"):
+            raise ValueError("kv_cache must be 'fp16', 'int8' or 'fp8'")
+        quantized = cfg.kv_cache != "fp16"
+        if quantized and device.type == "cuda" and cfg.head_dim not in (64, 128, 256):
+            raise ValueError("an 8-bit kv_cache on the GPU needs head_dim 64, 128 or 256")
+        frequencies, rope_factor = rope_frequencies(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling, cfg.max_seq_len)
         # The fused step is HIP-only (CPU runs the torch ops) and built for
-        # head_dim 64 and rows of K <= 16384.
-        self.fused = (fused and device.type == "cuda" and cfg.head_dim == 64
+        # head_dim 64 (64, 128 and 256 over an 8-bit cache) and rows of K <= 16384.
+        self.fused = (fused and device.type == "cuda" and cfg.head_dim in ((64, 128, 256) if quantized else (64,))
                       and max(cfg.hidden_size, cfg.intermediate_size) <= 16384)
         # attention + o projection as one launch (positions < 64): head layouts
         # the kernel supports
-        self.attn_o = (self.fused and fuse_attention_o and cfg.num_kv_heads in (1, 2, 4, 8)
+        # (over the fp16 cache, rotating by inv_freq alone: without a factor on the tables)
+        self.attn_o = (self.fused and fuse_attention_o and not quantized and rope_factor == 1.0
+                       and cfg.num_kv_heads in (1, 2, 4, 8)
                        and cfg.num_heads % cfg.num_kv_heads == 0 and cfg.num_heads // cfg.num_kv_heads <= 16
                        and cfg.num_heads * cfg.head_dim <= 4096 and cfg.group_size == 128)
         gen = torch.Generator(device=device).manual_seed(seed) if init == "random" else None
@@ -248,18 +282,30 @@ class LlamaDecoder(torch.nn.Module):
         self.layers = torch.nn.ModuleList([Block(cfg, device, gen) for _ in range(cfg.num_layers)])
         self.norm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps, device)
         self.lm_head = _quantized(cfg.vocab_size, cfg.hidden_size, cfg, device, gen)
-        inv_freq = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.head_dim, 2, device=device).float() / cfg.head_dim))
-        angles = torch.outer(torch.arange(cfg.max_seq_len, device=device).float(), inv_freq)
-        self.register_buffer("cos", angles.cos(), persistent=False)
-        self.register_buffer("sin", angles.sin(), persistent=False)
+        if quantized or cfg.rope_scaling is not None:
+            inv_freq = frequencies.to(device, torch.float32)
+            cos, sin = rope_tables(cfg.head_dim, cfg.max_seq_len, cfg.rope_theta, cfg.rope_scaling, device)
+        else:
+            inv_freq = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.head_dim, 2, device=device).float() / cfg.head_dim))
+            angles = torch.outer(torch.arange(cfg.max_seq_len, device=device).float(), inv_freq)
+            cos, sin = angles.cos(), angles.sin()
+        self.register_buffer("cos", cos, persistent=False)
+        self.register_buffer("sin", sin, persistent=False)
         self.register_buffer("inv_freq", inv_freq, persistent=False)
-        shape = (cfg.num_layers, cfg.num_kv_heads, cfg.max_seq_len, cfg.head_dim)
+        # the keys and values of the layers: an 8-bit cache each, or one fp16 buffer
+        self.kv_caches: list[QuantizedKVCache] | None = None
+        if quantized:
+            self.kv_caches = [QuantizedKVCache(1, cfg.num_kv_heads, cfg.max_seq_len, cfg.head_dim, cfg.kv_cache,
+                                               cfg.kv_block, device) for _ in range(cfg.num_layers)]
+        slots = 0 if quantized else cfg.max_seq_len
+        shape = (cfg.num_layers, cfg.num_kv_heads, slots, cfg.head_dim)
         self.register_buffer("k_cache", torch.zeros(shape, dtype=torch.float16, device=device), persistent=False)
         self.register_buffer("v_cache", torch.zeros(shape, dtype=torch.float16, device=device), persistent=False)
         self.slots = torch.arange(cfg.max_seq_len, device=device)
         # static decode-step state (graph inputs/outputs)
         self.token = torch.zeros((1,), dtype=torch.int64, device=device)
         self.position = torch.zeros((1,), dtype=torch.int64, device=device)
+        self.prompt_start = torch.zeros((1,), dtype=torch.int64, device=device)   # a prompt's first slot, always 0
         self.graph: torch.cuda.CUDAGraph | None = None
         self.graph_short: torch.cuda.CUDAGraph | None = None   # attention + o fused (position < 64)
         # several short steps in one graph (capture(tokens_per_replay=T)): graphs of T, T // 2, .. (> 1)
@@ -291,7 +337,7 @@ class LlamaDecoder(torch.nn.Module):
         # tok/s; up to 1024 it runs one workgroup per head as well, and does
         # not read the workspace
         self.attn_splits = (min(max(1, 256 // cfg.num_heads), max(1, cfg.max_seq_len // 128), 64)
-                            if cfg.max_seq_len > 512 else 0)
+                            if cfg.max_seq_len > 512 and not quantized else 0)
         self.attn_ws = torch.empty((max(1, cfg.num_heads * self.attn_splits * 66),), dtype=torch.float32,
                                    device=device)
         self.mlp_buf = torch.zeros((cfg.intermediate_size,), dtype=torch.float16, device=device)
@@ -306,6 +352,10 @@ class LlamaDecoder(torch.nn.Module):
     def _forward(self, tokens: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """tokens [T], positions [T] -> logits of the last position [vocab] fp16."""
         x = self.embed[tokens]
+        if self.kv_caches is not None:
+            for layer, cache in zip(self.layers, self.kv_caches):
+                x = layer(x, self.cos, self.sin, positions, None, None, None, cache)
+            return self.lm_head(self.norm(x[-1:]))[0]
         cos, sin = self.cos[positions], self.sin[positions]
         # additive mask: slot s visible to query t iff s <= positions[t]
         mask = torch.where(self.slots.unsqueeze(0) <= positions.unsqueeze(1), 0.0, float("-inf"))
@@ -318,9 +368,9 @@ class LlamaDecoder(torch.nn.Module):
         op for every projection and one launch for each RMSNorm, attention and
         SiLU-multiply (1 <= tokens <= max_seq_len; past FUSED_PREFILL_MAX_TOKENS
         only where the attention streams the caches through LDS, query heads
-        per KV head a power of two up to 64)."""
+        per KV head a power of two up to 64, or over an 8-bit cache)."""
         group = self.cfg.num_heads // self.cfg.num_kv_heads
-        streams = group & (group - 1) == 0 and group <= 64
+        streams = self.kv_caches is not None or (group & (group - 1) == 0 and group <= 64)
         limit = self.cfg.max_seq_len if streams else min(self.cfg.max_seq_len, FUSED_PREFILL_MAX_TOKENS)
         return self.fused and self.fuse_prefill and 1 <= tokens <= limit
 
@@ -369,13 +419,17 @@ class LlamaDecoder(torch.nn.Module):
             h = torch.empty_like(x)
             _lib.rmsnorm_f16(x, first.weight, first.eps, h)
         attn = (torch.empty((t, cfg.num_heads * cfg.head_dim), dtype=torch.float16, device=x.device)
-                if t > FUSED_PREFILL_NATIVE_MAX_ROWS else None)
+                if t > FUSED_PREFILL_NATIVE_MAX_ROWS and self.kv_caches is None else None)
         mlp = torch.empty((t, cfg.intermediate_size), dtype=torch.float16, device=x.device)
         for i, b in enumerate(self.layers):
             qkv_w, qkv_s = self.qkv[i]
             gu_w, gu_s = self.gate_up[i]
             qkv = self._prefill_linear(h, qkv_w, qkv_s)
-            if t <= FUSED_PREFILL_NATIVE_MAX_ROWS:
+            if self.kv_caches is not None:
+                o = self._prefill_linear(self._attend_quantized(i, qkv, self.prompt_start),
+                                         b.o_proj.packed_weights, b.o_proj.scales)
+                _lib.add_rmsnorm_f16(x, o, b.post_norm.weight, b.post_norm.eps, x, h)
+            elif t <= FUSED_PREFILL_NATIVE_MAX_ROWS:
                 # attention + o + residual add + norm (9..16 tokens: the attention inside the o op's launch)
                 _lib.prefill_attention_o_add_rmsnorm_f16(
                     qkv, self.k_cache[i], self.v_cache[i], self.cos, self.sin, 0, b.o_proj.packed_weights,
@@ -402,6 +456,17 @@ class LlamaDecoder(torch.nn.Module):
         _lib.argmax_embed_f16(self.logits, self.token, None, self.embed, self.x_buf)
         if not one_launch:
             self.position.fill_(t)
+
+    def _attend_quantized(self, layer: int, qkv: torch.Tensor, start: torch.Tensor) -> torch.Tensor:
+        """Rotary, cache write and attention of q|k|v rows [T, ..] at slots
+        start .. over the layer's 8-bit cache: [T, heads * head_dim], two or
+        three launches."""
+        cfg = self.cfg
+        rows = qkv.view(1, -1, cfg.num_heads + 2 * cfg.num_kv_heads, cfg.head_dim)
+        q, k, v = rows.split([cfg.num_heads, cfg.num_kv_heads, cfg.num_kv_heads], dim=2)
+        cache = self.kv_caches[layer]
+        q = cache.rotary_write(q, k, v, self.cos, self.sin, start)
+        return cache.attend(q, start).view(-1, cfg.num_heads * cfg.head_dim)
 
     def _prefill_linear(self, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
         """A fused-prefill projection: the W4A16 op up to
@@ -490,7 +555,10 @@ class LlamaDecoder(torch.nn.Module):
             else:
                 _lib.gemv_fused_f16(x, qkv_w, qkv_s, self.qkv_buf, norm_weight=b.input_norm.weight,
                                     eps=b.input_norm.eps)
-                if self.attn_splits:
+                attn = self.attn_buf
+                if self.kv_caches is not None:
+                    attn = self._attend_quantized(i, self.qkv_buf, self.position).view(-1)
+                elif self.attn_splits:
                     _lib.decode_attention_split_f16(self.qkv_buf, self.k_cache[i], self.v_cache[i], self.cos,
                                                     self.sin, self.position, self.attn_buf, cfg.num_heads,
                                                     cfg.num_kv_heads, self.attn_splits, self.attn_ws, cfg.head_dim)
@@ -498,7 +566,7 @@ class LlamaDecoder(torch.nn.Module):
                     _lib.decode_attention_f16(self.qkv_buf, self.k_cache[i], self.v_cache[i], self.cos, self.sin,
                                               self.position, self.attn_buf, cfg.num_heads, cfg.num_kv_heads,
                                               cfg.head_dim)
-                _lib.gemv_fused_f16(self.attn_buf, b.o_proj.packed_weights, b.o_proj.scales, x, residual=x)
+                _lib.gemv_fused_f16(attn, b.o_proj.packed_weights, b.o_proj.scales, x, residual=x)
             _lib.gemv_fused_f16(x, gu_w, gu_s, self.mlp_buf, norm_weight=b.post_norm.weight, eps=b.post_norm.eps,
                                 paired=True)
             _lib.gemv_fused_f16(self.mlp_buf, b.down_proj.packed_weights, b.down_proj.scales, x, residual=x)
@@ -558,15 +626,14 @@ class LlamaDecoder(torch.nn.Module):
         replay costs a fixed 12-16 us of GPU time: 31 tokens at T = 16 take 5
         replays). The KV cache, position and the fused step's input row are
         restored afterwards (capturing runs steps)."""
-        saved = (self.k_cache.clone(), self.v_cache.clone(), self.token.clone(), self.position.clone(),
-                 self.x_buf.clone())
+        state = [self.k_cache, self.v_cache, self.token, self.position, self.x_buf]
+        for cache in self.kv_caches or ():
+            state += cache.tensors()
+        saved = [t.clone() for t in state]
 
         def restore():
-            self.k_cache.copy_(saved[0])
-            self.v_cache.copy_(saved[1])
-            self.token.copy_(saved[2])
-            self.position.copy_(saved[3])
-            self.x_buf.copy_(saved[4])
+            for t, was in zip(state, saved):
+                t.copy_(was)
 
         self.graph = self._capture_step(False)
         restore()
