@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, int64_t ro
 }
 
 // ---------------------------------------------------------------------------
-// Prompt form: 128 query rows of a KV head a workgroup, 32 a wavefront.
+// Prompt form: 32 W query rows of a KV head a workgroup of W wavefronts.
 //
 // Bound: the matrix cores and the softmax's vector instructions (4 dim flops
 // a pair of row and slot). Tiles of 8192 / dim slots: their codes are
@@ -453,16 +453,26 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, int64_t ro
 // v_mfma_f32_32x32x16_f16: lane (n, h) = (lane & 31, lane >> 5) receives the
 // scores of row n for slots 8 (i >> 2) + 4 h + (i & 3) of each 32.
 // ---------------------------------------------------------------------------
-constexpr int kPromptWaves = 4;
-constexpr int kPromptRows = 32 * kPromptWaves;
+__device__ __forceinline__ float half_pair_max(float v) {   // over lanes l and l ^ 32
+    const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
+                                                    false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)x[0]), __builtin_bit_cast(float, (uint32_t)x[1]));
+}
+__device__ __forceinline__ float half_pair_sum(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
+                                                    false, false);
+    return __builtin_bit_cast(float, (uint32_t)x[0]) + __builtin_bit_cast(float, (uint32_t)x[1]);
+}
 
-template <int D, int CODES, int TYPE>
-__global__ void __launch_bounds__(64 * kPromptWaves)
+template <int D, int W, int CODES, int TYPE>
+__global__ void __launch_bounds__(64 * W, 2)
 prompt_kernel(const AttnArgs a) {
     constexpr int KT = 8192 / D;        // slots of a tile
     constexpr int KN = KT / 32;
     constexpr int KROW = D + 8;         // fp16 values of a key row in LDS
     constexpr int VROW = KT + 8;        // of a value dim's row
+    constexpr int KL = 512 / (64 * W);  // 16-byte units of keys a thread loads
+    constexpr int VT = 256;             // threads that load values
     __shared__ __align__(16) f16 keys[KT * KROW];
     __shared__ __align__(16) f16 values[D * VROW];
 
@@ -476,16 +486,16 @@ prompt_kernel(const AttnArgs a) {
     item /= a.kv_heads;
     // the last rows, which see the most slots, are dispatched first
     const int tile = a.row_tiles - 1 - item % a.row_tiles, b = item / a.row_tiles;
-    const int rows = a.tokens * a.group, row0 = tile * kPromptRows;
+    const int rows = a.tokens * a.group, row0 = tile * 32 * W, wave0 = row0 + 32 * wave;
 
     const Seen seen = seen_of(a, b);
-    const int end = seen_end(a, seen, row0, kPromptRows);
+    const int end = seen_end(a, seen, row0, 32 * W);
     const int last_slot = max(end - 1, 0);
     const int tiles = (end + KT - 1) / KT;
     const int share = (tiles + a.splits - 1) / a.splits;
     const int first = split * share, stop = min(tiles, first + share);
 
-    const int r = min(row0 + 32 * wave + n, rows - 1);
+    const int r = min(wave0 + n, rows - 1);
     const int t = r / a.group, g = r - t * a.group;
     u32x4 qr[D / 16];
     {
@@ -496,12 +506,10 @@ prompt_kernel(const AttnArgs a) {
     const int64_t p = seen.start + t;
     const bool inside = t < seen.count && p >= 0 && p < a.slots;
     const int last = inside ? (int)p : -1;
-    // slots past wave_end are hidden from all rows of the wavefront; up to wave_all no row needs a mask
-    const int wave_end = seen_end(a, seen, row0 + 32 * wave, 32);
-    const int first_t = min(row0 + 32 * wave, rows - 1) / a.group;
-    const int64_t p_first = seen.start + first_t;
-    const bool all_inside = row0 + 32 * wave + 32 <= rows && min(row0 + 32 * wave + 31, rows - 1) / a.group < seen.count &&
-                            p_first >= 0;
+    // slots from wave_end on are hidden from all rows of the wavefront; below wave_all no row needs a mask
+    const int wave_end = seen_end(a, seen, wave0, 32);
+    const int64_t p_first = seen.start + min(wave0, rows - 1) / a.group;
+    const bool all_inside = wave0 + 32 <= rows && (wave0 + 31) / a.group < seen.count && p_first >= 0;
     const int wave_all = all_inside ? (int)min(p_first, a.slots - 1) + 1 : 0;
 
     const uint8_t* kc = a.k_codes + b * a.kb + hk * a.kh;
@@ -509,43 +517,64 @@ prompt_kernel(const AttnArgs a) {
     const float* ks = a.k_scales + b * a.ksb + hk * a.ksh;
     const float* vs = a.v_scales + b * a.vsb + hk * a.vsh;
 
-    u32x4 kr[2];
+    u32x4 kr[KL];
     uint32_t vr[8];
-    const int vgroup = threadIdx.x / (D / 4), vdim = threadIdx.x % (D / 4);   // 8 slots, 4 dims of the values
+    float k_scale[2 * KN], v_scale[2 * KN];
+    const int vt = threadIdx.x % VT;
+    const int vgroup = vt / (D / 4), vdim = vt % (D / 4);   // 8 slots, 4 dims of the values
+    const bool loads_values = W == 4 || wave >= W - 4;
     auto load_tile = [&](int tile_at) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int u = threadIdx.x + 256 * i;
+        for (int i = 0; i < KL; ++i) {
+            const int u = threadIdx.x + 64 * W * i;
             const int row = min(tile_at * KT + u / (D / 16), last_slot);
             kr[i] = *reinterpret_cast<const u32x4*>(kc + (int64_t)row * D + 16 * (u % (D / 16)));
         }
+        if (loads_values) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int slot = tile_at * KT + 16 * (vgroup >> 1) + 8 * (i >> 2) + 4 * (vgroup & 1) + (i & 3);
-            const uint32_t v = *reinterpret_cast<const uint32_t*>(vc + (int64_t)min(slot, last_slot) * D + 4 * vdim);
-            vr[i] = slot < end ? v : 0u;   // rows behind the last slot may hold anything
+            for (int i = 0; i < 8; ++i) {
+                const int slot = tile_at * KT + 16 * (vgroup >> 1) + 8 * (i >> 2) + 4 * (vgroup & 1) + (i & 3);
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(vc + (int64_t)min(slot, last_slot) * D + 4 * vdim);
+                vr[i] = slot < end ? v : 0u;   // rows behind the last slot may hold anything
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 2 * KN; ++x) {
+            const int blk = min(tile_at * KT + 16 * x, last_slot) >> a.block_log;
+            k_scale[x] = ks[blk];
+            v_scale[x] = vs[blk];
         }
     };
     auto stage = [&]() {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int u = threadIdx.x + 256 * i;
+        for (int i = 0; i < KL; ++i) {
+            const int u = threadIdx.x + 64 * W * i;
             f16x8* dst = reinterpret_cast<f16x8*>(keys + (u / (D / 16)) * KROW + 16 * (u % (D / 16)));
             dst[0] = decode8<CODES>(kr[i][0], kr[i][1]);
             dst[1] = decode8<CODES>(kr[i][2], kr[i][3]);
         }
-        f16x8 value[4];
-        transpose8<CODES>(vr, value);
+        if (loads_values) {
+            f16x8 value[4];
+            transpose8<CODES>(vr, value);
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
-            *reinterpret_cast<f16x8*>(values + (4 * vdim + d) * VROW + 8 * vgroup) = value[d];
+            for (int d = 0; d < 4; ++d)
+                *reinterpret_cast<f16x8*>(values + (4 * vdim + d) * VROW + 8 * vgroup) = value[d];
+        }
     };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vr[i] = 0;
     load_tile(first);   // rows are clamped: no register is left undefined where there is no tile
-    const float row_scale = a.scale * kLog2e * query_to_f16<TYPE>(qr, [](float v) {
-        const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v),
-                                                        __builtin_bit_cast(uint32_t, v), false, false);
-        return fmaxf(__builtin_bit_cast(float, (uint32_t)x[0]), __builtin_bit_cast(float, (uint32_t)x[1]));
-    });
+    float row_scale = a.scale * kLog2e * query_to_f16<TYPE>(qr, half_pair_max);
+    // the largest score of a block is that of its largest product, and a masked
+    // one stays -inf: a negative scale goes to q, and a factor too small to keep
+    // its product with a scale of 2^-40 normal is raised (it makes scores of
+    // 2^-10 at most of what it would have made smaller still)
+    if (a.scale < 0.0f) {
+        row_scale = -row_scale;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) qr[s] ^= 0x80008000u;
+    }
+    row_scale = fmaxf(row_scale, 0x1p-80f);
     float run_max = -__builtin_inff(), run_sum = 0.0f;
     f32x16 acc[D / 32];
 #pragma unroll
@@ -557,12 +586,18 @@ prompt_kernel(const AttnArgs a) {
         const int slot0 = at * KT;
         if (at > first) __syncthreads();   // the tile before is used
         stage();
+        float mul[2 * KN], vex[2 * KN], vinv[2 * KN];
+#pragma unroll
+        for (int x = 0; x < 2 * KN; ++x) {
+            const int e = exponent_of(v_scale[x]);
+            mul[x] = row_scale * k_scale[x];
+            vex[x] = (float)e;
+            vinv[x] = exp2_int(-e);
+        }
         __syncthreads();
         if (at + 1 < stop) load_tile(at + 1);
         if (slot0 >= wave_end) continue;   // every wavefront meets the same barriers
         f32x16 st[KN];
-        float mx = run_max;
-        float vinv[KN][2], vex[KN][2];
 #pragma unroll
         for (int k = 0; k < KN; ++k) {
 #pragma unroll
@@ -573,19 +608,6 @@ prompt_kernel(const AttnArgs a) {
                     *reinterpret_cast<const f16x8*>(keys + (32 * k + n) * KROW + 16 * s + 8 * h),
                     __builtin_bit_cast(f16x8, qr[s]), st[k], 0, 0, 0);
         }
-#pragma unroll
-        for (int k = 0; k < KN; ++k) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int blk = min(slot0 + 32 * k + 16 * x, last_slot) >> a.block_log;
-                const int e = exponent_of(vs[blk]);
-                const float mul = row_scale * ks[blk];
-                vex[k][x] = (float)e;
-                vinv[k][x] = exp2_int(-e);
-#pragma unroll
-                for (int i = 8 * x; i < 8 * x + 8; ++i) st[k][i] = __builtin_fmaf(st[k][i], mul, vex[k][x]);
-            }
-        }
         if (slot0 + KT > wave_all) {
 #pragma unroll
             for (int k = 0; k < KN; ++k)
@@ -593,36 +615,37 @@ prompt_kernel(const AttnArgs a) {
                 for (int i = 0; i < 16; ++i)
                     if (slot0 + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3) > last) st[k][i] = -__builtin_inff();
         }
+        float mx = run_max;
 #pragma unroll
-        for (int k = 0; k < KN; ++k)
+        for (int x = 0; x < 2 * KN; ++x) {
+            float top = st[x >> 1][8 * (x & 1)];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[k][i]);
-        {
-            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
-                                                            __builtin_bit_cast(uint32_t, mx), false, false);
-            mx = fmaxf(__builtin_bit_cast(float, (uint32_t)x[0]), __builtin_bit_cast(float, (uint32_t)x[1]));
+            for (int i = 1; i < 8; ++i) top = fmaxf(top, st[x >> 1][8 * (x & 1) + i]);
+            mx = fmaxf(mx, __builtin_fmaf(top, mul[x], vex[x]));
         }
+        mx = half_pair_max(mx);
         const float base = mx == -__builtin_inff() ? 0.0f : mx;
         const float rescale = __builtin_amdgcn_exp2f(run_max - base);
         run_max = mx;
         f16x8 weights[KN][2];
         float total = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KN; ++k)
+        for (int x = 0; x < 2 * KN; ++x) {
+            const float shift = vex[x] - base;
+            float sum = 0.0f;
+            u32x4 packed;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float sum = 0.0f;
-                u32x4 packed;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float lo = __builtin_amdgcn_exp2f(st[k][8 * x + 2 * i] - base);
-                    const float hi = __builtin_amdgcn_exp2f(st[k][8 * x + 2 * i + 1] - base);
-                    sum += lo + hi;
-                    packed[i] = as_u32((f16x2){(f16)lo, (f16)hi});
-                }
-                weights[k][x] = __builtin_bit_cast(f16x8, packed);
-                total = __builtin_fmaf(sum, vinv[k][x], total);
+            for (int i = 0; i < 4; ++i) {
+                const float lo = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x >> 1][8 * (x & 1) + 2 * i], mul[x], shift));
+                const float hi = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x >> 1][8 * (x & 1) + 2 * i + 1], mul[x], shift));
+                // summed before the rounding: where values differ in scale, fp16 drops small
+                // weights of small values that hold most of the sum
+                sum += lo + hi;
+                packed[i] = as_u32((f16x2){(f16)lo, (f16)hi});
             }
+            weights[x >> 1][x & 1] = __builtin_bit_cast(f16x8, packed);
+            total = __builtin_fmaf(sum, vinv[x], total);
+        }
         run_sum = __builtin_fmaf(run_sum, rescale, total);
         if (__any(rescale != 1.0f)) {
 #pragma unroll
@@ -639,12 +662,8 @@ prompt_kernel(const AttnArgs a) {
                         weights[k][x], acc[d], 0, 0, 0);
     }
 
-    if (row0 + 32 * wave + n >= rows) return;
-    {
-        const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, run_sum),
-                                                        __builtin_bit_cast(uint32_t, run_sum), false, false);
-        run_sum = __builtin_bit_cast(float, (uint32_t)x[0]) + __builtin_bit_cast(float, (uint32_t)x[1]);
-    }
+    if (wave0 + n >= rows) return;
+    run_sum = half_pair_sum(run_sum);
     const int64_t at = ((int64_t)b * a.tokens + t) * a.heads + hk * a.group + g;
     if (a.splits > 1) {
         const int64_t sp = at * a.splits + split;
@@ -688,13 +707,14 @@ struct AttnPlan {
 };
 
 constexpr int kMaxSplits = 64;
+constexpr int kPromptWaves = 8;
 
 AttnPlan plan_attention(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t slots, int64_t dim) {
     AttnPlan p;
     const int64_t rows = tokens * (heads / kv_heads);
     p.prompt = rows > 64;
     p.column_tiles = rows <= 16 ? 1 : rows <= 32 || dim == 256 ? 2 : 4;
-    const int64_t per = p.prompt ? kPromptRows : 16 * p.column_tiles;
+    const int64_t per = p.prompt ? 32 * kPromptWaves : 16 * p.column_tiles;
     p.row_tiles = (rows + per - 1) / per;
     // shares: until the chip is full, and none of less than 256 slots
     const int64_t wanted = p.prompt ? 512 : 1024;
@@ -711,7 +731,7 @@ template <int D, int CODES, int TYPE>
 void launch_attention(const AttnPlan& p, const AttnArgs& a, int64_t grid, hipStream_t st) {
     const dim3 g((unsigned)grid);
     if (p.prompt)
-        hipLaunchKernelGGL((prompt_kernel<D, CODES, TYPE>), g, dim3(64 * kPromptWaves), 0, st, a);
+        hipLaunchKernelGGL((prompt_kernel<D, kPromptWaves, CODES, TYPE>), g, dim3(64 * kPromptWaves), 0, st, a);
     else if (p.column_tiles == 1)
         hipLaunchKernelGGL((decode_kernel<D, 1, CODES, TYPE>), g, dim3(64 * kDecodeWaves), 0, st, a);
     else if (p.column_tiles == 2)
