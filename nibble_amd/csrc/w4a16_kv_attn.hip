@@ -473,8 +473,8 @@ prompt_kernel(const AttnArgs a) {
     constexpr int VROW = KT + 8;        // of a value dim's row
     constexpr int KL = 512 / (64 * W);  // 16-byte units of keys a thread loads
     constexpr int VT = 256;             // threads that load values
-    __shared__ __align__(16) f16 keys[KT * KROW];
-    __shared__ __align__(16) f16 values[D * VROW];
+    __shared__ __align__(16) f16 keys[2][KT * KROW];
+    __shared__ __align__(16) f16 values[2][D * VROW];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
@@ -519,51 +519,52 @@ prompt_kernel(const AttnArgs a) {
 
     u32x4 kr[KL];
     uint32_t vr[8];
-    float k_scale[2 * KN], v_scale[2 * KN];
     const int vt = threadIdx.x % VT;
     const int vgroup = vt / (D / 4), vdim = vt % (D / 4);   // 8 slots, 4 dims of the values
     const bool loads_values = W == 4 || wave >= W - 4;
-    auto load_tile = [&](int tile_at) {
+    // rows are clamped: tiles past the last one read its last row again
+    auto load_keys = [&](int tile_at) {
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int u = threadIdx.x + 64 * W * i;
             const int row = min(tile_at * KT + u / (D / 16), last_slot);
             kr[i] = *reinterpret_cast<const u32x4*>(kc + (int64_t)row * D + 16 * (u % (D / 16)));
         }
-        if (loads_values) {
+    };
+    auto load_values = [&](int tile_at) {
+        if (!loads_values) return;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int slot = tile_at * KT + 16 * (vgroup >> 1) + 8 * (i >> 2) + 4 * (vgroup & 1) + (i & 3);
-                const uint32_t v = *reinterpret_cast<const uint32_t*>(vc + (int64_t)min(slot, last_slot) * D + 4 * vdim);
-                vr[i] = slot < end ? v : 0u;   // rows behind the last slot may hold anything
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < 2 * KN; ++x) {
-            const int blk = min(tile_at * KT + 16 * x, last_slot) >> a.block_log;
-            k_scale[x] = ks[blk];
-            v_scale[x] = vs[blk];
+        for (int i = 0; i < 8; ++i) {
+            const int slot = tile_at * KT + 16 * (vgroup >> 1) + 8 * (i >> 2) + 4 * (vgroup & 1) + (i & 3);
+            vr[i] = *reinterpret_cast<const uint32_t*>(vc + (int64_t)min(slot, last_slot) * D + 4 * vdim);
         }
     };
-    auto stage = [&]() {
+    auto stage_keys = [&](f16* to) {
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int u = threadIdx.x + 64 * W * i;
-            f16x8* dst = reinterpret_cast<f16x8*>(keys + (u / (D / 16)) * KROW + 16 * (u % (D / 16)));
+            f16x8* dst = reinterpret_cast<f16x8*>(to + (u / (D / 16)) * KROW + 16 * (u % (D / 16)));
             dst[0] = decode8<CODES>(kr[i][0], kr[i][1]);
             dst[1] = decode8<CODES>(kr[i][2], kr[i][3]);
         }
-        if (loads_values) {
-            f16x8 value[4];
-            transpose8<CODES>(vr, value);
+    };
+    auto stage_values = [&](f16* to, int tile_at) {
+        if (!loads_values) return;
+        if ((tile_at + 1) * KT > end) {   // rows behind the last slot may hold anything
 #pragma unroll
-            for (int d = 0; d < 4; ++d)
-                *reinterpret_cast<f16x8*>(values + (4 * vdim + d) * VROW + 8 * vgroup) = value[d];
+            for (int i = 0; i < 8; ++i)
+                if (tile_at * KT + 16 * (vgroup >> 1) + 8 * (i >> 2) + 4 * (vgroup & 1) + (i & 3) >= end) vr[i] = 0;
         }
+        f16x8 value[4];
+        transpose8<CODES>(vr, value);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+            *reinterpret_cast<f16x8*>(to + (4 * vdim + d) * VROW + 8 * vgroup) = value[d];
     };
 #pragma unroll
     for (int i = 0; i < 8; ++i) vr[i] = 0;
-    load_tile(first);   // rows are clamped: no register is left undefined where there is no tile
+    load_keys(first);
+    load_values(first);
     float row_scale = a.scale * kLog2e * query_to_f16<TYPE>(qr, half_pair_max);
     // the largest score of a block is that of its largest product, and a masked
     // one stays -inf: a negative scale goes to q, and a factor too small to keep
@@ -582,84 +583,106 @@ prompt_kernel(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
 
-    for (int at = first; at < stop; ++at) {
-        const int slot0 = at * KT;
-        if (at > first) __syncthreads();   // the tile before is used
-        stage();
-        float mul[2 * KN], vex[2 * KN], vinv[2 * KN];
-#pragma unroll
-        for (int x = 0; x < 2 * KN; ++x) {
-            const int e = exponent_of(v_scale[x]);
-            mul[x] = row_scale * k_scale[x];
-            vex[x] = (float)e;
-            vinv[x] = exp2_int(-e);
-        }
-        __syncthreads();
-        if (at + 1 < stop) load_tile(at + 1);
-        if (slot0 >= wave_end) continue;   // every wavefront meets the same barriers
-        f32x16 st[KN];
+    auto products = [&](f16x8 (&q)[D / 16], const f16* from, f32x16 (&to)[KN]) {   // scores of a tile
 #pragma unroll
         for (int k = 0; k < KN; ++k) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) st[k][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) to[k][i] = 0.0f;
 #pragma unroll
             for (int s = 0; s < D / 16; ++s)
-                st[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    *reinterpret_cast<const f16x8*>(keys + (32 * k + n) * KROW + 16 * s + 8 * h),
-                    __builtin_bit_cast(f16x8, qr[s]), st[k], 0, 0, 0);
+                to[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    *reinterpret_cast<const f16x8*>(from + (32 * k + n) * KROW + 16 * s + 8 * h), q[s], to[k], 0, 0, 0);
         }
-        if (slot0 + KT > wave_all) {
+    };
+    f16x8 q[D / 16];
 #pragma unroll
-            for (int k = 0; k < KN; ++k)
+    for (int s = 0; s < D / 16; ++s) q[s] = __builtin_bit_cast(f16x8, qr[s]);
+
+    // Tile `at` of the loop has its scores in st and its values in LDS, the next
+    // tile its keys: the next scores are formed while the softmax runs on the
+    // present ones, and the codes of the keys after next and of the next values
+    // are decoded while the present weights are multiplied.
+    stage_keys(keys[0]);
+    stage_values(values[0], first);
+    load_keys(first + 1);
+    load_values(first + 1);
+    __syncthreads();
+    f32x16 st[KN], next[KN];
+    products(q, keys[0], st);
+    stage_keys(keys[1]);
+    load_keys(first + 2);
+    __syncthreads();
+    for (int at = first; at < stop; ++at) {
+        const int slot0 = at * KT, now = (at - first) & 1;
+        f16* const keys_at = keys[now];
+        if (slot0 < wave_end) {   // every wavefront meets the same barriers
+            float mul[2 * KN], vex[2 * KN], vinv[2 * KN];
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (slot0 + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3) > last) st[k][i] = -__builtin_inff();
-        }
-        float mx = run_max;
-#pragma unroll
-        for (int x = 0; x < 2 * KN; ++x) {
-            float top = st[x >> 1][8 * (x & 1)];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) top = fmaxf(top, st[x >> 1][8 * (x & 1) + i]);
-            mx = fmaxf(mx, __builtin_fmaf(top, mul[x], vex[x]));
-        }
-        mx = half_pair_max(mx);
-        const float base = mx == -__builtin_inff() ? 0.0f : mx;
-        const float rescale = __builtin_amdgcn_exp2f(run_max - base);
-        run_max = mx;
-        f16x8 weights[KN][2];
-        float total = 0.0f;
-#pragma unroll
-        for (int x = 0; x < 2 * KN; ++x) {
-            const float shift = vex[x] - base;
-            float sum = 0.0f;
-            u32x4 packed;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float lo = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x >> 1][8 * (x & 1) + 2 * i], mul[x], shift));
-                const float hi = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x >> 1][8 * (x & 1) + 2 * i + 1], mul[x], shift));
-                // summed before the rounding: where values differ in scale, fp16 drops small
-                // weights of small values that hold most of the sum
-                sum += lo + hi;
-                packed[i] = as_u32((f16x2){(f16)lo, (f16)hi});
+            for (int x = 0; x < 2 * KN; ++x) {
+                const int blk = min(slot0 + 16 * x, last_slot) >> a.block_log;
+                const int e = exponent_of(vs[blk]);
+                mul[x] = row_scale * ks[blk];
+                vex[x] = (float)e;
+                vinv[x] = exp2_int(-e);
             }
-            weights[x >> 1][x & 1] = __builtin_bit_cast(f16x8, packed);
-            total = __builtin_fmaf(sum, vinv[x], total);
-        }
-        run_sum = __builtin_fmaf(run_sum, rescale, total);
-        if (__any(rescale != 1.0f)) {
+            if (slot0 + KT > wave_all) {
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) acc[d] *= rescale;
-        }
+                for (int k = 0; k < KN; ++k)
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
+                    for (int i = 0; i < 16; ++i)
+                        if (slot0 + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3) > last) st[k][i] = -__builtin_inff();
+            }
+            products(q, keys[now ^ 1], next);   // of no use past the last tile
+            float mx = run_max;
 #pragma unroll
-            for (int k = 0; k < KN; ++k)
+            for (int x = 0; x < 2 * KN; ++x) {
+                float top = st[x >> 1][8 * (x & 1)];
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
+                for (int i = 1; i < 8; ++i) top = fmaxf(top, st[x >> 1][8 * (x & 1) + i]);
+                mx = fmaxf(mx, __builtin_fmaf(top, mul[x], vex[x]));
+            }
+            mx = half_pair_max(mx);
+            const float base = mx == -__builtin_inff() ? 0.0f : mx;
+            const float rescale = __builtin_amdgcn_exp2f(run_max - base);
+            run_max = mx;
+            stage_keys(keys_at);
+            stage_values(values[now ^ 1], at + 1);
+            if (__any(rescale != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) acc[d] *= rescale;
+            }
+            float total = 0.0f;
+#pragma unroll
+            for (int x = 0; x < 2 * KN; ++x) {
+                const float shift = vex[x] - base;
+                float sum = 0.0f;
+                u32x4 packed;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float lo = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x >> 1][8 * (x & 1) + 2 * i], mul[x], shift));
+                    const float hi = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x >> 1][8 * (x & 1) + 2 * i + 1], mul[x], shift));
+                    // summed before the rounding: where values differ in scale, fp16 drops small
+                    // weights of small values that hold most of the sum
+                    sum += lo + hi;
+                    packed[i] = as_u32((f16x2){(f16)lo, (f16)hi});
+                }
+                total = __builtin_fmaf(sum, vinv[x], total);
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d)
                     acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                        *reinterpret_cast<const f16x8*>(values + (32 * d + n) * VROW + 32 * k + 16 * x + 8 * h),
-                        weights[k][x], acc[d], 0, 0, 0);
+                        *reinterpret_cast<const f16x8*>(values[now] + (32 * d + n) * VROW + 16 * x + 8 * h),
+                        __builtin_bit_cast(f16x8, packed), acc[d], 0, 0, 0);
+            }
+            run_sum = __builtin_fmaf(run_sum, rescale, total);
+#pragma unroll
+            for (int k = 0; k < KN; ++k) st[k] = next[k];
+        } else {
+            stage_keys(keys_at);
+            stage_values(values[now ^ 1], at + 1);
+        }
+        load_keys(at + 3);
+        load_values(at + 2);
+        __syncthreads();
     }
 
     if (wave0 + n >= rows) return;
