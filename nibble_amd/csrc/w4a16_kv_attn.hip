@@ -72,6 +72,19 @@ __device__ __forceinline__ int seen_end(const AttnArgs& a, const Seen& s, int ro
     return p < 0 ? 0 : (int)p + 1;
 }
 
+// The shares that a workgroup's `parts` chunks or tiles are divided into:
+// `splits` of them at most, none of fewer than `least`. One share writes the
+// outputs itself; with more each writes its state, and merge_kernel joins them.
+struct Shares {
+    int size, count;
+};
+__device__ __forceinline__ Shares shares_of(int parts, int splits, int least) {
+    const int size = max((parts + splits - 1) / splits, least);
+    return {size, (parts + size - 1) / size};
+}
+constexpr int kLeastChunks = 8;   // of 32 slots
+constexpr int kLeastTiles = 8;    // of 64 slots (32 with head_dim 256)
+
 // A query row's 16-bit values -> fp16, with the power of two that was divided
 // out (bf16 only). The row's values are spread over the lanes that `rowmax`
 // joins.
@@ -193,8 +206,9 @@ decode_kernel(const AttnArgs a) {
     const int end = seen_end(a, seen, row0, 16 * NT);
     const int last_slot = max(end - 1, 0);
     const int chunks = (end + 31) >> 5;
-    const int share = (chunks + a.splits - 1) / a.splits;
-    const int first = split * share, stop = min(chunks, first + share);
+    const Shares shares = shares_of(chunks, a.splits, kLeastChunks);
+    if (split > 0 && split >= shares.count) return;
+    const int first = split * shares.size, stop = min(chunks, first + shares.size);
 
     const uint8_t* kc = a.k_codes + b * a.kb + hk * a.kh;
     const uint8_t* vc = a.v_codes + b * a.vb + hk * a.vh;
@@ -386,7 +400,7 @@ decode_kernel(const AttnArgs a) {
                     : (D / 16) * (4 * (q / (4 / PARTS)) + part * (4 / PARTS) + q % (4 / PARTS)) + col % (D / 16);
                 const int t = r / a.group, g = r - t * a.group;
                 const int64_t at = ((int64_t)b * a.tokens + t) * a.heads + hk * a.group + g;
-                if (a.splits > 1) {
+                if (shares.count > 1) {
                     const int64_t sp = at * a.splits + split;
                     *reinterpret_cast<f32x4*>(a.partial + sp * D + dim) = o;
                     if (col == 0 && part == 0) a.states[sp] = make_float2(t0, l);
@@ -408,31 +422,46 @@ decode_kernel(const AttnArgs a) {
 
 // The shares of each output row joined, a wavefront a row: out = sum_s acc_s
 // 2^(R_s - R) / sum_s l_s 2^(R_s - R). Lane s holds share s's state (at most
-// 64 shares); a share without slots has R = -inf and drops out.
+// 64 shares). `rows_per` rows make a workgroup of the launch before, `unit`
+// slots a chunk or tile of it: they give the shares that were written.
 template <int D, int TYPE>
-__global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, int64_t rows) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ void __launch_bounds__(256)
+merge_kernel(const AttnArgs a, int64_t rows, int rows_per, int unit, int least) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= rows) return;
     const int lane = threadIdx.x & 63;
     const int64_t bt = row / a.heads;
+    const int head = (int)(row - bt * a.heads);
     const int b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens);
     const Seen seen = seen_of(a, b);
+    const int r = t * a.group + head % a.group;
+    const int end = seen_end(a, seen, r - r % rows_per, rows_per);
+    const int count = shares_of((end + unit - 1) / unit, a.splits, least).count;
     const int64_t p = seen.start + t;
+    if (count < 2) return;   // the one share has written the row
     constexpr int E = D / 64;   // dims a lane
     float o[E] = {};
     float inv = 0.0f;
     if (t < seen.count && p >= 0 && p < a.slots) {
         float2 state = make_float2(-__builtin_inff(), 0.0f);
-        if (lane < a.splits) state = a.states[row * a.splits + lane];
+        if (lane < count) state = a.states[row * a.splits + lane];
+        const float* part = a.partial + row * a.splits * D + lane * E;
         const float top = wave_max(state.x);
         const float f = state.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.x - top);
         inv = 1.0f / wave_sum(state.y * f);
-        const float* part = a.partial + row * a.splits * D + lane * E;
-        for (int s = 0; s < a.splits; ++s) {
-            const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
-            if (fs == 0.0f) continue;   // nothing was written there
+        for (int s0 = 0; s0 < count; s0 += 4) {   // four shares in flight
+            float v[4][E], fs[4];
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(part[(int64_t)s * D + e], fs, o[e]);
+            for (int x = 0; x < 4; ++x) {
+                const int s = min(s0 + x, count - 1);
+                fs[x] = s0 + x < count ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s)) : 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[x][e] = part[(int64_t)s * D + e];
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(v[x][e], fs[x], o[e]);
         }
     } else if (t < seen.count) {
         inv = __builtin_nanf("");
@@ -453,6 +482,17 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, int64_t ro
 // v_mfma_f32_32x32x16_f16: lane (n, h) = (lane & 31, lane >> 5) receives the
 // scores of row n for slots 8 (i >> 2) + 4 h + (i & 3) of each 32.
 // ---------------------------------------------------------------------------
+// The larger of two values without the quieting of signalling NaN that fmaxf
+// brings (an instruction for each operand that a matrix product left).
+__device__ __forceinline__ float larger(float a, float b) {
+    return __builtin_amdgcn_fmed3f(a, b, __builtin_inff());
+}
+
+// A row's reference R of the weights 2^(w - R) follows its largest w only when
+// that has grown by this much: weights are then up to 2^8 and keep their
+// precision, and the outputs are rarely rescaled.
+constexpr float kSlack = 8.0f;
+
 __device__ __forceinline__ float half_pair_max(float v) {   // over lanes l and l ^ 32
     const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
                                                     false, false);
@@ -464,15 +504,18 @@ __device__ __forceinline__ float half_pair_sum(float v) {
     return __builtin_bit_cast(float, (uint32_t)x[0]) + __builtin_bit_cast(float, (uint32_t)x[1]);
 }
 
+// head_dim 256 keeps its outputs and queries in 512 registers, one wavefront a SIMD
 template <int D, int W, int CODES, int TYPE>
-__global__ void __launch_bounds__(64 * W, 2)
+__global__ void __launch_bounds__(64 * W, D == 256 ? 1 : 2)
 prompt_kernel(const AttnArgs a) {
-    constexpr int KT = 8192 / D;        // slots of a tile
+    constexpr int KT = D == 256 ? 32 : 64;   // slots of a tile
     constexpr int KN = KT / 32;
-    constexpr int KROW = D + 8;         // fp16 values of a key row in LDS
-    constexpr int VROW = KT + 8;        // of a value dim's row
-    constexpr int KL = 512 / (64 * W);  // 16-byte units of keys a thread loads
-    constexpr int VT = 256;             // threads that load values
+    constexpr int KROW = D + 8;              // fp16 values of a key row in LDS
+    constexpr int VROW = KT + 8;             // of a value dim's row
+    constexpr int KU = KT * D / 16;          // 16-byte units of a tile's keys
+    constexpr int KL = KU > 64 * W ? KU / (64 * W) : 1;   // of a thread
+    constexpr int KW = KU < 64 * W ? KU / 64 : W;         // wavefronts that load keys: the first ones
+    constexpr int VW = KT * D / 32 / 64;                  // and values: the last ones
     __shared__ __align__(16) f16 keys[2][KT * KROW];
     __shared__ __align__(16) f16 values[2][D * VROW];
 
@@ -492,8 +535,9 @@ prompt_kernel(const AttnArgs a) {
     const int end = seen_end(a, seen, row0, 32 * W);
     const int last_slot = max(end - 1, 0);
     const int tiles = (end + KT - 1) / KT;
-    const int share = (tiles + a.splits - 1) / a.splits;
-    const int first = split * share, stop = min(tiles, first + share);
+    const Shares shares = shares_of(tiles, a.splits, kLeastTiles);
+    if (split > 0 && split >= shares.count) return;
+    const int first = split * shares.size, stop = min(tiles, first + shares.size);
 
     const int r = min(wave0 + n, rows - 1);
     const int t = r / a.group, g = r - t * a.group;
@@ -519,27 +563,40 @@ prompt_kernel(const AttnArgs a) {
 
     u32x4 kr[KL];
     uint32_t vr[8];
-    const int vt = threadIdx.x % VT;
+    const int vt = (int)threadIdx.x & (64 * VW - 1);
     const int vgroup = vt / (D / 4), vdim = vt % (D / 4);   // 8 slots, 4 dims of the values
-    const bool loads_values = W == 4 || wave >= W - 4;
-    // rows are clamped: tiles past the last one read its last row again
-    auto load_keys = [&](int tile_at) {
-#pragma unroll
-        for (int i = 0; i < KL; ++i) {
-            const int u = threadIdx.x + 64 * W * i;
-            const int row = min(tile_at * KT + u / (D / 16), last_slot);
-            kr[i] = *reinterpret_cast<const u32x4*>(kc + (int64_t)row * D + 16 * (u % (D / 16)));
-        }
+    const bool loads_keys = KW == W || wave < KW, loads_values = VW == W || wave >= W - VW;
+    // the scales of a tile's keys and values, 16 slots a lane (vector loads: scalar
+    // ones share their counter with LDS, whose reads would wait for them)
+    const float* scale_row = lane & (2 * KN) ? vs : ks;
+    auto load_scales = [&](int tile_at) {
+        return scale_row[min(tile_at * KT + 16 * (lane & (2 * KN - 1)), last_slot) >> a.block_log];
     };
+    float scales = load_scales(first), scales_next = load_scales(first + 1);
+    // one uniform base and a 32-bit offset a load, at most that of the last
+    // slot's row (tiles past the last one read the last one's rows again)
+    const int last_tile = max(tiles - 1, 0);
+    auto load_keys = [&](int tile_at) {
+        if (!loads_keys) return;
+        tile_at = min(tile_at, last_tile);
+        const uint8_t* tile0 = kc + (int64_t)tile_at * (KT * D);
+        const uint32_t most = (uint32_t)(last_slot - tile_at * KT) * D + 16 * (threadIdx.x % (D / 16));
+#pragma unroll
+        for (int i = 0; i < KL; ++i)
+            kr[i] = *reinterpret_cast<const u32x4*>(tile0 + min((uint32_t)(16 * (threadIdx.x + 64 * W * i)), most));
+    };
+    const uint32_t value0 = (16 * (vgroup >> 1) + 4 * (vgroup & 1)) * D + 4 * vdim;
     auto load_values = [&](int tile_at) {
         if (!loads_values) return;
+        tile_at = min(tile_at, last_tile);
+        const uint8_t* tile0 = vc + (int64_t)tile_at * (KT * D);
+        const uint32_t most = (uint32_t)(last_slot - tile_at * KT) * D + 4 * vdim;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int slot = tile_at * KT + 16 * (vgroup >> 1) + 8 * (i >> 2) + 4 * (vgroup & 1) + (i & 3);
-            vr[i] = *reinterpret_cast<const uint32_t*>(vc + (int64_t)min(slot, last_slot) * D + 4 * vdim);
-        }
+        for (int i = 0; i < 8; ++i)
+            vr[i] = *reinterpret_cast<const uint32_t*>(tile0 + min(value0 + (8 * (i >> 2) + (i & 3)) * D, most));
     };
     auto stage_keys = [&](f16* to) {
+        if (!loads_keys) return;
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int u = threadIdx.x + 64 * W * i;
@@ -562,6 +619,8 @@ prompt_kernel(const AttnArgs a) {
             *reinterpret_cast<f16x8*>(to + (4 * vdim + d) * VROW + 8 * vgroup) = value[d];
     };
 #pragma unroll
+    for (int i = 0; i < KL; ++i) kr[i] = (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
     for (int i = 0; i < 8; ++i) vr[i] = 0;
     load_keys(first);
     load_values(first);
@@ -583,15 +642,34 @@ prompt_kernel(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
 
+    // Fragments are read four ahead of the matrix instructions that take them;
+    // only vector instructions may be scheduled across (kOrder).
+    constexpr int kOrder = 0x406;
     auto products = [&](f16x8 (&q)[D / 16], const f16* from, f32x16 (&to)[KN]) {   // scores of a tile
+        constexpr int G = KN * D / 16 / 4;
+        f16x8 frag[2][4];
+        auto read = [&](int g, f16x8 (&f)[4]) {
 #pragma unroll
-        for (int k = 0; k < KN; ++k) {
+            for (int i = 0; i < 4; ++i) {
+                const int m = 4 * g + i;
+                f[i] = *reinterpret_cast<const f16x8*>(from + (32 * (m % KN) + n) * KROW + 16 * (m / KN) + 8 * h);
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < KN; ++k)
 #pragma unroll
             for (int i = 0; i < 16; ++i) to[k][i] = 0.0f;
+        read(0, frag[0]);
 #pragma unroll
-            for (int s = 0; s < D / 16; ++s)
-                to[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                    *reinterpret_cast<const f16x8*>(from + (32 * k + n) * KROW + 16 * s + 8 * h), q[s], to[k], 0, 0, 0);
+        for (int g = 0; g < G; ++g) {
+            if (g + 1 < G) read(g + 1, frag[(g + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(kOrder);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int m = 4 * g + i;
+                to[m % KN] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[g & 1][i], q[m / KN], to[m % KN], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(kOrder);
         }
     };
     f16x8 q[D / 16];
@@ -612,16 +690,15 @@ prompt_kernel(const AttnArgs a) {
     stage_keys(keys[1]);
     load_keys(first + 2);
     __syncthreads();
-    for (int at = first; at < stop; ++at) {
-        const int slot0 = at * KT, now = (at - first) & 1;
-        f16* const keys_at = keys[now];
+    auto tile_step = [&](int at, int now, f32x16 (&st)[KN], f32x16 (&next)[KN]) {
+        const int slot0 = at * KT;
         if (slot0 < wave_end) {   // every wavefront meets the same barriers
             float mul[2 * KN], vex[2 * KN], vinv[2 * KN];
 #pragma unroll
             for (int x = 0; x < 2 * KN; ++x) {
-                const int blk = min(slot0 + 16 * x, last_slot) >> a.block_log;
-                const int e = exponent_of(vs[blk]);
-                mul[x] = row_scale * ks[blk];
+                const int bits = __builtin_bit_cast(int, scales);
+                const int e = exponent_of(__builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 2 * KN + x)));
+                mul[x] = row_scale * __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, x));
                 vex[x] = (float)e;
                 vinv[x] = exp2_int(-e);
             }
@@ -633,25 +710,35 @@ prompt_kernel(const AttnArgs a) {
                         if (slot0 + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3) > last) st[k][i] = -__builtin_inff();
             }
             products(q, keys[now ^ 1], next);   // of no use past the last tile
-            float mx = run_max;
+            float mx = -__builtin_inff();
 #pragma unroll
             for (int x = 0; x < 2 * KN; ++x) {
                 float top = st[x >> 1][8 * (x & 1)];
 #pragma unroll
-                for (int i = 1; i < 8; ++i) top = fmaxf(top, st[x >> 1][8 * (x & 1) + i]);
-                mx = fmaxf(mx, __builtin_fmaf(top, mul[x], vex[x]));
+                for (int i = 1; i < 8; ++i) top = larger(top, st[x >> 1][8 * (x & 1) + i]);
+                mx = larger(mx, __builtin_fmaf(top, mul[x], vex[x]));
             }
             mx = half_pair_max(mx);
-            const float base = mx == -__builtin_inff() ? 0.0f : mx;
-            const float rescale = __builtin_amdgcn_exp2f(run_max - base);
-            run_max = mx;
-            stage_keys(keys_at);
+            stage_keys(keys[now]);
             stage_values(values[now ^ 1], at + 1);
-            if (__any(rescale != 1.0f)) {
+            load_keys(at + 3);
+            load_values(at + 2);
+            if (__any(mx > run_max + kSlack)) {
+                mx = fmaxf(mx, run_max);
+                const float rescale = mx == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(run_max - mx);
+                run_max = mx;
+                run_sum *= rescale;
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) acc[d] *= rescale;
             }
-            float total = 0.0f;
+            const float base = run_max == -__builtin_inff() ? 0.0f : run_max;   // no slot of the row seen yet
+            f16x8 frag[2][D / 32];
+            auto read = [&](int x, f16x8 (&f)[D / 32]) {
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d)
+                    f[d] = *reinterpret_cast<const f16x8*>(values[now] + (32 * d + n) * VROW + 16 * x + 8 * h);
+            };
+            read(0, frag[0]);
 #pragma unroll
             for (int x = 0; x < 2 * KN; ++x) {
                 const float shift = vex[x] - base;
@@ -666,29 +753,35 @@ prompt_kernel(const AttnArgs a) {
                     sum += lo + hi;
                     packed[i] = as_u32((f16x2){(f16)lo, (f16)hi});
                 }
-                total = __builtin_fmaf(sum, vinv[x], total);
+                run_sum = __builtin_fmaf(sum, vinv[x], run_sum);
+                if (x + 1 < 2 * KN) read(x + 1, frag[(x + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(kOrder);
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d)
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                        *reinterpret_cast<const f16x8*>(values[now] + (32 * d + n) * VROW + 16 * x + 8 * h),
-                        __builtin_bit_cast(f16x8, packed), acc[d], 0, 0, 0);
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[x & 1][d], __builtin_bit_cast(f16x8, packed),
+                                                                    acc[d], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(kOrder);
             }
-            run_sum = __builtin_fmaf(run_sum, rescale, total);
-#pragma unroll
-            for (int k = 0; k < KN; ++k) st[k] = next[k];
         } else {
-            stage_keys(keys_at);
+            stage_keys(keys[now]);
             stage_values(values[now ^ 1], at + 1);
+            load_keys(at + 3);
+            load_values(at + 2);
         }
-        load_keys(at + 3);
-        load_values(at + 2);
+        scales = scales_next;
+        scales_next = load_scales(at + 2);
         __syncthreads();
+    };
+    // two tiles a round, so that the scores change places without copies
+    for (int at = first; at < stop; at += 2) {
+        tile_step(at, 0, st, next);
+        if (at + 1 < stop) tile_step(at + 1, 1, next, st);
     }
 
     if (wave0 + n >= rows) return;
     run_sum = half_pair_sum(run_sum);
     const int64_t at = ((int64_t)b * a.tokens + t) * a.heads + hk * a.group + g;
-    if (a.splits > 1) {
+    if (shares.count > 1) {
         const int64_t sp = at * a.splits + split;
         if (h == 0) a.states[sp] = make_float2(run_max, run_sum);
         float* o = a.partial + sp * D + 4 * h;
@@ -724,25 +817,39 @@ using w4a16_internal::kv_fail;
 // How a call is launched: the form, the rows of a workgroup, the shares of the slots.
 struct AttnPlan {
     bool prompt;
+    int waves;          // W of the prompt form
     int column_tiles;   // NT of the decode form
+    int rows_per;
     int64_t row_tiles;
     int splits;
 };
 
 constexpr int kMaxSplits = 64;
-constexpr int kPromptWaves = 8;
 
 AttnPlan plan_attention(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t slots, int64_t dim) {
     AttnPlan p;
     const int64_t rows = tokens * (heads / kv_heads);
     p.prompt = rows > 64;
     p.column_tiles = rows <= 16 ? 1 : rows <= 32 || dim == 256 ? 2 : 4;
-    const int64_t per = p.prompt ? 32 * kPromptWaves : 16 * p.column_tiles;
-    p.row_tiles = (rows + per - 1) / per;
-    // shares: until the chip is full, and none of less than 256 slots
-    const int64_t wanted = p.prompt ? 512 : 1024;
+    // Prompts: a workgroup of 256 rows decodes a tile once for twice the rows,
+    // two of 128 rows a compute unit do not wait for each other (32/8 heads of
+    // 128: 4096 tokens, 512 workgroups of 256 rows 152 against 168 us; 2000
+    // tokens, 256 of them, 68 against 58; 32/4 heads of 64, 2048 tokens 51
+    // against 40). head_dim 256 has registers for 128 rows only.
+    p.waves = dim <= 128 && batch * kv_heads * ((rows + 255) / 256) >= 512 ? 8 : 4;
+    p.rows_per = p.prompt ? 32 * p.waves : 16 * p.column_tiles;
+    p.row_tiles = (rows + p.rows_per - 1) / p.rows_per;
+    // Shares of the slots, where the rows alone leave the chip empty: a share
+    // writes fp32 outputs and brings the merge's launch (5 to 8 us with a
+    // prompt's rows; 300 tokens 20 against 15 us), so prompts are divided from
+    // 1024 slots on, to fill the chip once, and twice from 8192 on (100 tokens
+    // behind 4000: 8 shares 29 us, one 99).
     const int64_t groups = batch * kv_heads * p.row_tiles;
-    int64_t splits = (wanted + groups - 1) / (groups > 0 ? groups : 1);
+    int64_t splits = 1;
+    if (groups > 0 && p.prompt)
+        splits = slots < 1024 ? 1 : (slots < 8192 ? 256 : 512) / groups;
+    else if (groups > 0)
+        splits = (1024 + groups - 1) / groups;
     const int64_t most = (slots + 255) / 256;
     if (splits > most) splits = most;
     if (splits > kMaxSplits) splits = kMaxSplits;
@@ -753,8 +860,11 @@ AttnPlan plan_attention(int64_t batch, int64_t tokens, int64_t heads, int64_t kv
 template <int D, int CODES, int TYPE>
 void launch_attention(const AttnPlan& p, const AttnArgs& a, int64_t grid, hipStream_t st) {
     const dim3 g((unsigned)grid);
-    if (p.prompt)
-        hipLaunchKernelGGL((prompt_kernel<D, kPromptWaves, CODES, TYPE>), g, dim3(64 * kPromptWaves), 0, st, a);
+    if (p.prompt && p.waves == 4)
+        hipLaunchKernelGGL((prompt_kernel<D, 4, CODES, TYPE>), g, dim3(256), 0, st, a);
+    else if (p.prompt) {
+        if constexpr (D <= 128) hipLaunchKernelGGL((prompt_kernel<D, 8, CODES, TYPE>), g, dim3(512), 0, st, a);
+    }
     else if (p.column_tiles == 1)
         hipLaunchKernelGGL((decode_kernel<D, 1, CODES, TYPE>), g, dim3(64 * kDecodeWaves), 0, st, a);
     else if (p.column_tiles == 2)
@@ -770,7 +880,8 @@ void launch_typed(const AttnPlan& p, const AttnArgs& a, int code_type, int64_t g
     else
         launch_attention<D, W4A16_KV_FP8, TYPE>(p, a, grid, st);
     if (a.splits > 1)
-        hipLaunchKernelGGL((merge_kernel<D, TYPE>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, rows);
+        hipLaunchKernelGGL((merge_kernel<D, TYPE>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, rows,
+                           p.rows_per, p.prompt ? (D == 256 ? 32 : 64) : 32, p.prompt ? kLeastTiles : kLeastChunks);
 }
 
 template <int D>
