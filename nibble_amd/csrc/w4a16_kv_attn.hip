@@ -45,7 +45,7 @@ struct AttnArgs {
     int64_t kb, kh, vb, vh, ksb, ksh, vsb, vsh;
     int64_t slots;
     float scale;
-    int tokens, heads, kv_heads, group, block_log, splits, row_tiles;
+    int tokens, heads, kv_heads, group, block_log, splits, least, row_tiles;
     bool vec;
 };
 
@@ -73,17 +73,17 @@ __device__ __forceinline__ int seen_end(const AttnArgs& a, const Seen& s, int ro
 }
 
 // The shares that a workgroup's `parts` chunks or tiles are divided into:
-// `splits` of them at most, none of fewer than `least`. One share writes the
-// outputs itself; with more each writes its state, and merge_kernel joins them.
+// `splits` of them at most, none of fewer than `least`, one up to three times
+// that. One share writes the outputs itself; with more each writes its state,
+// and merge_kernel joins them.
 struct Shares {
     int size, count;
 };
-__device__ __forceinline__ Shares shares_of(int parts, int splits, int least) {
-    const int size = max((parts + splits - 1) / splits, least);
+__host__ __device__ __forceinline__ Shares shares_of(int parts, int splits, int least) {
+    const int even = (parts + splits - 1) / splits;
+    const int size = parts <= 3 * least ? (parts > 0 ? parts : 1) : even > least ? even : least;
     return {size, (parts + size - 1) / size};
 }
-constexpr int kLeastChunks = 8;   // of 32 slots
-constexpr int kLeastTiles = 8;    // of 64 slots (32 with head_dim 256)
 
 // A query row's 16-bit values -> fp16, with the power of two that was divided
 // out (bf16 only). The row's values are spread over the lanes that `rowmax`
@@ -151,24 +151,44 @@ __device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, f
                                               narrow16<TYPE>(c) | (narrow16<TYPE>(d) << 16));
 }
 
+// The larger of two values without the quieting of signalling NaN that fmaxf
+// brings (an instruction for each operand that a matrix product left).
+__device__ __forceinline__ float larger(float a, float b) {
+    return __builtin_amdgcn_fmed3f(a, b, __builtin_inff());
+}
+
+// A row's reference R of the weights 2^(w - R) follows its largest w only when
+// that has grown by this much: weights are then up to 2^8 and keep their
+// precision, and the outputs are rarely rescaled.
+constexpr float kSlack = 8.0f;
+
 // ---------------------------------------------------------------------------
-// Decode form: up to 16 NT query rows of a KV head, every wavefront streaming
-// chunks of 32 slots.
+// Decode form: up to 16 NT query rows of a KV head, every wavefront taking
+// chunks of 16 M slots.
 //
-// Bound: the cache's bytes. Lane (c, h) = (lane & 15, lane >> 4). Keys: 16
-// bytes of row c at 64 j + 16 h, so that two loads of 1 KiB read 16 rows of 64
-// (128, 256) bytes; values: dim / 16 bytes at dim / 16 c of the rows that the
-// lane's weights stand for (slots 4 h + i and 16 + 4 h + i), whole rows again.
-// The next chunk's keys are requested when the present ones are multiplied,
-// its values likewise. Wavefronts of a workgroup join through LDS; the slots
-// of a sequence are divided into `splits` shares, joined by merge_kernel.
+// Bound: the cache's bytes with many sequences, the latency of a chunk (about
+// 1 us from request to weights) with few. Lane (c, h) = (lane & 15, lane >> 4).
+// Keys: 16 bytes of row c at 64 j + 16 h, so that the loads of a row read it
+// whole; values: dim / 16 bytes at dim / 16 c of the rows that the lane's
+// weights stand for (slots 32 y + 4 h + i and 32 y + 16 + 4 h + i), whole rows
+// again. The next chunk's keys are requested when the present ones are
+// multiplied, its values likewise. Wavefronts of a workgroup join through LDS;
+// the chunks of a sequence go round the shares, which merge_kernel joins. The
+// first share's first chunk does not depend on the sequence's length and is
+// requested before `start` has arrived.
 // ---------------------------------------------------------------------------
 constexpr int kDecodeWaves = 4;
+// M, the 16-slot tiles of a chunk: four where they leave registers for two
+// wavefronts a SIMD, as the latency of a chunk is paid once for more of them
+// (one token over 8000 slots, 8 KV heads of 128, in one share: 63 us against 76
+// with two); two with more rows (20 rows over 131072 slots of int8: 63 us against 73).
+constexpr int chunk_tiles(int dim, int column_tiles) { return dim == 256 || column_tiles > 1 ? 2 : 4; }
 
 template <int D, int NT, int CODES, int TYPE>
-__global__ void __launch_bounds__(64 * kDecodeWaves)
+__global__ void __launch_bounds__(64 * kDecodeWaves, D * NT > 256 || D == 256 ? 1 : 2)
 decode_kernel(const AttnArgs a) {
     constexpr int W = kDecodeWaves;
+    constexpr int M = chunk_tiles(D, NT), C = 16 * M;
     constexpr int J = D / 64;                    // 16-byte loads of a key row's quarter; words of a value load
     constexpr int PARTS = D > 128 ? D / 128 : 1;
     constexpr int DP = D / PARTS;
@@ -186,10 +206,52 @@ decode_kernel(const AttnArgs a) {
     const int hk = item % a.kv_heads, b = item / a.kv_heads;
     const int rows = a.tokens * a.group, row0 = tile * 16 * NT;
 
+    const uint8_t* kc = a.k_codes + b * a.kb + hk * a.kh;
+    const uint8_t* vc = a.v_codes + b * a.vb + hk * a.vh;
+    const float* ks = a.k_scales + b * a.ksb + hk * a.ksh;
+    const float* vs = a.v_scales + b * a.vsb + hk * a.vsh;
+    u32x4 kr[M][J];
+    uint32_t vr[M][4][J];   // rows 16 y + 4 h + i of the chunk
+    float k_scale[M], v_scale[M];
+    auto load_keys = [&](int chunk, int limit) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const uint8_t* row = kc + (int64_t)min(C * chunk + 16 * m + c, limit) * D + 16 * h;
+#pragma unroll
+            for (int j = 0; j < J; ++j) kr[m][j] = *reinterpret_cast<const u32x4*>(row + 64 * j);
+            const int at = min(C * chunk + 16 * m, limit) >> a.block_log;
+            k_scale[m] = ks[at];
+            v_scale[m] = vs[at];
+        }
+    };
+    auto load_values = [&](int chunk, int limit) {
+#pragma unroll
+        for (int y = 0; y < M; ++y)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint8_t* row = vc + (int64_t)min(C * chunk + 16 * y + 4 * h + i, limit) * D + (D / 16) * c;
+                if constexpr (J == 1) {
+                    vr[y][i][0] = *reinterpret_cast<const uint32_t*>(row);
+                } else if constexpr (J == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(row);
+                    vr[y][i][0] = v.x;
+                    vr[y][i][1] = v.y;
+                } else {
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(row);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) vr[y][i][w] = v[w];
+                }
+            }
+    };
+    // the other shares read the first rows here and their own below: registers
+    // that only one side of a branch defines have been miscompiled
+    int chunk = split * W + wave;
+    load_keys(split == 0 ? chunk : 0, (int)a.slots - 1);
+    load_values(split == 0 ? chunk : 0, (int)a.slots - 1);
+
     u32x4 qr[NT][2 * J];
     float row_scale[NT];
     int last[NT];
-    const Seen seen = seen_of(a, b);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int r = min(row0 + 16 * n + c, rows - 1);
@@ -200,59 +262,24 @@ decode_kernel(const AttnArgs a) {
             qr[n][2 * j] = load8(q + 64 * j + 16 * h, a.vec);
             qr[n][2 * j + 1] = load8(q + 64 * j + 16 * h + 8, a.vec);
         }
+    }
+    const Seen seen = seen_of(a, b);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int t = min(row0 + 16 * n + c, rows - 1) / a.group;
         const int64_t p = seen.start + t;
         last[n] = t < seen.count && p >= 0 && p < a.slots ? (int)p : -1;
     }
     const int end = seen_end(a, seen, row0, 16 * NT);
     const int last_slot = max(end - 1, 0);
-    const int chunks = (end + 31) >> 5;
-    const Shares shares = shares_of(chunks, a.splits, kLeastChunks);
-    if (split > 0 && split >= shares.count) return;
-    const int first = split * shares.size, stop = min(chunks, first + shares.size);
-
-    const uint8_t* kc = a.k_codes + b * a.kb + hk * a.kh;
-    const uint8_t* vc = a.v_codes + b * a.vb + hk * a.vh;
-    const float* ks = a.k_scales + b * a.ksb + hk * a.ksh;
-    const float* vs = a.v_scales + b * a.vsb + hk * a.vsh;
-
-    u32x4 kr[2][J];
-    uint32_t vr[8][J];
-    float k_scale[2], v_scale[2];
-    auto load_keys = [&](int chunk) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const uint8_t* row = kc + (int64_t)min(32 * chunk + 16 * m + c, last_slot) * D + 16 * h;
-#pragma unroll
-            for (int j = 0; j < J; ++j) kr[m][j] = *reinterpret_cast<const u32x4*>(row + 64 * j);
-            const int at = min(32 * chunk + 16 * m, last_slot) >> a.block_log;
-            k_scale[m] = ks[at];
-            v_scale[m] = vs[at];
-        }
-    };
-    auto load_values = [&](int chunk) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int slot = 32 * chunk + 16 * (i >> 2) + 4 * h + (i & 3);
-            const uint8_t* row = vc + (int64_t)min(slot, last_slot) * D + (D / 16) * c;
-            if constexpr (J == 1) {
-                vr[i][0] = *reinterpret_cast<const uint32_t*>(row);
-            } else if constexpr (J == 2) {
-                const uint2 v = *reinterpret_cast<const uint2*>(row);
-                vr[i][0] = v.x;
-                vr[i][1] = v.y;
-            } else {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(row);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) vr[i][w] = v[w];
-            }
-        }
-    };
-
-    // the first chunk whether or not there is one (rows are clamped): registers
-    // that only one side of a branch defines have been miscompiled here
-    int chunk = first + wave;
-    load_keys(chunk);
-    load_values(chunk);
+    const int chunks = (end + C - 1) / C;
+    const Shares shares = shares_of(chunks, a.splits, a.least);
+    if (split > 0) {
+        if (split >= shares.count) return;
+        load_keys(chunk, last_slot);
+        load_values(chunk, last_slot);
+    }
+    const int step = W * max(shares.count, 1);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
         row_scale[n] = a.scale * kLog2e * query_to_f16<TYPE>(qr[n], row_pair_max);
@@ -266,12 +293,12 @@ decode_kernel(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) acc[n][i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    while (chunk < stop) {
-        const int slot0 = 32 * chunk;
-        f32x4 st[NT][2];
-        float ksc[2], vex[2], vinv[2];
+    while (chunk < chunks) {
+        const int slot0 = C * chunk;
+        f32x4 st[NT][M];
+        float ksc[M], vex[M], vinv[M];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int m = 0; m < M; ++m) {
             ksc[m] = k_scale[m];
             const int e = exponent_of(v_scale[m]);
             vex[m] = (float)e;
@@ -289,68 +316,78 @@ decode_kernel(const AttnArgs a) {
                             key, __builtin_bit_cast(f16x8, qr[n][2 * j + x]), st[n][m], 0, 0, 0);
                 }
         }
-        const bool more = chunk + W < stop;
-        if (more) load_keys(chunk + W);
-        f16x8 weights[NT];
+        const int next = chunk + step;
+        if (next < chunks) load_keys(next, last_slot);
+        f16x8 weights[NT][M / 2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float w[2][4], mx = run_max[n];
+            float mx = -__builtin_inff();
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < M; ++m)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    w[m][e] = __builtin_fmaf(st[n][m][e], row_scale[n] * ksc[m], vex[m]);
-                    if (slot0 + 16 * m + 4 * h + e > last[n]) w[m][e] = -__builtin_inff();
-                    mx = fmaxf(mx, w[m][e]);
+                    float w = __builtin_fmaf(st[n][m][e], row_scale[n] * ksc[m], vex[m]);
+                    if (slot0 + 16 * m + 4 * h + e > last[n]) w = -__builtin_inff();
+                    st[n][m][e] = w;
+                    mx = larger(mx, w);
                 }
             mx = row_pair_max(mx);
-            const float base = mx == -__builtin_inff() ? 0.0f : mx;   // no slot of the row seen yet
-            const float rescale = __builtin_amdgcn_exp2f(run_max[n] - base);
-            run_max[n] = mx;
-            float sum[2] = {0.0f, 0.0f};
-            u32x4 packed;
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                float p[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(w[m][e] - base);
-                    sum[m] += p[e];
-                }
-                packed[2 * m] = as_u32((f16x2){(f16)p[0], (f16)p[1]});
-                packed[2 * m + 1] = as_u32((f16x2){(f16)p[2], (f16)p[3]});
-            }
-            weights[n] = __builtin_bit_cast(f16x8, packed);
-            run_sum[n] = run_sum[n] * rescale + (sum[0] * vinv[0] + sum[1] * vinv[1]);
-            if (__any(rescale != 1.0f)) {
+            if (__any(mx > run_max[n] + kSlack)) {
+                mx = fmaxf(mx, run_max[n]);
+                const float rescale = mx == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(run_max[n] - mx);
+                run_max[n] = mx;
+                run_sum[n] *= rescale;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) acc[n][i] *= rescale;
             }
+            const float base = run_max[n] == -__builtin_inff() ? 0.0f : run_max[n];   // no slot of the row seen yet
+#pragma unroll
+            for (int y = 0; y < M / 2; ++y) {
+                u32x4 packed;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int m = 2 * y + x;
+                    float p[4], sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p[e] = __builtin_amdgcn_exp2f(st[n][m][e] - base);
+                        sum += p[e];
+                    }
+                    run_sum[n] = __builtin_fmaf(sum, vinv[m], run_sum[n]);
+                    packed[2 * x] = as_u32((f16x2){(f16)p[0], (f16)p[1]});
+                    packed[2 * x + 1] = as_u32((f16x2){(f16)p[2], (f16)p[3]});
+                }
+                weights[n][y] = __builtin_bit_cast(f16x8, packed);
+            }
         }
-        if (slot0 + 32 > end) {   // rows behind the last slot may hold anything, NaN codes too
+        if (slot0 + C > end) {   // rows behind the last slot may hold anything, NaN codes too
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (slot0 + 16 * (i >> 2) + 4 * h + (i & 3) >= end)
+            for (int y = 0; y < M; ++y)
 #pragma unroll
-                    for (int j = 0; j < J; ++j) vr[i][j] = 0;
+                for (int i = 0; i < 4; ++i)
+                    if (slot0 + 16 * y + 4 * h + i >= end)
+#pragma unroll
+                        for (int j = 0; j < J; ++j) vr[y][i][j] = 0;
         }
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            uint32_t words[8];
+        for (int y = 0; y < M / 2; ++y)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) words[i] = vr[i][j];
-            f16x8 value[4];
-            transpose8<CODES>(words, value);
+            for (int j = 0; j < J; ++j) {
+                uint32_t words[8];
 #pragma unroll
-            for (int d = 0; d < 4; ++d)
+                for (int i = 0; i < 8; ++i) words[i] = vr[2 * y + (i >> 2)][i & 3][j];
+                f16x8 value[4];
+                transpose8<CODES>(words, value);
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    acc[n][4 * j + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[d], weights[n],
-                                                                               acc[n][4 * j + d], 0, 0, 0);
-        }
-        if (!more) break;
-        chunk += W;
-        load_values(chunk);
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[n][4 * j + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[d], weights[n][y],
+                                                                                   acc[n][4 * j + d], 0, 0, 0);
+            }
+        if (next >= chunks) break;
+        chunk = next;
+        load_values(chunk, last_slot);
     }
 
     // the wavefronts' states joined: lane (c, h) holds row c's dims D / 16 (4 h + i) + j in acc[][j][i]
@@ -420,55 +457,66 @@ decode_kernel(const AttnArgs a) {
     }
 }
 
-// The shares of each output row joined, a wavefront a row: out = sum_s acc_s
-// 2^(R_s - R) / sum_s l_s 2^(R_s - R). Lane s holds share s's state (at most
-// 64 shares). `rows_per` rows make a workgroup of the launch before, `unit`
-// slots a chunk or tile of it: they give the shares that were written.
+// The shares of an output row joined by a workgroup: out = sum_s acc_s 2^(R_s
+// - R) / sum_s l_s 2^(R_s - R). Lane s holds share s's state (at most 64
+// shares); wavefront w takes the shares w, w + 4, .., four in flight.
+// `rows_per` rows make a workgroup of the launch before, `unit` slots a chunk
+// or tile of it: they give the shares that were written.
 template <int D, int TYPE>
-__global__ void __launch_bounds__(256)
-merge_kernel(const AttnArgs a, int64_t rows, int rows_per, int unit, int least) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (row >= rows) return;
-    const int lane = threadIdx.x & 63;
+__global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, int rows_per, int unit) {
+    constexpr int E = D / 64;   // dims a lane
+    constexpr int F = 4;        // shares of a wavefront in flight
+    __shared__ float parts[4][D];
+    const int64_t row = blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const float* part = a.partial + row * a.splits * D + lane * E;
+    float v[F][E];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int x = 0; x < F; ++x)
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[x][e] = part[(int64_t)min(s0 + 4 * x, a.splits - 1) * D + e];
+    };
+    // requested before `start` tells which of them were written
+    load(wave);
+    float2 state = a.states[row * a.splits + min(lane, a.splits - 1)];
     const int64_t bt = row / a.heads;
     const int head = (int)(row - bt * a.heads);
     const int b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens);
     const Seen seen = seen_of(a, b);
     const int r = t * a.group + head % a.group;
     const int end = seen_end(a, seen, r - r % rows_per, rows_per);
-    const int count = shares_of((end + unit - 1) / unit, a.splits, least).count;
-    const int64_t p = seen.start + t;
+    const int count = shares_of((end + unit - 1) / unit, a.splits, a.least).count;
     if (count < 2) return;   // the one share has written the row
-    constexpr int E = D / 64;   // dims a lane
+    const int64_t p = seen.start + t;
+    const bool inside = t < seen.count && p >= 0 && p < a.slots;   // else nothing was written
+    if (!inside || lane >= count) state = make_float2(-__builtin_inff(), 0.0f);
     float o[E] = {};
-    float inv = 0.0f;
-    if (t < seen.count && p >= 0 && p < a.slots) {
-        float2 state = make_float2(-__builtin_inff(), 0.0f);
-        if (lane < count) state = a.states[row * a.splits + lane];
-        const float* part = a.partial + row * a.splits * D + lane * E;
-        const float top = wave_max(state.x);
-        const float f = state.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.x - top);
-        inv = 1.0f / wave_sum(state.y * f);
-        for (int s0 = 0; s0 < count; s0 += 4) {   // four shares in flight
-            float v[4][E], fs[4];
+    const float top = wave_max(state.x);
+    const float f = state.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.x - top);
+    if (inside) {
+        for (int s0 = wave; s0 < count; s0 += 4 * F) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int s = min(s0 + x, count - 1);
-                fs[x] = s0 + x < count ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s)) : 0.0f;
+            for (int x = 0; x < F; ++x) {
+                const int s = s0 + 4 * x;
+                const float fs = __builtin_bit_cast(
+                    float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(s, count - 1)));
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[x][e] = part[(int64_t)s * D + e];
+                for (int e = 0; e < E; ++e) o[e] = s < count ? __builtin_fmaf(v[x][e], fs, o[e]) : o[e];
             }
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(v[x][e], fs[x], o[e]);
+            if (s0 + 4 * F < count) load(s0 + 4 * F);
         }
-    } else if (t < seen.count) {
-        inv = __builtin_nanf("");
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e) parts[wave][lane * E + e] = o[e];
+    __syncthreads();
+    if (wave != 0) return;
+    const float inv = t >= seen.count ? 0.0f : inside ? 1.0f / wave_sum(state.y * f) : __builtin_nanf("");
     uint16_t* out = a.out + row * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[e] = (uint16_t)narrow16<TYPE>(o[e] * inv);
+    for (int e = 0; e < E; ++e)
+        out[e] = (uint16_t)narrow16<TYPE>(((parts[0][lane * E + e] + parts[1][lane * E + e]) +
+                                           (parts[2][lane * E + e] + parts[3][lane * E + e])) * inv);
 }
 
 // ---------------------------------------------------------------------------
@@ -482,17 +530,6 @@ merge_kernel(const AttnArgs a, int64_t rows, int rows_per, int unit, int least) 
 // v_mfma_f32_32x32x16_f16: lane (n, h) = (lane & 31, lane >> 5) receives the
 // scores of row n for slots 8 (i >> 2) + 4 h + (i & 3) of each 32.
 // ---------------------------------------------------------------------------
-// The larger of two values without the quieting of signalling NaN that fmaxf
-// brings (an instruction for each operand that a matrix product left).
-__device__ __forceinline__ float larger(float a, float b) {
-    return __builtin_amdgcn_fmed3f(a, b, __builtin_inff());
-}
-
-// A row's reference R of the weights 2^(w - R) follows its largest w only when
-// that has grown by this much: weights are then up to 2^8 and keep their
-// precision, and the outputs are rarely rescaled.
-constexpr float kSlack = 8.0f;
-
 __device__ __forceinline__ float half_pair_max(float v) {   // over lanes l and l ^ 32
     const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v),
                                                     false, false);
@@ -535,7 +572,7 @@ prompt_kernel(const AttnArgs a) {
     const int end = seen_end(a, seen, row0, 32 * W);
     const int last_slot = max(end - 1, 0);
     const int tiles = (end + KT - 1) / KT;
-    const Shares shares = shares_of(tiles, a.splits, kLeastTiles);
+    const Shares shares = shares_of(tiles, a.splits, a.least);
     if (split > 0 && split >= shares.count) return;
     const int first = split * shares.size, stop = min(tiles, first + shares.size);
 
@@ -821,7 +858,8 @@ struct AttnPlan {
     int column_tiles;   // NT of the decode form
     int rows_per;
     int64_t row_tiles;
-    int splits;
+    int unit;           // slots of a chunk or tile
+    int splits, least;  // shares of the slots, and the units of the smallest
 };
 
 constexpr int kMaxSplits = 64;
@@ -839,20 +877,26 @@ AttnPlan plan_attention(int64_t batch, int64_t tokens, int64_t heads, int64_t kv
     p.waves = dim <= 128 && batch * kv_heads * ((rows + 255) / 256) >= 512 ? 8 : 4;
     p.rows_per = p.prompt ? 32 * p.waves : 16 * p.column_tiles;
     p.row_tiles = (rows + p.rows_per - 1) / p.rows_per;
-    // Shares of the slots, where the rows alone leave the chip empty: a share
-    // writes fp32 outputs and brings the merge's launch (5 to 8 us with a
-    // prompt's rows; 300 tokens 20 against 15 us), so prompts are divided from
-    // 1024 slots on, to fill the chip once, and twice from 8192 on (100 tokens
-    // behind 4000: 8 shares 29 us, one 99).
+    // Shares of the slots, where the rows alone leave the chip empty. Each writes
+    // fp32 outputs and all bring the merge's launch (3 us, 5 to 8 with a prompt's
+    // rows).
+    // Decoding: one workgroup a compute unit (one token over 130000 slots, 8 KV
+    // heads of 128: 56 us, with two 58), two with 17 to 32 rows, whose chunks are
+    // shorter (20 rows over 131072 slots: 63 us, with one 83).
+    // Prompts: from 1024 slots on, to fill the chip once, and twice from 8192 on
+    // (100 tokens behind 4000: 8 shares 29 us, one 99; but 300 tokens from the
+    // start 15 us in one share, 20 in two, so shares are of 512 slots at least,
+    // 2048 where the rows give more than 64 workgroups).
     const int64_t groups = batch * kv_heads * p.row_tiles;
+    p.least = !p.prompt ? 4 : groups <= 64 ? 8 : 32;
+    p.unit = p.prompt ? (dim == 256 ? 32 : 64) : 16 * chunk_tiles((int)dim, p.column_tiles);
     int64_t splits = 1;
     if (groups > 0 && p.prompt)
         splits = slots < 1024 ? 1 : (slots < 8192 ? 256 : 512) / groups;
     else if (groups > 0)
-        splits = (1024 + groups - 1) / groups;
-    const int64_t most = (slots + 255) / 256;
+        splits = ((p.column_tiles == 2 ? 512 : 256) + groups - 1) / groups;
+    const int64_t most = shares_of((int)((slots + p.unit - 1) / p.unit), kMaxSplits, p.least).count;
     if (splits > most) splits = most;
-    if (splits > kMaxSplits) splits = kMaxSplits;
     p.splits = splits < 1 ? 1 : (int)splits;
     return p;
 }
@@ -880,8 +924,8 @@ void launch_typed(const AttnPlan& p, const AttnArgs& a, int code_type, int64_t g
     else
         launch_attention<D, W4A16_KV_FP8, TYPE>(p, a, grid, st);
     if (a.splits > 1)
-        hipLaunchKernelGGL((merge_kernel<D, TYPE>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, rows,
-                           p.rows_per, p.prompt ? (D == 256 ? 32 : 64) : 32, p.prompt ? kLeastTiles : kLeastChunks);
+        hipLaunchKernelGGL((merge_kernel<D, TYPE>), dim3((unsigned)rows), dim3(256), 0, st, a, p.rows_per,
+                           p.unit);
 }
 
 template <int D>
@@ -934,7 +978,7 @@ int w4a16_kv_attention(const w4a16_kv_rows* q, void* out, int64_t tokens, int64_
             return kv_fail(W4A16_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
     }
     const int64_t grid = batch * cache->kv_heads * p.row_tiles * p.splits;
-    if (grid > 0x7FFFFFFF || rows / 4 > 0x7FFFFFFE) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
+    if (grid > 0x7FFFFFFF || rows > 0x7FFFFFFF) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
     AttnArgs a{};
     a.q = static_cast<const uint16_t*>(q->data);
     a.out = static_cast<uint16_t*>(out);
@@ -966,6 +1010,7 @@ int w4a16_kv_attention(const w4a16_kv_rows* q, void* out, int64_t tokens, int64_
     a.group = (int)(heads / cache->kv_heads);
     a.block_log = cache->block == 16 ? 4 : cache->block == 32 ? 5 : cache->block == 64 ? 6 : 7;
     a.splits = p.splits;
+    a.least = p.least;
     a.row_tiles = (int)p.row_tiles;
     a.vec = (reinterpret_cast<uintptr_t>(q->data) & 15u) == 0 &&
             ((q->batch_stride | q->token_stride | q->head_stride) & 7) == 0;
