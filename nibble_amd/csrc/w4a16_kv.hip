@@ -16,10 +16,58 @@ namespace w4a16 {
 // Rotary positions.
 //
 // Bound: memory, 2 bytes read and 2 written per value. A thread holds one unit
-// (16 values: dims 8 u .. + 7 and rot / 2 + 8 u .. + 7, or 16 u .. + 15 of
-// interleaved pairs; past rot 16 values to copy) of HPT heads of one token, so
-// that a token's table rows are read once for HPT heads.
+// of HPT heads of one token, so that a token's table rows are read once for HPT
+// heads: two vectors of 8 values that rotate each other (dims 8 u and rot / 2 +
+// 8 u), or any two of interleaved or copied dims, half a row apart, so that the
+// lanes of a row lie next to each other.
 // ---------------------------------------------------------------------------
+struct Unit {
+    int lo, hi;                  // dims of its two vectors of 8 values
+    bool lo_turned, hi_turned;   // half layout: both or none
+    int one, two;                // table columns of the pairs: 4 from each, or (half layout) 8 from the first
+};
+template <bool INTERLEAVED>
+__device__ __forceinline__ Unit unit_of(int u, int dim, int rot) {
+    Unit t;
+    if constexpr (INTERLEAVED) {
+        t.lo = 8 * u;
+        t.hi = 8 * u + dim / 2;
+        t.lo_turned = t.lo < rot;
+        t.hi_turned = t.hi < rot;
+        t.one = t.lo_turned ? t.lo / 2 : 0;
+        t.two = t.hi_turned ? t.hi / 2 : 0;
+    } else {
+        const bool turned = 16 * u < rot;
+        t.lo = turned ? 8 * u : 8 * u + rot / 2;
+        t.hi = t.lo + (turned ? rot : dim - rot) / 2;
+        t.lo_turned = t.hi_turned = turned;
+        t.one = turned ? t.lo : 0;
+        t.two = t.one + 4;
+    }
+    return t;
+}
+
+// The unit's vectors rotated where they are turned, rounded to the rows' type.
+template <int TYPE, bool INTERLEAVED>
+__device__ __forceinline__ void rotate_unit(const Unit& t, u32x4& a, u32x4& b, const float (&c)[8], const float (&s)[8]) {
+    float x1[8], x2[8];
+    widen8<TYPE>(a, x1);
+    widen8<TYPE>(b, x2);
+    if constexpr (INTERLEAVED) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            rotate_pair(x1[2 * j], x1[2 * j + 1], c[j], s[j]);
+            rotate_pair(x2[2 * j], x2[2 * j + 1], c[4 + j], s[4 + j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rotate_pair(x1[j], x2[j], c[j], s[j]);
+    }
+    const u32x4 r1 = narrow8<TYPE>(x1), r2 = narrow8<TYPE>(x2);
+    a = t.lo_turned ? r1 : a;
+    b = t.hi_turned ? r2 : b;
+}
+
 struct RotaryArgs {
     const uint16_t* x;
     uint16_t* out;
@@ -41,16 +89,14 @@ __device__ __forceinline__ void rotary_units(const RotaryArgs& a, int64_t first)
     rest /= a.head_groups;
     const int t = (int)(rest % a.tokens), b = (int)(rest / a.tokens);
 
-    const bool turned = 16 * u < a.rot;
-    const int lo = INTERLEAVED || !turned ? 16 * u : 8 * u;
-    const int hi = INTERLEAVED || !turned ? lo + 8 : lo + a.rot / 2;
+    const Unit unit = unit_of<INTERLEAVED>(u, a.dim, a.rot);
     u32x4 va[HPT], vb[HPT];
     const uint16_t* x = a.x + b * a.xb + t * a.xt;
 #pragma unroll
     for (int i = 0; i < HPT; ++i) {
         const uint16_t* row = x + min(hg + i * a.head_groups, a.heads - 1) * a.xh;
-        va[i] = *reinterpret_cast<const u32x4*>(row + lo);
-        vb[i] = *reinterpret_cast<const u32x4*>(row + hi);
+        va[i] = *reinterpret_cast<const u32x4*>(row + unit.lo);
+        vb[i] = *reinterpret_cast<const u32x4*>(row + unit.hi);
     }
     int64_t p;
     bool padding = false;
@@ -64,38 +110,24 @@ __device__ __forceinline__ void rotary_units(const RotaryArgs& a, int64_t first)
     }
     const bool known = p >= 0 && p < limit;
     float c[8], s[8];
-    const int64_t at = (known && turned ? p : 0) * (a.rot / 2) + (turned ? 8 * u : 0);
+    const int64_t at = (known ? p : 0) * (a.rot / 2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        c[i] = known ? a.cos_table[at + i] : __builtin_nanf("");
-        s[i] = known ? a.sin_table[at + i] : __builtin_nanf("");
+    for (int i = 0; i < 4; ++i) {
+        c[i] = known ? a.cos_table[at + unit.one + i] : __builtin_nanf("");
+        s[i] = known ? a.sin_table[at + unit.one + i] : __builtin_nanf("");
+        c[4 + i] = known ? a.cos_table[at + unit.two + i] : __builtin_nanf("");
+        s[4 + i] = known ? a.sin_table[at + unit.two + i] : __builtin_nanf("");
     }
     uint16_t* out = a.out + ((int64_t)b * a.tokens + t) * a.heads * a.dim;
 #pragma unroll
     for (int i = 0; i < HPT; ++i) {
         const int h = hg + i * a.head_groups;
         if (h >= a.heads) break;
-        if (turned) {
-            float x1[8], x2[8];
-            widen8<TYPE>(va[i], x1);
-            widen8<TYPE>(vb[i], x2);
-            if constexpr (INTERLEAVED) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    rotate_pair(x1[2 * j], x1[2 * j + 1], c[j], s[j]);
-                    rotate_pair(x2[2 * j], x2[2 * j + 1], c[4 + j], s[4 + j]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) rotate_pair(x1[j], x2[j], c[j], s[j]);
-            }
-            va[i] = narrow8<TYPE>(x1);
-            vb[i] = narrow8<TYPE>(x2);
-        }
+        rotate_unit<TYPE, INTERLEAVED>(unit, va[i], vb[i], c, s);
         if (padding) va[i] = vb[i] = (u32x4){0u, 0u, 0u, 0u};
         uint16_t* row = out + (int64_t)h * a.dim;
-        *reinterpret_cast<u32x4*>(row + lo) = va[i];
-        *reinterpret_cast<u32x4*>(row + hi) = vb[i];
+        *reinterpret_cast<u32x4*>(row + unit.lo) = va[i];
+        *reinterpret_cast<u32x4*>(row + unit.hi) = vb[i];
     }
 }
 
@@ -138,7 +170,7 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryArgs a) {
 // Bound: memory (2 bytes read and 1 written per value) for prompts, one chain
 // of latencies (start, rows, scale, stores) for single tokens. A workgroup
 // owns one block of one head's keys or values: it holds the block's new rows
-// in registers (UPT units of 8 values a thread), reduces their magnitude, and
+// in registers (UPT units of 16 values a thread), reduces their magnitude, and
 // writes codes under the joint scale, so that every value is read once and no
 // other workgroup touches the block's scale. Only where the scale of a block
 // with earlier tokens grows are those read and rescaled.
@@ -180,59 +212,49 @@ __device__ __forceinline__ void write_block(const WriteArgs& a, int item) {
     float* scale_at = w.scales + b * w.sb + h * w.sh + j;
     const float was = earlier > 0 ? *scale_at : 0.0f;
 
-    const int per_row = a.dim >> 3;
+    const int per_row = a.dim >> 4;
     const int units = rows * per_row;
     const uint16_t* x = w.x + b * w.xb + h * w.xh + (r0 - start) * w.xt;
-    float v[UPT][8];
-    float amax = 0.0f;
-    u32x4 raw[UPT], other[ROTATE ? UPT : 1];
     const bool rotate = ROTATE && values == 0;
+    float amax = 0.0f;
+    u32x4 raw[UPT][2];
+    Unit unit[UPT];
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
         const int u = min((int)(threadIdx.x + i * blockDim.x), units - 1);
-        const int r = u / per_row, d = (u - r * per_row) * 8;
-        raw[i] = load8(x + r * w.xt + d, w.vec);
-        if constexpr (ROTATE && !INTERLEAVED) {
-            if (rotate && d < a.rot)
-                other[i] = load8(x + r * w.xt + (d < a.rot / 2 ? d + a.rot / 2 : d - a.rot / 2), w.vec);
-        }
+        const int r = u / per_row;
+        unit[i] = unit_of<INTERLEAVED>(u - r * per_row, a.dim, rotate ? a.rot : a.dim);
+        raw[i][0] = load8(x + r * w.xt + unit[i].lo, w.vec);
+        raw[i][1] = load8(x + r * w.xt + unit[i].hi, w.vec);
     }
+    if constexpr (ROTATE) {
+        if (rotate) {
 #pragma unroll
-    for (int i = 0; i < UPT; ++i) {
-        const int u = min((int)(threadIdx.x + i * blockDim.x), units - 1);
-        widen8<TYPE>(raw[i], v[i]);
-        if constexpr (ROTATE) {
-            const int r = u / per_row, d = (u - r * per_row) * 8;
-            if (rotate && d < a.rot) {
-                const int64_t at = (r0 + r) * (a.rot / 2);
-                if constexpr (INTERLEAVED) {
+            for (int i = 0; i < UPT; ++i) {
+                const int u = min((int)(threadIdx.x + i * blockDim.x), units - 1);
+                const int64_t at = (r0 + u / per_row) * (a.rot / 2);
+                float c[8], s[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        rotate_pair(v[i][2 * e], v[i][2 * e + 1], a.cos_table[at + d / 2 + e],
-                                    a.sin_table[at + d / 2 + e]);
-                } else {
-                    const bool second = d >= a.rot / 2;
-                    const int64_t c0 = at + (second ? d - a.rot / 2 : d);
-                    float o[8];
-                    widen8<TYPE>(other[i], o);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float x1 = second ? o[e] : v[i][e], x2 = second ? v[i][e] : o[e];
-                        rotate_pair(x1, x2, a.cos_table[c0 + e], a.sin_table[c0 + e]);
-                        v[i][e] = second ? x2 : x1;
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    c[e] = a.cos_table[at + unit[i].one + e];
+                    s[e] = a.sin_table[at + unit[i].one + e];
+                    c[4 + e] = a.cos_table[at + unit[i].two + e];
+                    s[4 + e] = a.sin_table[at + unit[i].two + e];
                 }
                 // the cache holds keys as the rotary op returns them: rounded to the rows' type
-                const u32x4 rounded = narrow8<TYPE>(v[i]);
-                widen8<TYPE>(rounded, v[i]);
+                rotate_unit<TYPE, INTERLEAVED>(unit[i], raw[i][0], raw[i][1], c, s);
             }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[i][e] = v[i][e] == v[i][e] ? v[i][e] : 0.0f;
-            amax = __builtin_fmaxf(amax, __builtin_fabsf(v[i][e]));
-        }
     }
+#pragma unroll
+    for (int i = 0; i < UPT; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float v[8];
+            widen8<TYPE>(raw[i][k], v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = __builtin_fmaxf(amax, __builtin_fabsf(v[e]));   // (leaves NaN out)
+        }
     amax = wave_max(amax);
     if (blockDim.x > 64) {
         if ((threadIdx.x & 63) == 0) wave_amax[threadIdx.x >> 6] = amax;
@@ -250,16 +272,26 @@ __device__ __forceinline__ void write_block(const WriteArgs& a, int item) {
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
         const int u = threadIdx.x + i * blockDim.x;
-        uint32_t c[4];
+        if (u >= units) break;
+        uint8_t* row = fresh + (u / per_row) * a.dim;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = encode2<CODES>(v[i][2 * e] * inverse, v[i][2 * e + 1] * inverse);
-        if (u < units) reinterpret_cast<uint2*>(fresh)[u] = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+        for (int k = 0; k < 2; ++k) {
+            float v[8];
+            widen8<TYPE>(raw[i][k], v);
+            uint32_t c[4];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] == v[e] ? v[e] * inverse : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] = encode2<CODES>(v[2 * e], v[2 * e + 1]);
+            *reinterpret_cast<uint2*>(row + (k ? unit[i].hi : unit[i].lo)) =
+                make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+        }
     }
     if (threadIdx.x == 0) *scale_at = scale;
     if (earlier > 0 && scale > was) {
         const float ratio = was * inverse;
         uint2* held = reinterpret_cast<uint2*>(codes + j * a.block * a.dim);
-        for (int u = threadIdx.x; u < earlier * per_row; u += blockDim.x) {
+        for (int u = threadIdx.x; u < earlier * (a.dim >> 3); u += blockDim.x) {
             const uint2 q = held[u];
             uint32_t o[2];
 #pragma unroll
@@ -363,9 +395,11 @@ bool aligned16(const w4a16_kv_rows& x) {
            ((x.batch_stride | x.token_stride | x.head_stride) & 7) == 0;
 }
 
-// Heads a thread takes: four where that still leaves the chip full.
+// Heads a thread takes: four where that still leaves the chip full (4022 tokens
+// of 32 heads of 128, interleaved: 13.0 us at four, 16.0 at one; 700 tokens of 32
+// heads of 64: 5.0 and 4.6).
 int heads_per_thread(int64_t batch, int64_t tokens, int64_t heads, int64_t dim) {
-    return heads >= 4 && batch * tokens * heads * (dim / 16) >= 4 * 256 * 1024 ? 4 : 1;
+    return heads >= 4 && batch * tokens * heads * (dim / 16) >= 384 * 1024 ? 4 : 1;
 }
 
 template <int TYPE, int HPT>
@@ -396,10 +430,8 @@ void launch_write_units(int upt, const WriteArgs& a, const RotaryArgs& q, int it
         WRITE_UNITS(2);
     else if (upt <= 4)
         WRITE_UNITS(4);
-    else if (upt <= 8)
-        WRITE_UNITS(8);
     else
-        WRITE_UNITS(16);
+        WRITE_UNITS(8);
 #undef WRITE_UNITS
 }
 
@@ -468,7 +500,7 @@ int write_tokens(const w4a16_kv_rows* q, void* q_out, int64_t heads, const w4a16
     a.blocks = (int)((tokens + block - 2) / block + 1);
     const int64_t items = 2 * cache->kv_heads * cache->batch * a.blocks;
     // a workgroup's rows: at most a block's; one wavefront while they fit its lanes
-    const int64_t units = (tokens < block ? tokens : block) * cache->head_dim / 8;
+    const int64_t units = (tokens < block ? tokens : block) * cache->head_dim / 16;
     const int threads = units <= 64 ? 64 : units <= 128 ? 128 : 256;
     const int upt = (int)((units + threads - 1) / threads);
     RotaryArgs r{};
