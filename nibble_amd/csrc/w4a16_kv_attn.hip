@@ -649,11 +649,12 @@ prompt_kernel(const AttnArgs a) {
             for (int i = 0; i < 8; ++i)
                 if (tile_at * KT + 16 * (vgroup >> 1) + 8 * (i >> 2) + 4 * (vgroup & 1) + (i & 3) >= end) vr[i] = 0;
         }
+        // dim 4 v + d in row d D / 4 + v: neighbouring lanes write neighbouring rows
         f16x8 value[4];
         transpose8<CODES>(vr, value);
 #pragma unroll
         for (int d = 0; d < 4; ++d)
-            *reinterpret_cast<f16x8*>(to + (4 * vdim + d) * VROW + 8 * vgroup) = value[d];
+            *reinterpret_cast<f16x8*>(to + (d * (D / 4) + vdim) * VROW + 8 * vgroup) = value[d];
     };
 #pragma unroll
     for (int i = 0; i < KL; ++i) kr[i] = (u32x4){0u, 0u, 0u, 0u};
@@ -679,35 +680,33 @@ prompt_kernel(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
 
-    // Fragments are read four ahead of the matrix instructions that take them;
-    // only vector instructions may be scheduled across (kOrder).
-    constexpr int kOrder = 0x406;
-    auto products = [&](f16x8 (&q)[D / 16], const f16* from, f32x16 (&to)[KN]) {   // scores of a tile
-        constexpr int G = KN * D / 16 / 4;
-        f16x8 frag[2][4];
-        auto read = [&](int g, f16x8 (&f)[4]) {
+    // A tile's products go in 2 KN parts of P instructions each, so that those
+    // of the next scores lie between the exponentials and the products of the
+    // present weights. Fragments are read a part ahead; across kOrder only
+    // vector instructions may be scheduled.
+    constexpr int kOrder = 0x406, P = D / 32;
+    f16x8 key[P], value[P];
+    auto read_keys = [&](const f16* from, int part) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int m = 4 * g + i;
-                f[i] = *reinterpret_cast<const f16x8*>(from + (32 * (m % KN) + n) * KROW + 16 * (m / KN) + 8 * h);
-            }
-        };
-#pragma unroll
-        for (int k = 0; k < KN; ++k)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) to[k][i] = 0.0f;
-        read(0, frag[0]);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            if (g + 1 < G) read(g + 1, frag[(g + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(kOrder);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int m = 4 * g + i;
-                to[m % KN] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[g & 1][i], q[m / KN], to[m % KN], 0, 0, 0);
-            }
-            __builtin_amdgcn_sched_barrier(kOrder);
+        for (int i = 0; i < P; ++i) {
+            const int m = P * part + i;
+            key[i] = *reinterpret_cast<const f16x8*>(from + (32 * (m % KN) + n) * KROW + 16 * (m / KN) + 8 * h);
         }
+    };
+    auto products = [&](f16x8 (&q)[D / 16], int part, f32x16 (&to)[KN]) {   // of the scores
+        if (part == 0) {
+#pragma unroll
+            for (int k = 0; k < KN; ++k)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) to[k][i] = 0.0f;
+        }
+        __builtin_amdgcn_sched_barrier(kOrder);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int m = P * part + i;
+            to[m % KN] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key[i], q[m / KN], to[m % KN], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(kOrder);
     };
     f16x8 q[D / 16];
 #pragma unroll
@@ -723,7 +722,11 @@ prompt_kernel(const AttnArgs a) {
     load_values(first + 1);
     __syncthreads();
     f32x16 st[KN], next[KN];
-    products(q, keys[0], st);
+#pragma unroll
+    for (int x = 0; x < 2 * KN; ++x) {
+        read_keys(keys[0], x);
+        products(q, x, st);
+    }
     stage_keys(keys[1]);
     load_keys(first + 2);
     __syncthreads();
@@ -746,7 +749,7 @@ prompt_kernel(const AttnArgs a) {
                     for (int i = 0; i < 16; ++i)
                         if (slot0 + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3) > last) st[k][i] = -__builtin_inff();
             }
-            products(q, keys[now ^ 1], next);   // of no use past the last tile
+            read_keys(keys[now ^ 1], 0);
             float mx = -__builtin_inff();
 #pragma unroll
             for (int x = 0; x < 2 * KN; ++x) {
@@ -769,15 +772,13 @@ prompt_kernel(const AttnArgs a) {
                 for (int d = 0; d < D / 32; ++d) acc[d] *= rescale;
             }
             const float base = run_max == -__builtin_inff() ? 0.0f : run_max;   // no slot of the row seen yet
-            f16x8 frag[2][D / 32];
-            auto read = [&](int x, f16x8 (&f)[D / 32]) {
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d)
-                    f[d] = *reinterpret_cast<const f16x8*>(values[now] + (32 * d + n) * VROW + 16 * x + 8 * h);
-            };
-            read(0, frag[0]);
 #pragma unroll
             for (int x = 0; x < 2 * KN; ++x) {
+#pragma unroll
+                for (int d = 0; d < P; ++d)
+                    value[d] = *reinterpret_cast<const f16x8*>(values[now] + (32 * d + n) * VROW + 16 * x + 8 * h);
+                products(q, x, next);   // of no use past the last tile
+                if (x + 1 < 2 * KN) read_keys(keys[now ^ 1], x + 1);
                 const float shift = vex[x] - base;
                 float sum = 0.0f;
                 u32x4 packed;
@@ -791,12 +792,11 @@ prompt_kernel(const AttnArgs a) {
                     packed[i] = as_u32((f16x2){(f16)lo, (f16)hi});
                 }
                 run_sum = __builtin_fmaf(sum, vinv[x], run_sum);
-                if (x + 1 < 2 * KN) read(x + 1, frag[(x + 1) & 1]);
                 __builtin_amdgcn_sched_barrier(kOrder);
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d)
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag[x & 1][d], __builtin_bit_cast(f16x8, packed),
-                                                                    acc[d], 0, 0, 0);
+                for (int d = 0; d < P; ++d)
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value[d], __builtin_bit_cast(f16x8, packed), acc[d],
+                                                                    0, 0, 0);
                 __builtin_amdgcn_sched_barrier(kOrder);
             }
         } else {
@@ -818,30 +818,40 @@ prompt_kernel(const AttnArgs a) {
     if (wave0 + n >= rows) return;
     run_sum = half_pair_sum(run_sum);
     const int64_t at = ((int64_t)b * a.tokens + t) * a.heads + hk * a.group + g;
+    // Row x of the values in LDS is dim 4 (x mod D / 4) + x / (D / 4), and acc[d][i]
+    // is row 32 d + 8 (i >> 2) + 4 h + (i & 3): the v-th of the D / 8 runs of four
+    // dims that a lane holds lies D / 4 rows apart.
+    auto place = [](int v) { return 32 * (v >> 4) + 8 * ((v >> 2) & 3) + (v & 3); };   // its first row, without 4 h
+    auto dim_of = [&](int v) { return 4 * (place(v) + 4 * h); };
+    auto four = [&](int v) {
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = place(v) + e * (D / 4);
+            x[e] = acc[row >> 5][4 * ((row >> 3) & 3) + (row & 3)];
+        }
+        return x;
+    };
     if (shares.count > 1) {
         const int64_t sp = at * a.splits + split;
         if (h == 0) a.states[sp] = make_float2(run_max, run_sum);
-        float* o = a.partial + sp * D + 4 * h;
+        float* o = a.partial + sp * D;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f32x4*>(o + 32 * d + 2 * i) =
-                    (f32x4){acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+        for (int v = 0; v < D / 8; ++v) {
+            const f32x4 x = four(v);
+            *reinterpret_cast<f32x4*>(o + dim_of(v)) = x;
+        }
         return;
     }
     const bool padding = t >= seen.count;
     const float inv = padding ? 0.0f : inside ? 1.0f / run_sum : __builtin_nanf("");
-    uint16_t* o = a.out + at * D + 4 * h;
+    uint16_t* o = a.out + at * D;
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = padding ? 0.0f : acc[d][i + e] * inv;
-            store4<TYPE>(o + 32 * d + 2 * i, v[0], v[1], v[2], v[3]);
-        }
+    for (int v = 0; v < D / 8; ++v) {
+        f32x4 x = four(v) * inv;
+        if (padding) x = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        store4<TYPE>(o + dim_of(v), x[0], x[1], x[2], x[3]);
+    }
 }
 
 }  // namespace w4a16
