@@ -116,7 +116,11 @@ int w4a16_kv_read(const w4a16_kv_codes* side, void* out, int64_t batch, int64_t 
  * query head h reads KV head h / (heads / kv_heads). The tokens' own keys and
  * values must be in the cache (w4a16_kv_write first). Padding rows come out
  * zero, rows at positions outside the cache NaN. Slots behind a sequence's
- * last token may hold anything.
+ * last token may hold anything; the codes of those that a row of the call sees
+ * are numbers (w4a16_kv_write writes no others: an e4m3 NaN among the values
+ * may turn other rows of the call into NaN, too).
+ * The weights enter the second product as fp16 (each off by 2^-11 of itself),
+ * scores and sums are fp32. The same call gives the same bits.
  * workspace: w4a16_kv_attention_workspace_bytes(...) bytes (0: none needed),
  * 16-byte aligned, contents ignored, not shared by calls that overlap.
  */

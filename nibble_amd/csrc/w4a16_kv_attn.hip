@@ -47,6 +47,7 @@ struct AttnArgs {
     float scale;
     int tokens, heads, kv_heads, group, block_log, splits, least, row_tiles;
     bool vec;
+    bool early;   // shares request their first chunk before `start` has arrived
 };
 
 // What a workgroup's rows see: rows row0 .. of sequence b.
@@ -166,15 +167,16 @@ constexpr float kSlack = 8.0f;
 // Decode form: up to 16 NT query rows of a KV head, every wavefront taking
 // chunks of 16 M slots.
 //
-// Bound: the cache's bytes with many sequences, the latency of a chunk (about
-// 1 us from request to weights) with few. Lane (c, h) = (lane & 15, lane >> 4).
+// Bound: the cache's bytes with many sequences (32 of 7000 tokens, 8 KV heads of
+// 128: 84.7 us, 5.5 TB/s), the latency of a chunk (about 1.5 us from request to
+// output) with few. Lane (c, h) = (lane & 15, lane >> 4).
 // Keys: 16 bytes of row c at 64 j + 16 h, so that the loads of a row read it
 // whole; values: dim / 16 bytes at dim / 16 c of the rows that the lane's
 // weights stand for (slots 32 y + 4 h + i and 32 y + 16 + 4 h + i), whole rows
 // again. The next chunk's keys are requested when the present ones are
 // multiplied, its values likewise. Wavefronts of a workgroup join through LDS;
-// the chunks of a sequence go round the shares, which merge_kernel joins. The
-// first share's first chunk does not depend on the sequence's length and is
+// the chunks of a sequence go round the shares, which merge_kernel joins. Which
+// chunk comes first does not depend on the sequence's length, so that it is
 // requested before `start` has arrived.
 // ---------------------------------------------------------------------------
 constexpr int kDecodeWaves = 4;
@@ -243,11 +245,13 @@ decode_kernel(const AttnArgs a) {
                 }
             }
     };
-    // the other shares read the first rows here and their own below: registers
-    // that only one side of a branch defines have been miscompiled
+    // (where the cache is large the other shares, which may turn out to have no
+    // slots, read the first rows here and their own below: registers that only
+    // one side of a branch defines have been miscompiled)
     int chunk = split * W + wave;
-    load_keys(split == 0 ? chunk : 0, (int)a.slots - 1);
-    load_values(split == 0 ? chunk : 0, (int)a.slots - 1);
+    const bool early = split == 0 || a.early;
+    load_keys(early ? chunk : 0, (int)a.slots - 1);
+    load_values(early ? chunk : 0, (int)a.slots - 1);
 
     u32x4 qr[NT][2 * J];
     float row_scale[NT];
@@ -274,8 +278,8 @@ decode_kernel(const AttnArgs a) {
     const int last_slot = max(end - 1, 0);
     const int chunks = (end + C - 1) / C;
     const Shares shares = shares_of(chunks, a.splits, a.least);
-    if (split > 0) {
-        if (split >= shares.count) return;
+    if (split > 0 && split >= shares.count) return;
+    if (!early) {
         load_keys(chunk, last_slot);
         load_values(chunk, last_slot);
     }
@@ -300,7 +304,9 @@ decode_kernel(const AttnArgs a) {
 #pragma unroll
         for (int m = 0; m < M; ++m) {
             ksc[m] = k_scale[m];
-            const int e = exponent_of(v_scale[m]);
+            // a tile behind the last slot may have any scale: its weights are 0, but
+            // their factor has to be a number
+            const int e = min(max(exponent_of(v_scale[m]), -100), 100);
             vex[m] = (float)e;
             vinv[m] = exp2_int(-e);
 #pragma unroll
@@ -520,13 +526,17 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, int rows_p
 }
 
 // ---------------------------------------------------------------------------
-// Prompt form: 32 W query rows of a KV head a workgroup of W wavefronts.
+// Prompt form: 32 W query rows of a KV head a workgroup, 32 a wavefront.
 //
-// Bound: the matrix cores and the softmax's vector instructions (4 dim flops
-// a pair of row and slot). Tiles of 8192 / dim slots: their codes are
-// requested into registers while the tile before is multiplied, decoded to
-// fp16 once for the workgroup's rows and kept in LDS, keys row by row, values
-// transposed with their slots in the order of the score registers.
+// Bound: the matrix cores and the softmax's vector instructions together (4 dim
+// flops a pair of row and slot; 4096 tokens of 32/8 heads of 128: 151 us, 912
+// TFLOP/s, two thirds of what an 8192^3 product reaches; the counters show the
+// matrix cores busy 36% of the time, the vector unit 42%, LDS 31%: two
+// wavefronts a SIMD, which the registers allow, do not cover each other's
+// waits). Tiles of 64 slots (32 with head_dim 256): their codes are requested
+// into registers a tile and a half ahead, decoded to fp16 once for the
+// workgroup's rows and kept in LDS, keys row by row, values transposed with
+// their slots in the order of the score registers.
 // v_mfma_f32_32x32x16_f16: lane (n, h) = (lane & 31, lane >> 5) receives the
 // scores of row n for slots 8 (i >> 2) + 4 h + (i & 3) of each 32.
 // ---------------------------------------------------------------------------
@@ -1064,6 +1074,9 @@ int w4a16_kv_attention(const w4a16_kv_rows* q, void* out, int64_t tokens, int64_
     a.block_log = cache->block == 16 ? 4 : cache->block == 32 ? 5 : cache->block == 64 ? 6 : 7;
     a.splits = p.splits;
     a.least = p.least;
+    // first chunks of up to 8 MB in all (one token over 1500 of 2048 slots, 32/4
+    // heads of 64: 7.4 against 8.1 us)
+    a.early = batch * cache->kv_heads * p.row_tiles * p.splits * 4 * p.unit * dim * 2 <= (8 << 20);
     a.row_tiles = (int)p.row_tiles;
     a.vec = (reinterpret_cast<uintptr_t>(q->data) & 15u) == 0 &&
             ((q->batch_stride | q->token_stride | q->head_stride) & 7) == 0;

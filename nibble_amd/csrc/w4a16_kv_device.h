@@ -13,7 +13,7 @@ __device__ __forceinline__ float exp2_int(int e) {   // 2^e, -126 <= e <= 127
     return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
 }
 __device__ __forceinline__ int exponent_of(float scale) {   // of a power of two
-    return (int)(__builtin_bit_cast(uint32_t, scale) >> 23) - 127;
+    return (int)((__builtin_bit_cast(uint32_t, scale) >> 23) & 255u) - 127;
 }
 
 // The smallest e in [kKvLowest, kKvHighest] with amax <= M 2^e; M = 127 is

@@ -306,6 +306,55 @@ def test_attention_ignores_what_lies_behind(gpu, codes, tokens):
     assert torch.equal(padded, torch.zeros_like(padded))
 
 
+@pytest.mark.parametrize("tokens", [1, 50])
+@pytest.mark.parametrize("slots", [90, 2000])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), float("-inf"), -3.0, 0.0, 1e-45, 3e38])
+def test_attention_ignores_scales_that_lie_behind(gpu, tokens, slots, junk):
+    """Scales of blocks without tokens are never written: memory as it was allocated."""
+    q = _kv.rows((3, tokens, 4, 64), "fp16", 57)
+    kc, ks = _kv.cache(3, 2, slots, 64, "fp8", 16, 58)
+    vc, vs = _kv.cache(3, 2, slots, 64, "fp8", 16, 59)
+    starts = [3, 17, slots // 2 - tokens]
+    want, bound = _kv.attend(q, kc, ks, vc, vs, starts, None, 16)
+    for b, start in enumerate(starts):
+        ks[b, :, -(-(start + tokens) // 16):] = junk
+        vs[b, :, -(-(start + tokens) // 16):] = junk
+    got = kv_attention_cuda(*_dev(q, kc, ks, vc, vs), torch.tensor(starts).cuda())
+    _kv.close(got, want, bound)
+
+
+@pytest.mark.parametrize("tokens", [1, 9, 60])
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+def test_attention_shares_with_padding(gpu, codes, tokens):
+    """Divided slots: padding rows, rows outside the cache, sequences of one share and of many."""
+    q = _kv.rows((5, tokens, 8, 64), "fp16", 51)
+    kc, ks = _kv.cache(5, 1, 2500, 64, codes, 32, 52)
+    vc, vs = _kv.cache(5, 1, 2500, 64, codes, 32, 53)
+    starts, counts = [2400, 3, 2495, 1200, -4], [tokens, tokens // 2, tokens, 0, tokens]
+    want, bound = _kv.attend(q, kc, ks, vc, vs, starts, counts, 32)
+    for b, (start, count) in enumerate(zip(starts, counts)):
+        end = max(start + count, 0)
+        vc[b, :, end:].view(torch.uint8).fill_(0x7F)
+    got = kv_attention_cuda(*_dev(q, kc, ks, vc, vs), torch.tensor(starts).cuda(), torch.tensor(counts).cuda())
+    _kv.close(got, want, bound)
+
+
+@pytest.mark.parametrize("dim,codes,dtype", [(64, "int8", "bf16"), (64, "fp8", "fp16"), (128, "int8", "fp16"),
+                                             (128, "fp8", "bf16")])
+def test_attention_of_many_prompts(gpu, dim, codes, dtype):
+    """Enough rows for workgroups of 256 of them; ragged, some of one sequence padding."""
+    q = _kv.rows((64, 36, 16, dim), dtype, 54)
+    kc, ks = _kv.cache(64, 8, 150, dim, codes, 64, 55)
+    vc, vs = _kv.cache(64, 8, 150, dim, codes, 64, 56)
+    starts = [(7 * b) % 100 for b in range(64)]
+    counts = [36 - b % 5 for b in range(64)]
+    got = kv_attention_cuda(*_dev(q, kc, ks, vc, vs), torch.tensor(starts).cuda(), torch.tensor(counts).cuda())
+    for b in (0, 14, 63):
+        one = slice(b, b + 1)
+        want, bound = _kv.attend(q[one], kc[one], ks[one], vc[one], vs[one], starts[one], counts[one], 64)
+        _kv.close(got[one], want, bound)
+
+
 @pytest.mark.parametrize("tokens", [1, 70])
 def test_attention_of_unequal_values(gpu, tokens):
     """Blocks of values 2^30 apart: the weights keep their precision, whichever
