@@ -21,7 +21,7 @@ from nibble_amd.integration import load_packed_state_dict, replace_linear_layers
 from nibble_amd.kv_cache import QuantizedKVCache
 from nibble_amd.linear import Int4Linear, QuantizedLinear
 from nibble_amd.quantization import pack_int4, quantize_and_pack_weights, quantize_groupwise, unpack_int4
-from nibble_amd.rotary import rope_frequencies, rope_tables, rotary
+from nibble_amd.rope import rope_frequencies, rope_tables, rotary
 
 __all__ = [
     "QuantizedLinear",

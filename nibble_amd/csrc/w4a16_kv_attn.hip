@@ -6,13 +6,13 @@
 // j's blocks, the score in powers of two is
 //     s_j = (q . code_k,j) 2^e_k scale log2(e),
 // and the value's scale joins the softmax instead of the product:
-//     w_j = s_j + e_v,   R = max_j w_j,   P_j = 2^(w_j - R) in [0, 1],
+//     w_j = s_j + e_v,   R ~ max_j w_j (kSlack),   P_j = 2^(w_j - R),
 //     o = sum_j P_j code_v,j / sum_j 2^-e_v P_j.
 // Both products run on the matrix cores with fp16 operands: codes are exact in
-// fp16, q is exact too (bf16 rows are moved into fp16's range by a power of
-// two per row), and P is the only rounding: relative 2^-11, one for each
-// weight, whatever the scales of the values are, as the largest P is 1. Scores,
-// R, both sums and the outputs are fp32.
+// fp16, q is exact too (bf16 rows are moved into fp16's range by a power of two
+// per row), and P is the only rounding: relative 2^-11, one for each weight,
+// whatever the scales of the values are, as the largest P lies between 1 and
+// 2^8. Scores, R, both sums and the outputs are fp32.
 //
 // S^T = K Q^T and O^T = V^T P^T: with keys in the rows of the first product a
 // lane receives weights of consecutive keys of its own query column, which are
@@ -127,7 +127,7 @@ __device__ __forceinline__ f16x8 decode8(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(f16x8, v);
 }
 
-// Words x[0..7] of 8 keys, 4 dims each -> for dim DD the 8 keys' values as a
+// Words x[0..7] of 8 slots, 4 dims each -> for each dim the 8 slots' values as a
 // matrix operand. Byte pairs of neighbouring keys come together by v_perm.
 template <int CODES>
 __device__ __forceinline__ void transpose8(const uint32_t (&x)[8], f16x8 (&out)[4]) {

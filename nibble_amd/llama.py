@@ -64,7 +64,7 @@ from nibble_amd.cuda import dequantize_cuda
 from nibble_amd.kv_cache import QuantizedKVCache
 from nibble_amd.linear import QuantizedLinear
 from nibble_amd.quantization import quantize_and_pack_weights
-from nibble_amd.rotary import rope_frequencies, rope_tables
+from nibble_amd.rope import rope_frequencies, rope_tables
 
 # Longest prompt the fused prefill takes where the prefill attention cannot
 # stream the caches (query heads per KV head not a power of two up to 64:
@@ -99,7 +99,7 @@ class LlamaConfig:
     init_std: float = 0.02
     kv_cache: str = "fp16"             # or "int8", "fp8": QuantizedKVCache
     kv_block: int = 64                 # slots of a scale of an 8-bit cache
-    rope_scaling: dict | None = None   # as in Hugging Face configs (nibble_amd/rotary.py)
+    rope_scaling: dict | None = None   # as in Hugging Face configs (nibble_amd/rope.py)
 
     @property
     def num_linear_layers(self) -> int:

@@ -160,7 +160,7 @@ def hf_to_decoder_state_dict(state_dict: dict, group_size: int = 128) -> dict:
     return out
 
 
-# Kinds of rope scaling that nibble_amd.rotary knows.
+# Kinds of rope scaling that nibble_amd.rope knows.
 _ROPE_SCALINGS = ("linear", "dynamic", "llama3", "yarn")
 
 

@@ -333,3 +333,12 @@ def test_fake_tensors():
         assert nibble_amd.kv_read_cuda(codes, scales, torch.float32).dtype == torch.float32
         assert nibble_amd.rotary_cuda(q[0], start, cos, cos).shape == (3, 4, 64)
         assert nibble_amd.kv_write_cuda(q[:, :, :2], q[:, :, :2], codes, scales, codes, scales, start) is None
+
+
+def test_both_import_names():
+    import w4a16
+    from w4a16.kv_cache import QuantizedKVCache as same
+    from w4a16.rope import rope_tables as tables
+
+    assert same is QuantizedKVCache is w4a16.QuantizedKVCache and tables is rope_tables
+    assert w4a16.kv_attention_cuda is nibble_amd.kv_attention_cuda and w4a16.rotary is rotary
