@@ -1024,6 +1024,7 @@ int w4a16_kv_attention(const w4a16_kv_rows* q, void* out, int64_t tokens, int64_
     if (type != W4A16_FP16 && type != W4A16_BF16) return kv_fail(W4A16_ERR_CONFIG, "queries must be fp16 or bf16");
     if (tokens < 0 || heads < 1 || heads % cache->kv_heads != 0)
         return kv_fail(W4A16_ERR_SHAPE, "heads must be a positive multiple of the cache's KV heads");
+    if (!(scale - scale == 0.0f)) return kv_fail(W4A16_ERR_CONFIG, "scale must be a finite number");
     if (!sizes_fit(cache->batch, tokens, heads, cache->kv_heads))
         return kv_fail(W4A16_ERR_TOO_LARGE, "too many tokens or heads");
     if (cache->batch == 0 || tokens == 0) return W4A16_OK;

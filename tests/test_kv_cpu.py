@@ -216,10 +216,10 @@ def _write(cache, tokens=3, type_=0, k=None, start=1 << 24):
                                      type_, None)
 
 
-def _attend(cache, tokens=1, heads=4, type_=0, out=1 << 23, q=None, workspace=None, nbytes=0):
+def _attend(cache, tokens=1, heads=4, type_=0, out=1 << 23, q=None, workspace=None, nbytes=0, scale=0.125):
     rows = _rows() if q is None else q
     return _lib.lib().w4a16_kv_attention(ctypes.byref(rows), out, tokens, heads, ctypes.byref(cache), 1 << 24, None,
-                                         0.125, type_, workspace, nbytes, None)
+                                         scale, type_, workspace, nbytes, None)
 
 
 @pytest.mark.parametrize("changes,code", [
@@ -305,6 +305,8 @@ def test_attention_refusals():
     assert _attend(_cache(), out=None) == _lib.W4A16_ERR_NULL
     assert _attend(_cache(), out=(1 << 23) + 8) == _lib.W4A16_ERR_ALIGNMENT
     assert _attend(_cache(), tokens=-1) == _lib.W4A16_ERR_SHAPE
+    for scale in (float("nan"), float("inf"), float("-inf")):
+        assert _attend(_cache(), scale=scale) == _lib.W4A16_ERR_CONFIG
     assert _attend(_cache(), tokens=0) == _lib.W4A16_OK
     wide = _cache(slots=4096, k=_side(batch_stride=1 << 20, head_stride=1 << 19),
                   v=_side(1 << 21, batch_stride=1 << 20, head_stride=1 << 19))
