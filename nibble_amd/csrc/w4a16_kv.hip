@@ -72,13 +72,13 @@ struct RotaryArgs {
     const uint16_t* x;
     uint16_t* out;
     const float *cos_table, *sin_table;
-    const int64_t* positions;    // of (b, t), or NULL: start[b] + t
+    const int64_t* positions;    // of (b, t), or, beside a write, start[b] + t
     const int64_t *start, *counts;
     int64_t xb, xt, xh, pb, pt, table_rows, slots;
     int batch, tokens, heads, dim, rot, head_groups;
 };
 
-template <int TYPE, bool INTERLEAVED, int HPT>
+template <int TYPE, bool INTERLEAVED, int HPT, bool BESIDE_WRITE>
 __device__ __forceinline__ void rotary_units(const RotaryArgs& a, int64_t first) {
     const int units = a.dim >> 4;
     const int64_t total = (int64_t)a.batch * a.tokens * a.head_groups * units;
@@ -90,6 +90,22 @@ __device__ __forceinline__ void rotary_units(const RotaryArgs& a, int64_t first)
     const int t = (int)(rest % a.tokens), b = (int)(rest / a.tokens);
 
     const Unit unit = unit_of<INTERLEAVED>(u, a.dim, a.rot);
+    uint16_t* out = a.out + ((int64_t)b * a.tokens + t) * a.heads * a.dim;
+    if (BESIDE_WRITE && a.counts != nullptr && t >= a.counts[b]) {
+        // padding: zeros, and the rows are not read
+        for (int h = hg; h < a.heads; h += a.head_groups) {
+            *reinterpret_cast<u32x4*>(out + (int64_t)h * a.dim + unit.lo) = (u32x4){0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4*>(out + (int64_t)h * a.dim + unit.hi) = (u32x4){0u, 0u, 0u, 0u};
+        }
+        return;
+    }
+    // Rows before positions where there are positions (12.5 against 14.5 us for 2 x 2011 tokens, 32 heads of 128),
+    // and after the start beside a write (37.4 against 38.7 us for 4 x 2000 tokens, 32/8 heads of 128).
+    int64_t p, limit;
+    if constexpr (BESIDE_WRITE) {
+        p = min(a.start[b], a.slots) + t;   // past the slots: outside, and no sum that wraps
+        limit = a.slots;
+    }
     u32x4 va[HPT], vb[HPT];
     const uint16_t* x = a.x + b * a.xb + t * a.xt;
 #pragma unroll
@@ -98,15 +114,10 @@ __device__ __forceinline__ void rotary_units(const RotaryArgs& a, int64_t first)
         va[i] = *reinterpret_cast<const u32x4*>(row + unit.lo);
         vb[i] = *reinterpret_cast<const u32x4*>(row + unit.hi);
     }
-    int64_t p;
-    bool padding = false;
-    int64_t limit = a.table_rows;
-    if (a.positions != nullptr) {
+    if constexpr (!BESIDE_WRITE) {
+        __builtin_amdgcn_sched_barrier(0);
         p = a.positions[b * a.pb + t * a.pt];
-    } else {
-        p = min(a.start[b], a.slots) + t;   // past the slots: outside, and no sum that wraps
-        padding = a.counts != nullptr && t >= a.counts[b];
-        limit = a.slots;
+        limit = a.table_rows;
     }
     const bool known = p >= 0 && p < limit;
     float c[8], s[8];
@@ -118,13 +129,11 @@ __device__ __forceinline__ void rotary_units(const RotaryArgs& a, int64_t first)
         c[4 + i] = known ? a.cos_table[at + unit.two + i] : __builtin_nanf("");
         s[4 + i] = known ? a.sin_table[at + unit.two + i] : __builtin_nanf("");
     }
-    uint16_t* out = a.out + ((int64_t)b * a.tokens + t) * a.heads * a.dim;
 #pragma unroll
     for (int i = 0; i < HPT; ++i) {
         const int h = hg + i * a.head_groups;
         if (h >= a.heads) break;
         rotate_unit<TYPE, INTERLEAVED>(unit, va[i], vb[i], c, s);
-        if (padding) va[i] = vb[i] = (u32x4){0u, 0u, 0u, 0u};
         uint16_t* row = out + (int64_t)h * a.dim;
         *reinterpret_cast<u32x4*>(row + unit.lo) = va[i];
         *reinterpret_cast<u32x4*>(row + unit.hi) = vb[i];
@@ -133,7 +142,7 @@ __device__ __forceinline__ void rotary_units(const RotaryArgs& a, int64_t first)
 
 template <int TYPE, bool INTERLEAVED, int HPT>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
-    rotary_units<TYPE, INTERLEAVED, HPT>(a, (int64_t)blockIdx.x * blockDim.x + threadIdx.x);
+    rotary_units<TYPE, INTERLEAVED, HPT, false>(a, (int64_t)blockIdx.x * blockDim.x + threadIdx.x);
 }
 
 // Any even rot, any head_dim and any alignment: a thread per pair or copied value.
@@ -311,7 +320,7 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteArgs a, const Rot
     if ((int)blockIdx.x < items)
         write_block<TYPE, CODES, ROTATE, INTERLEAVED, UPT>(a, blockIdx.x);
     else if constexpr (ROTATE)
-        rotary_units<TYPE, INTERLEAVED, HPT>(q, (int64_t)((int)blockIdx.x - items) * blockDim.x + threadIdx.x);
+        rotary_units<TYPE, INTERLEAVED, HPT, true>(q, (int64_t)((int)blockIdx.x - items) * blockDim.x + threadIdx.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -396,7 +405,7 @@ bool aligned16(const w4a16_kv_rows& x) {
 }
 
 // Heads a thread takes: four where that still leaves the chip full (4022 tokens
-// of 32 heads of 128, interleaved: 13.0 us at four, 16.0 at one; 700 tokens of 32
+// of 32 heads of 128, interleaved: 12.5 us at four, 16.0 at one; 700 tokens of 32
 // heads of 64: 5.0 and 4.6).
 int heads_per_thread(int64_t batch, int64_t tokens, int64_t heads, int64_t dim) {
     return heads >= 4 && batch * tokens * heads * (dim / 16) >= 384 * 1024 ? 4 : 1;
