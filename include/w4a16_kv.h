@@ -82,8 +82,10 @@ int w4a16_rotary(const w4a16_kv_rows* x, void* out, int64_t batch, int64_t token
  * tokens (slots below start). Earlier tokens' codes are rescaled where the
  * scale grows (code * old / new, rounded half to even). New codes are value /
  * scale rounded half to even and saturated; NaN becomes 0. Slots behind the
- * new tokens keep their codes. Tokens whose slot lies outside the cache are
- * not written.
+ * new tokens are taken to be free: they keep their codes, whose values change
+ * with the scale (a sequence grows, or is taken back to an earlier length and
+ * written on from there). Tokens whose slot lies outside the cache are not
+ * written.
  */
 int w4a16_kv_write(const w4a16_kv_rows* k, const w4a16_kv_rows* v, int64_t tokens, const w4a16_kv_cache* cache,
                    const int64_t* start, const int64_t* counts, int type, void* stream);

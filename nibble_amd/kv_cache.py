@@ -62,7 +62,8 @@ class QuantizedKVCache:
 
     def write(self, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, counts: torch.Tensor | None = None) -> None:
         """k, v fp16 / bf16 [batch, tokens, kv_heads, head_dim] into the slots
-        start[b] .. (int64 [batch]); the first counts[b] tokens, or all."""
+        start[b] .. (int64 [batch]); the first counts[b] tokens, or all. Slots
+        behind them are taken to be free."""
         call = kv_write_cuda if self.k_codes.is_cuda else kv_reference.kv_write_reference
         call(k, v, *self.tensors(), start, counts)
 

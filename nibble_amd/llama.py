@@ -375,6 +375,8 @@ class LlamaDecoder(torch.nn.Module):
         return self.fused and self.fuse_prefill and 1 <= tokens <= limit
 
     def _prefill(self, prompt: torch.Tensor, positions: torch.Tensor) -> None:
+        if self.kv_caches is not None and prompt.numel() > self.cfg.max_seq_len:
+            raise IndexError("the prompt is longer than the key/value cache")
         if self.fused_prefill(prompt.numel()):
             # no cache reset: every fused attention kernel selects away the
             # slots past the position it attends to, whatever they hold

@@ -57,6 +57,8 @@ def test_configs():
         LlamaDecoder(_cfg(kv_block=24), device="cpu")
     with pytest.raises(ValueError, match="unknown rope scaling"):
         LlamaDecoder(_cfg(rope_scaling={"rope_type": "other"}), device="cpu")
+    with pytest.raises(IndexError, match="longer"):
+        LlamaDecoder(_cfg(max_seq_len=8), device="cpu").prefill(_prompt(9))
     plain = LlamaDecoder(_cfg(kv_cache="fp16"), device="cpu")
     assert plain.kv_caches is None and plain.k_cache.shape[2] == 96
 
