@@ -383,8 +383,7 @@ namespace {
 
 using namespace w4a16;
 using w4a16_internal::kv_fail;
-
-constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+using w4a16_internal::launch_fits;
 
 int finish() {
     const hipError_t e = hipGetLastError();
@@ -521,10 +520,11 @@ int write_tokens(const w4a16_kv_rows* q, void* q_out, int64_t heads, const w4a16
                        cache->slots, (int)cache->batch, (int)tokens, (int)heads, (int)cache->head_dim, (int)rot, 0};
         hpt = heads_per_thread(cache->batch, tokens, heads, cache->head_dim);
         r.head_groups = (int)((heads + hpt - 1) / hpt);
-        const int64_t work = cache->batch * tokens * r.head_groups * (cache->head_dim / 16);
-        extra = (work + threads - 1) / threads;
+        const __int128 work = (__int128)cache->batch * tokens * r.head_groups * (cache->head_dim / 16);
+        if (!launch_fits(work / threads, threads)) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
+        extra = ((int64_t)work + threads - 1) / threads;
     }
-    if (items + extra > kMaxGrid) return kv_fail(W4A16_ERR_TOO_LARGE, "too many workgroups for one launch");
+    if (!launch_fits(items + extra, threads)) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool inter = interleaved != 0;
     if (type == W4A16_FP16 && cache->code_type == W4A16_KV_INT8)
@@ -629,7 +629,7 @@ int w4a16_rotary(const w4a16_kv_rows* x, void* out, int64_t batch, int64_t token
         const int hpt = heads_per_thread(batch, tokens, heads, head_dim);
         a.head_groups = (int)((heads + hpt - 1) / hpt);
         const __int128 work = (__int128)batch * tokens * a.head_groups * (head_dim / 16);
-        if (work > (__int128)kMaxGrid * 256) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
+        if (!launch_fits((work + 255) / 256, 256)) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
         const int64_t grid = ((int64_t)work + 255) / 256;
         if (type == W4A16_FP16 && hpt == 4)
             launch_rotary<W4A16_FP16, 4>(a, interleaved != 0, grid, st);
@@ -641,7 +641,7 @@ int w4a16_rotary(const w4a16_kv_rows* x, void* out, int64_t batch, int64_t token
             launch_rotary<W4A16_BF16, 1>(a, interleaved != 0, grid, st);
     } else {
         const __int128 work = (__int128)batch * tokens * heads * (head_dim - rot / 2);
-        if (work > (__int128)kMaxGrid * 256) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
+        if (!launch_fits((work + 255) / 256, 256)) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
         const int64_t grid = ((int64_t)work + 255) / 256;
         if (type == W4A16_FP16)
             launch_rotary_any<W4A16_FP16>(a, interleaved != 0, grid, st);
@@ -683,7 +683,7 @@ int w4a16_kv_read(const w4a16_kv_codes* side, void* out, int64_t batch, int64_t 
         return kv_fail(W4A16_ERR_ALIGNMENT, "out must be 16-byte aligned");
     const int64_t units = slots * (head_dim / 8);
     const int64_t chunks = (units + 256 * kReadVectors - 1) / (256 * kReadVectors);
-    if ((__int128)chunks * batch * kv_heads > kMaxGrid)
+    if (!launch_fits((__int128)chunks * batch * kv_heads, 256))
         return kv_fail(W4A16_ERR_TOO_LARGE, "too many values for one launch");
     const int64_t grid = chunks * batch * kv_heads;
     const int block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;

@@ -1042,7 +1042,9 @@ int w4a16_kv_attention(const w4a16_kv_rows* q, void* out, int64_t tokens, int64_
             return kv_fail(W4A16_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
     }
     const int64_t grid = batch * cache->kv_heads * p.row_tiles * p.splits;
-    if (grid > 0x7FFFFFFF || rows > 0x7FFFFFFF) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
+    const int threads = 64 * (p.prompt ? p.waves * p.groups : kDecodeWaves);
+    if (!w4a16_internal::launch_fits(grid, threads) || rows > 0x7FFFFFFF)
+        return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
     AttnArgs a{};
     a.q = static_cast<const uint16_t*>(q->data);
     a.out = static_cast<uint16_t*>(out);

@@ -14,4 +14,9 @@ int kv_fail(int code, const std::string& message);
 int check_kv_block(int64_t block, int code_type);
 int check_kv_cache(const w4a16_kv_cache* cache);   // a batch of 0 has no pointers to check
 
+// Whether a launch of so many workgroups is one that HIP takes (fewer than 2^32 threads).
+inline bool launch_fits(__int128 workgroups, int threads) {
+    return workgroups <= INT32_MAX && workgroups * threads <= UINT32_MAX;
+}
+
 }  // namespace w4a16_internal

@@ -265,6 +265,25 @@ def test_rotary_refusals():
     assert call(batch=0) == _lib.W4A16_OK
 
 
+def test_calls_past_a_launch_are_refused():
+    """2^32 threads or more, and products of sizes past 64 bits."""
+    rows = _rows()
+    many = dict(batch=1 << 22, kv_heads=16)
+    assert _write(_cache(**many), tokens=1) == _lib.W4A16_ERR_TOO_LARGE
+    assert _attend(_cache(**many), heads=16) == _lib.W4A16_ERR_TOO_LARGE
+    lib = _lib.lib()
+    assert lib.w4a16_rotary_kv_write(ctypes.byref(rows), 1 << 23, 1 << 16, ctypes.byref(rows), ctypes.byref(rows),
+                                     1 << 24, 1 << 22, 1 << 22, 16, 64, 0, ctypes.byref(_cache(batch=1 << 24)),
+                                     1 << 24, None, 0, None) == _lib.W4A16_ERR_TOO_LARGE
+    for offset in (0, 2):   # whole vectors, and any alignment
+        x = _rows((1 << 22) + offset)
+        assert lib.w4a16_rotary(ctypes.byref(x), 1 << 23, 1, 1 << 28, 16, 64, 1 << 22, 1 << 22, 10, 64, 1 << 24, 0, 1,
+                                0, 0, None) == _lib.W4A16_ERR_TOO_LARGE
+    side = _side()
+    assert lib.w4a16_kv_read(ctypes.byref(side), 1 << 23, 1 << 24, 1, 16, 64, 16, 0, 0,
+                             None) == _lib.W4A16_ERR_TOO_LARGE
+
+
 def test_rotary_write_refusals():
     fn = _lib.lib().w4a16_rotary_kv_write
     rows = _rows()
