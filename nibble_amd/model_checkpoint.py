@@ -160,22 +160,11 @@ def hf_to_decoder_state_dict(state_dict: dict, group_size: int = 128) -> dict:
     return out
 
 
-# Kinds of rope scaling that nibble_amd.rope knows.
-_ROPE_SCALINGS = ("linear", "dynamic", "llama3", "yarn")
-
-
 def _rope_scaling(hf_config: dict) -> dict | None:
     """The scaling of the rotary positions that a config asks for (None: none).
-    ``original_max_position_embeddings`` defaults to the config's context; a
-    kind that is not known is left out with a ``UserWarning``."""
+    ``original_max_position_embeddings`` defaults to the config's context."""
     scaling = hf_config.get("rope_scaling") or hf_config.get("rope_parameters")
-    if not scaling:
-        return None
-    kind = scaling.get("rope_type", scaling.get("type", "default"))
-    if kind == "default":
-        return None
-    if kind not in _ROPE_SCALINGS:
-        warnings.warn(f"rope scaling '{kind}' is not supported: positions stay unscaled", UserWarning, stacklevel=3)
+    if not scaling or scaling.get("rope_type", scaling.get("type", "default")) == "default":
         return None
     scaling = {key: value for key, value in scaling.items() if value is not None}
     if "max_position_embeddings" in hf_config:
@@ -183,9 +172,12 @@ def _rope_scaling(hf_config: dict) -> dict | None:
     return scaling
 
 
-def decoder_config(hf_config: dict, max_seq_len: int = 2048, kv_cache: str = "fp16"):
+def decoder_config(hf_config: dict, max_seq_len: int = 2048, kv_cache: str = "fp16", rope_scaling: bool = False):
     """``LlamaConfig`` of ``nibble_amd.llama`` from a Hugging Face Llama config
-    dict; ``kv_cache`` "int8" or "fp8" keeps the keys and values in 8 bits."""
+    dict; ``kv_cache`` "int8" or "fp8" keeps the keys and values in 8 bits,
+    ``rope_scaling`` takes the config's scaling of the rotary positions over
+    (positions stay unscaled without it; the decoder refuses a kind that it
+    does not know)."""
     from nibble_amd.llama import LlamaConfig
 
     heads = hf_config["num_attention_heads"]
@@ -195,7 +187,8 @@ def decoder_config(hf_config: dict, max_seq_len: int = 2048, kv_cache: str = "fp
         num_heads=heads, num_kv_heads=hf_config.get("num_key_value_heads", heads),
         head_dim=hf_config.get("head_dim") or hf_config["hidden_size"] // heads,
         rms_norm_eps=hf_config.get("rms_norm_eps", 1e-6), rope_theta=hf_config.get("rope_theta", 10000.0),
-        max_seq_len=max_seq_len, kv_cache=kv_cache, rope_scaling=_rope_scaling(hf_config),
+        max_seq_len=max_seq_len, kv_cache=kv_cache,
+        rope_scaling=_rope_scaling(hf_config) if rope_scaling else None,
     )
 
 

@@ -68,14 +68,17 @@ def test_checkpoint_configs():
                 max_position_embeddings=4096)
     assert mc.decoder_config(base).rope_scaling is None and mc.decoder_config(base).kv_cache == "fp16"
     assert mc.decoder_config(base, 64, kv_cache="fp8").kv_cache == "fp8"
-    assert mc.decoder_config({**base, "rope_parameters": {"rope_type": "default", "rope_theta": 1e4}}).rope_scaling is None
+    scaled = lambda config, slots=2048: mc.decoder_config(config, slots, rope_scaling=True).rope_scaling
+    assert scaled(base) is None
+    assert scaled({**base, "rope_parameters": {"rope_type": "default", "rope_theta": 1e4}}) is None
     llama = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
              "original_max_position_embeddings": 512}
-    assert mc.decoder_config({**base, "rope_scaling": llama}).rope_scaling == llama
-    dynamic = mc.decoder_config({**base, "rope_scaling": {"type": "dynamic", "factor": 2.0}}, 8192)
-    assert dynamic.rope_scaling["original_max_position_embeddings"] == 4096
-    with pytest.warns(UserWarning, match="longrope"):
-        assert mc.decoder_config({**base, "rope_scaling": {"type": "longrope"}}).rope_scaling is None
+    assert scaled({**base, "rope_scaling": llama}) == llama
+    assert mc.decoder_config({**base, "rope_scaling": llama}).rope_scaling is None
+    assert scaled({**base, "rope_scaling": {"type": "dynamic", "factor": 2.0}}, 8192)[
+        "original_max_position_embeddings"] == 4096
+    with pytest.raises(ValueError, match="longrope"):
+        LlamaDecoder(mc.decoder_config({**base, "rope_scaling": {"type": "longrope"}}, 64, rope_scaling=True), device="cpu")
 
 
 def test_scaled_positions_reach_the_tables():
