@@ -170,6 +170,7 @@ w4a16_kv_codes codes_of(const at::Tensor& codes, const at::Tensor& scales, bool 
     TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), name, " codes and scales must be CUDA tensors");
     TORCH_CHECK(codes.device() == scales.device(), name, " codes and scales must be on the same CUDA device");
     TORCH_CHECK(scales.scalar_type() == at::kFloat, name, " scales must have dtype torch.float32");
+    TORCH_CHECK(!scales.requires_grad(), name, " scales must not require grad");
     TORCH_CHECK(codes.dim() == 4, name, " codes must have shape [batch, kv_heads, slots, head_dim]");
     TORCH_CHECK(scales.dim() == 3 && scales.size(0) == codes.size(0) && scales.size(1) == codes.size(1), name,
                 " scales must have shape [batch, kv_heads, blocks]");
@@ -224,6 +225,7 @@ const int64_t* counts_of(const c10::optional<at::Tensor>& counts, int64_t batch,
 void check_tables(const at::Tensor& cos, const at::Tensor& sin, const at::Device& device) {
     TORCH_CHECK(cos.is_cuda() && cos.device() == device && sin.is_cuda() && sin.device() == device,
                 "cos and sin must be on the same CUDA device as the rows");
+    TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), "cos and sin must not require grad");
     TORCH_CHECK(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat,
                 "cos and sin must have dtype torch.float32");
     TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.is_contiguous() && sin.is_contiguous(),

@@ -66,6 +66,9 @@ def test_refusals(gpu):
     refuse("positions must have shape", rotary_cuda, q, start, cos, cos)
     refuse("positions must have dtype", rotary_cuda, q[0], torch.zeros(3, device="cuda"), cos, cos)
     refuse("dtype must be", kv_read_cuda, kc, sc, torch.float64)
+    refuse("must not require grad", kv_read_cuda, kc, sc.clone().requires_grad_())
+    refuse("must not require grad", attend, vs=vs.clone().requires_grad_())
+    refuse("must not require grad", rotate_write, cos, cos.clone().requires_grad_())
 
 
 # ------------------------------------------------------------------------------ rotary
