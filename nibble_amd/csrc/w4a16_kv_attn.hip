@@ -594,12 +594,14 @@ prompt_kernel(const AttnArgs a) {
     const int vgroup = vt / (D / 4), vdim = vt % (D / 4);   // 8 slots, 4 dims of the values
     const bool loads_keys = KW == W || wave < KW, loads_values = VW == W || wave >= W - VW;
     // one uniform base and a 32-bit offset a load, at most that of the row of slot
-    // `limit` (tiles past it read its tile's rows again)
+    // `limit` (tiles past it read its tile's rows again) and of the tile's last
+    // row: `limit` may lie more than 2^32 bytes behind the tile
+    auto last_row = [&](int tile_at, int limit) { return (uint32_t)min(limit - tile_at * KT, KT - 1) * D; };
     auto load_keys = [&](int tile_at, int limit) {
         if (!loads_keys) return;
         tile_at = min(tile_at, limit / KT);
         const uint8_t* tile0 = kc + (int64_t)tile_at * (KT * D);
-        const uint32_t most = (uint32_t)(limit - tile_at * KT) * D + 16 * (tid % (D / 16));
+        const uint32_t most = last_row(tile_at, limit) + 16 * (tid % (D / 16));
 #pragma unroll
         for (int i = 0; i < KL; ++i)
             kr[i] = *reinterpret_cast<const u32x4*>(tile0 + min((uint32_t)(16 * (tid + 64 * W * i)), most));
@@ -609,7 +611,7 @@ prompt_kernel(const AttnArgs a) {
         if (!loads_values) return;
         tile_at = min(tile_at, limit / KT);
         const uint8_t* tile0 = vc + (int64_t)tile_at * (KT * D);
-        const uint32_t most = (uint32_t)(limit - tile_at * KT) * D + 4 * vdim;
+        const uint32_t most = last_row(tile_at, limit) + 4 * vdim;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             vr[i] = *reinterpret_cast<const uint32_t*>(tile0 + min(value0 + (8 * (i >> 2) + (i & 3)) * D, most));

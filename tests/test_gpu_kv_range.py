@@ -1,0 +1,60 @@
+"""Attention over the 8-bit key/value cache at the ends of its range: caches past
+32-bit offsets within a head."""
+
+import math
+
+import pytest
+import torch
+
+from nibble_amd import kv_attention_cuda, kv_read_cuda, kv_write_cuda
+from tests import _kv
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend(q, cache, starts, counts=None, scale=None):
+    at = torch.tensor(starts).cuda()
+    limits = None if counts is None else torch.tensor(counts).cuda()
+    return kv_attention_cuda(q.cuda(), *(t.cuda() for t in cache), at, limits, scale)
+
+
+# --------------------------------------------------------------- offsets within a head
+
+@pytest.mark.parametrize("dim,slots", [(256, (1 << 24) + 5), (128, (1 << 25) + 5), (64, (1 << 26) + 5)])
+def test_prompt_in_a_head_past_32_bits(gpu, dim, slots):
+    """A prompt at the start and one at the end of a head of more than 2^32
+    bytes. Slots 0 .. 69 and the last 70 hold numbers, all between score 0 and
+    value 0."""
+    tokens = 70
+    kc, vc = (torch.zeros((2, 1, slots, dim), dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.full((2, 1, -(-slots // 64)), 2.0 ** -6, device="cuda") for _ in range(2))
+    last = slots - tokens
+    k, v = (_kv.rows((2, tokens, 1, dim), "fp16", i, spread).cuda() for i, spread in ((61, 1.0), (62, 1000.0)))
+    kv_write_cuda(k, v, kc, ks, vc, vs, torch.tensor([0, 0]).cuda())
+    kv_write_cuda(k, v, kc, ks, vc, vs, torch.tensor([last, last]).cuda())
+    q = _kv.rows((2, tokens, 2, dim), "fp16", 63)
+    got = kv_attention_cuda(q.cuda(), kc, ks, vc, vs, torch.tensor([0, last]).cuda())
+
+    def held(codes, scales, at):   # the tokens' values, from the block that `at` lies in
+        first = at - at % 64
+        end = min(first + 192, slots)
+        part = kv_read_cuda(codes[:, :, first:end], scales[:, :, first // 64:-(-end // 64)], torch.float32)
+        return part[:, 0, at - first:at - first + tokens].double().cpu()
+
+    kk, vv = ([held(c, s, at) for at in (0, last)] for c, s in ((kc, ks), (vc, vs)))
+    del kc, vc
+    causal = torch.arange(tokens) <= torch.arange(tokens).unsqueeze(1)
+    for b in range(2):
+        rows = q[b].double().transpose(0, 1)                                    # [heads, tokens, dim]
+        near = torch.exp(torch.matmul(rows, kk[b][b].t().contiguous()) / math.sqrt(dim)) * causal
+        total = near.sum(-1, keepdim=True)
+        out, size = torch.matmul(near, vv[b][b]), torch.matmul(near, vv[b][b].abs())
+        if b == 1:   # the slots at the start, seen whole, and those of weight 1 between
+            far = torch.exp(torch.matmul(rows, kk[0][1].t().contiguous()) / math.sqrt(dim))
+            total = total + far.sum(-1, keepdim=True) + (last - tokens)
+            out, size = out + torch.matmul(far, vv[0][1]), size + torch.matmul(far, vv[0][1].abs())
+        want, size = (out / total).transpose(0, 1), (size / total).transpose(0, 1)
+        # weights off by 2^-11 of themselves, scores by 2^-12 (fp32 sums of dim products of up to 2^6); a lane adds
+        # up the weights of 2^20 slots at most, 16 at a time: 2^16 additions, each off by 2^-24 of the sum so far,
+        # which is half of the whole on average: 2^-9
+        _kv.close(got[b], want.numpy(), (2.0 ** -11 + 2.0 ** -12 + 2.0 ** -9) * size.numpy(), f"sequence {b}")
