@@ -525,6 +525,79 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttnArgs a, int rows_p
                                            (parts[2][lane * E + e] + parts[3][lane * E + e])) * inv);
 }
 
+// The prompt form takes w - R in one step, (q . code_k) mul + (e_v - R), where R
+// came from w's rounded to fp32. From this size of R on their roundings together
+// reach a unit of the exponent and more, up to weights that fp16 does not hold or
+// that are all 0: a wavefront that met such an R attends its rows once more by
+// attend_row, which forms w first and takes R off after, as the decode form does.
+constexpr float kLarge = 0x1p22f;
+
+// Row r of a KV head over the slots from `lo` to `hi`, by one wavefront and in
+// fp32 throughout: a lane a slot for the scores, D / 64 dims a lane for the
+// outputs. `split` is the share, -1 where there is one. Right for scores of any
+// size, and slow: 4096 tokens of 32/8 heads of 128 in 19 ms.
+template <int D, int CODES, int TYPE>
+__device__ __forceinline__ void attend_row(const AttnArgs& a, const Seen& seen, int b, int hk, int r, int64_t lo,
+                                           int64_t hi, int split) {
+    constexpr int E = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int t = r / a.group, g = r - t * a.group;
+    const int64_t p = seen.start + t;
+    const bool inside = t < seen.count && p >= 0 && p < a.slots;
+    hi = inside ? min(hi, p + 1) : lo;
+    const uint16_t* q = a.q + b * a.qb + t * a.qt + (hk * a.group + g) * a.qh;
+    const uint8_t* kc = a.k_codes + b * a.kb + hk * a.kh;
+    const uint8_t* vc = a.v_codes + b * a.vb + hk * a.vh + lane * E;
+    const float* ks = a.k_scales + b * a.ksb + hk * a.ksh;
+    const float* vs = a.v_scales + b * a.vsb + hk * a.vsh;
+    // bf16 queries may be of any size: a power of two brings the largest to 2^14 .. 2^15
+    float amax = 0.0f;
+    for (int i = 0; i < E; ++i) amax = fmaxf(amax, fabsf(widen16<TYPE>(q[lane * E + i])));
+    const int shift = min(max(14 - exponent_of(wave_max(amax)), -120), 120);
+    const float m = exp2_int(shift), row_scale = a.scale * kLog2e * exp2_int(-shift);
+    float top = -__builtin_inff(), sum = 0.0f, o[E] = {};
+    for (int64_t slot0 = lo; slot0 < hi; slot0 += 64) {
+        const int64_t slot = min(slot0 + lane, hi - 1);
+        float dot = 0.0f;
+        for (int d = 0; d < D; d += 4) {
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(kc + slot * D + d);
+            const f32x2 x = decode2_f32<CODES, false>(word), y = decode2_f32<CODES, true>(word);
+            dot = __builtin_fmaf(widen16<TYPE>(q[d]) * m, x.x, dot);
+            dot = __builtin_fmaf(widen16<TYPE>(q[d + 1]) * m, x.y, dot);
+            dot = __builtin_fmaf(widen16<TYPE>(q[d + 2]) * m, y.x, dot);
+            dot = __builtin_fmaf(widen16<TYPE>(q[d + 3]) * m, y.y, dot);
+        }
+        const int e = exponent_of(vs[slot >> a.block_log]);
+        float w = __builtin_fmaf(dot, row_scale * ks[slot >> a.block_log], (float)e);
+        if (slot0 + lane >= hi) w = -__builtin_inff();
+        const float mx = fmaxf(wave_max(w), top);
+        const float rescale = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - mx);
+        top = mx;
+        const float weight = __builtin_amdgcn_exp2f(w - top);
+        sum = __builtin_fmaf(sum, rescale, weight * exp2_int(-e));
+        for (int i = 0; i < E; ++i) o[i] *= rescale;
+        const int n = (int)min(hi - slot0, (int64_t)64);
+        for (int j = 0; j < n; ++j) {
+            const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), j));
+            uint32_t word = 0;
+            for (int i = 0; i < E; ++i) word |= (uint32_t)vc[(slot0 + j) * D + i] << (8 * i);
+            const f32x2 lower = decode2_f32<CODES, false>(word), upper = decode2_f32<CODES, true>(word);
+            const float value[4] = {lower.x, lower.y, upper.x, upper.y};
+            for (int i = 0; i < E; ++i) o[i] = __builtin_fmaf(x, value[i], o[i]);
+        }
+    }
+    sum = wave_sum(sum);
+    const int64_t at = ((int64_t)b * a.tokens + t) * a.heads + hk * a.group + g;
+    if (split >= 0) {
+        const int64_t sp = at * a.splits + split;
+        for (int i = 0; i < E; ++i) a.partial[sp * D + lane * E + i] = o[i];
+        if (lane == 0) a.states[sp] = make_float2(top, sum);
+        return;
+    }
+    const float inv = t >= seen.count ? 0.0f : inside ? 1.0f / sum : __builtin_nanf("");
+    for (int i = 0; i < E; ++i) a.out[at * D + lane * E + i] = (uint16_t)narrow16<TYPE>(o[i] * inv);
+}
+
 // ---------------------------------------------------------------------------
 // Prompt form: 32 W query rows of a KV head a workgroup, 32 a wavefront.
 //
@@ -861,6 +934,18 @@ prompt_kernel(const AttnArgs a) {
         run_sum = run_sum * f0 + other[64] * f1;
 #pragma unroll
         for (int i = 0; i < A; ++i) acc[i >> 4][i & 15] = acc[i >> 4][i & 15] * f0 + other[64 * (2 + i)] * f1;
+    }
+    // R only grows: what a large one before the last has left is multiplied by 0, and shows if it is not finite
+    float finite = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) finite = __builtin_fmaf(acc[d][i], 0.0f, finite);
+    if (__any(fabsf(run_max) < __builtin_inff() && (fabsf(run_max) >= kLarge || finite != 0.0f))) {
+        for (int row = wave0; row < min(wave0 + 32, rows); ++row)
+            attend_row<D, CODES, TYPE>(a, seen, b, hk, row, (int64_t)split * shares.size * KT, (int64_t)stop * KT,
+                                       shares.count > 1 ? split : -1);
+        return;
     }
     if (wave0 + n >= rows) return;
     const int64_t at = ((int64_t)b * a.tokens + t) * a.heads + hk * a.group + g;

@@ -1,8 +1,9 @@
 """Attention over the 8-bit key/value cache at the ends of its range: caches past
-32-bit offsets within a head."""
+32-bit offsets within a head, scores of any size."""
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -58,3 +59,37 @@ def test_prompt_in_a_head_past_32_bits(gpu, dim, slots):
         # up the weights of 2^20 slots at most, 16 at a time: 2^16 additions, each off by 2^-24 of the sum so far,
         # which is half of the whole on average: 2^-9
         _kv.close(got[b], want.numpy(), (2.0 ** -11 + 2.0 ** -12 + 2.0 ** -9) * size.numpy(), f"sequence {b}")
+
+
+# ------------------------------------------------------------------ scores of any size
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("codes,dim", [("int8", 64), ("fp8", 128), ("int8", 256)])
+@pytest.mark.parametrize("power", [6, 14, 18, 22, 28])
+@pytest.mark.parametrize("tokens", [2, 80])
+def test_large_scores(gpu, tokens, power, codes, dim, dtype):
+    """Scores of 2^18 to 2^40: a softmax that is one-hot wherever two scores
+    differ by more than their fp32 sums can be off."""
+    slots, block = 300, 16
+    q = (_kv.rows((1, tokens, 4, dim), "fp32", 65) * 1000).to(_kv.TYPES[dtype])
+    kc, ks = _kv.cache(1, 2, slots, dim, codes, block, 66)
+    vc, vs = _kv.cache(1, 2, slots, dim, codes, block, 67)
+    ks *= 2.0 ** power
+    got = _kv.numbers(_attend(q, (kc, ks, vc, vs), [slots - tokens]))[0]
+    assert np.isfinite(got).all()
+    keys, values = _kv.values(kc, ks, block)[0], _kv.values(vc, vs, block)[0]
+    rows = _kv.numbers(q)[0]
+    checked = 0
+    for t in range(tokens):
+        for h in range(4):
+            kk, vv = keys[h // 2, :slots - tokens + t + 1], values[h // 2, :slots - tokens + t + 1]
+            s = kk @ rows[t, h] * dim ** -0.5
+            slip = (dim + 4) * 2.0 ** -24 * (np.abs(kk) @ np.abs(rows[t, h])).max() * dim ** -0.5
+            best = int(np.argmax(s))
+            assert (np.abs(got[t, h]) <= np.abs(vv).max(axis=0) * (1 + 2.0 ** -8)).all()
+            if s[best] - np.delete(s, best).max() > 2 * slip + 40:   # the rest weighs less than 300 e^-40
+                half = _kv.HALF_STEP[q.dtype]
+                # the one weight cancels up to the fp16 rounding of both
+                assert (np.abs(got[t, h] - vv[best]) <= (2.0 ** -11 + half * 1.01) * np.abs(vv[best]) + 1e-7).all()
+                checked += 1
+    assert checked > 2 * tokens
