@@ -121,8 +121,11 @@ int w4a16_kv_read(const w4a16_kv_codes* side, void* out, int64_t batch, int64_t 
  * last token may hold anything; the codes of those that a row of the call sees
  * are numbers (w4a16_kv_write writes no others: an e4m3 NaN among the values
  * may turn other rows of the call into NaN, too).
- * The weights enter the second product as fp16 (each off by 2^-11 of itself),
- * scores and sums are fp32. The same call gives the same bits.
+ * Scores and sums are fp32. In the second product a weight times its value's
+ * scale is an fp16 number: off by 2^-11 of itself down to 2^-21 of the row's
+ * largest, by 2^-32 of the largest below. bf16 queries enter the first one as
+ * fp16 times a power of two per row: exact down to 2^-31 of the row's largest
+ * value, off by 2^-39 of it below. The same call gives the same bits.
  * workspace: w4a16_kv_attention_workspace_bytes(...) bytes (0: none needed),
  * 16-byte aligned, contents ignored, not shared by calls that overlap.
  */

@@ -6,13 +6,14 @@
 // j's blocks, the score in powers of two is
 //     s_j = (q . code_k,j) 2^e_k scale log2(e),
 // and the value's scale joins the softmax instead of the product:
-//     w_j = s_j + e_v,   R ~ max_j w_j (kSlack),   P_j = 2^(w_j - R),
+//     w_j = s_j + e_v,   R ~ max_j w_j - 7,   P_j = 2^(w_j - R),
 //     o = sum_j P_j code_v,j / sum_j 2^-e_v P_j.
-// Both products run on the matrix cores with fp16 operands: codes are exact in
-// fp16, q is exact too (bf16 rows are moved into fp16's range by a power of two
-// per row), and P is the only rounding: relative 2^-11, one for each weight,
-// whatever the scales of the values are, as the largest P lies between 1 and
-// 2^8. Scores, R, both sums and the outputs are fp32.
+// Both products run on the matrix cores with fp16 operands. Codes are exact in
+// fp16, fp16 queries too; bf16 rows are moved into fp16's range by a power of
+// two per row, exact for values down to 2^-31 of the row's largest and off by
+// 2^-39 of it below. P is rounded to fp16, by 2^-11 of itself for weights down
+// to 2^-21 of the row's largest P, by 2^-32 of that below (kBelow). Scores, R,
+// both sums and the outputs are fp32.
 //
 // S^T = K Q^T and O^T = V^T P^T: with keys in the rows of the first product a
 // lane receives weights of consecutive keys of its own query column, which are
@@ -158,10 +159,17 @@ __device__ __forceinline__ float larger(float a, float b) {
     return __builtin_amdgcn_fmed3f(a, b, __builtin_inff());
 }
 
-// A row's reference R of the weights 2^(w - R) follows its largest w only when
-// that has grown by this much: weights are then up to 2^8 and keep their
-// precision, and the outputs are rarely rescaled.
-constexpr float kSlack = 8.0f;
+// A row's reference R of the weights 2^(w - R) lies kBelow under its largest w,
+// and follows that only when a weight would pass 2^kMost, so that the outputs
+// are rarely rescaled. fp16 ends at 2^16 and is normal down to 2^-14: a weight
+// is off by 2^-11 of itself down to 2^-21 of the row's largest, below by 2^-32
+// of the largest. (With R at the largest w, weights under 2^-25 of it are lost:
+// a prompt's row over 131071 slots of score 0 and one of score 17.5 whose value
+// is 0 came out 0 where 0.026 was right.)
+constexpr float kBelow = 7.0f, kMost = 15.0f;
+
+// R after larger weights w <= mx came: -inf as long as there were none.
+__device__ __forceinline__ float reference(float mx, float before) { return fmaxf(mx - kBelow, before); }
 
 // ---------------------------------------------------------------------------
 // Decode form: up to 16 NT query rows of a KV head, every wavefront taking
@@ -338,8 +346,8 @@ decode_kernel(const AttnArgs a) {
                     mx = larger(mx, w);
                 }
             mx = row_pair_max(mx);
-            if (__any(mx > run_max[n] + kSlack)) {
-                mx = fmaxf(mx, run_max[n]);
+            if (__any(mx - run_max[n] > kMost)) {
+                mx = reference(mx, run_max[n]);
                 const float rescale = mx == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(run_max[n] - mx);
                 run_max[n] = mx;
                 run_sum[n] *= rescale;
@@ -860,8 +868,8 @@ prompt_kernel(const AttnArgs a) {
             stage_values(values[now ^ 1], at + KS);
             load_keys(at + 3 * KS, last_slot);
             load_values(at + 2 * KS, last_slot);
-            if (__any(mx > run_max + kSlack)) {
-                mx = fmaxf(mx, run_max);
+            if (__any(mx - run_max > kMost)) {
+                mx = reference(mx, run_max);
                 const float rescale = mx == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(run_max - mx);
                 run_max = mx;
                 run_sum *= rescale;

@@ -1,5 +1,6 @@
 """Attention over the 8-bit key/value cache at the ends of its range: caches past
-32-bit offsets within a head, scores of any size."""
+32-bit offsets within a head, weights far below a row's largest, scores of any
+size."""
 
 import math
 
@@ -59,6 +60,37 @@ def test_prompt_in_a_head_past_32_bits(gpu, dim, slots):
         # up the weights of 2^20 slots at most, 16 at a time: 2^16 additions, each off by 2^-24 of the sum so far,
         # which is half of the whole on average: 2^-9
         _kv.close(got[b], want.numpy(), (2.0 ** -11 + 2.0 ** -12 + 2.0 ** -9) * size.numpy(), f"sequence {b}")
+
+
+# ----------------------------------------------------- weights far below the largest one
+
+@pytest.mark.parametrize("gap", [10.0, 16.0, 17.5, 19.0])
+@pytest.mark.parametrize("codes,dim", [("int8", 64), ("fp8", 128), ("int8", 256)])
+@pytest.mark.parametrize("batch,kv_heads,tokens", [(1, 1, 1), (32, 8, 1), (1, 1, 70), (64, 8, 70)])
+def test_weights_behind_a_sink(gpu, batch, kv_heads, tokens, codes, dim, gap):
+    """131072 slots, one of score `gap` whose value is zero and the others of
+    score 0: the output is made of weights exp(-gap) of the largest. In shares,
+    and (many sequences, which read one cache) by a workgroup alone."""
+    slots = 131072
+    kc, vc = torch.zeros((1, 1, slots, dim), dtype=_kv.CODES[codes]), torch.zeros((1, 1, slots, dim))
+    kc[0, 0, 0] = torch.ones(dim).to(kc.dtype)
+    vc[0, 0, 1:] = torch.randint(1, 16, (slots - 1, dim), generator=_kv.gen(64)).float()
+    ks = torch.ones((1, 1, slots // 64))
+    cache = [t.cuda().expand(batch, kv_heads, *t.shape[2:]) for t in (kc, ks, vc.to(kc.dtype), ks)]
+    q = torch.full((batch, tokens, 2 * kv_heads, dim), gap / dim ** 0.5).half()   # q.k scale = gap up to q's rounding
+    scores = float(q[0, 0, 0, 0]) * dim * dim ** -0.5
+    got = _attend(q, cache, [slots - tokens] * batch)
+    seen = torch.arange(slots - tokens + 1, slots + 1)                 # slots of each row
+    weight = math.exp(-scores)
+    sums = torch.cumsum(vc[0, 0].double(), dim=0)[seen - 1]
+    want = weight * sums / (1.0 + weight * (seen.double().unsqueeze(1) - 1.0))
+    want = want.unsqueeze(1).expand(batch, tokens, 2 * kv_heads, dim).numpy()
+    # each weight off by 2^-11 of itself, or by 2^-25 where the largest is at least 2^7: 2^-32 of the largest times
+    # the largest value (16); its exponent, up to 28, by 28 2^-24 and two roundings more; the fp32 sums of each
+    # lane, at most slots / 32 additions, by 2^-24 each
+    bound = ((2.0 ** -11 + 40 * 2.0 ** -24 + slots / 32 * 2.0 ** -24) * want + slots * 2.0 ** -32 * 16
+             / (1.0 + weight * (slots - 1)))
+    _kv.close(got, want, bound)
 
 
 # ------------------------------------------------------------------ scores of any size
