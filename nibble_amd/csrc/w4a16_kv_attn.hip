@@ -770,14 +770,14 @@ prompt_kernel(const AttnArgs a) {
     float row_scale = a.scale * kLog2e * query_to_f16<TYPE>(qr, half_pair_max);
     // the largest score of a block is that of its largest product, and a masked
     // one stays -inf: a negative scale goes to q, and a factor too small to keep
-    // its product with a scale of 2^-40 normal is raised (it makes scores of
-    // 2^-10 at most of what it would have made smaller still)
+    // its product with a scale of 2^-40 normal is raised (queries, codes and scales
+    // at their ends then make scores of 2^-13, where they were to be smaller still)
     if (a.scale < 0.0f) {
         row_scale = -row_scale;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) qr[s] ^= 0x80008000u;
     }
-    row_scale = fmaxf(row_scale, 0x1p-80f);
+    row_scale = fmaxf(row_scale, 0x1p-86f);
     float run_max = -__builtin_inff(), run_sum = 0.0f;
     f32x16 acc[D / 32];
 #pragma unroll

@@ -1,6 +1,6 @@
 """Attention over the 8-bit key/value cache at the ends of its range: caches past
-32-bit offsets within a head, weights far below a row's largest, scores of any
-size."""
+32-bit offsets within a head, weights far below a row's largest, scores and
+scale factors of any size."""
 
 import math
 
@@ -125,3 +125,22 @@ def test_large_scores(gpu, tokens, power, codes, dim, dtype):
                 assert (np.abs(got[t, h] - vv[best]) <= (2.0 ** -11 + half * 1.01) * np.abs(vv[best]) + 1e-7).all()
                 checked += 1
     assert checked > 2 * tokens
+
+
+@pytest.mark.parametrize("scale", [1e-30, -1e-30, 1e-38])
+@pytest.mark.parametrize("tokens", [2, 80])
+def test_tiny_scale(gpu, tokens, scale):
+    """The largest codes and queries under a factor that makes all scores 0 to
+    fp32: every weight is the same."""
+    dim, slots = 256, 160
+    kc = torch.full((1, 1, slots, dim), 448.0)
+    kc[:, :, 1::2] = -448.0
+    kc = kc.to(torch.float8_e4m3fn)
+    vc = torch.sign(kc.float()).to(torch.float8_e4m3fn)
+    ks, vs = torch.full((1, 1, 10), 2.0 ** 40), torch.ones((1, 1, 10))
+    q = torch.full((1, tokens, 1, dim), 65504.0).half()
+    got = _attend(q, (kc, ks, vc, vs), [slots - tokens], scale=scale)
+    seen = np.arange(slots - tokens + 1, slots + 1)
+    want = np.broadcast_to((seen % 2 / seen)[:, None, None], (tokens, 1, dim))   # +1 and -1 in turn
+    # weights off by 2^-11, and by ln 2 times the exponents' 2^-13.2 where the factor is raised
+    _kv.close(got[0], want, 2.0 ** -11 + 2.0 ** -13)
