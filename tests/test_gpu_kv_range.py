@@ -1,6 +1,6 @@
 """Attention over the 8-bit key/value cache at the ends of its range: caches past
 32-bit offsets within a head, weights far below a row's largest, scores and
-scale factors of any size."""
+scale factors of any size, prompts of the widest heads in shares."""
 
 import math
 
@@ -144,3 +144,16 @@ def test_tiny_scale(gpu, tokens, scale):
     want = np.broadcast_to((seen % 2 / seen)[:, None, None], (tokens, 1, dim))   # +1 and -1 in turn
     # weights off by 2^-11, and by ln 2 times the exponents' 2^-13.2 where the factor is raised
     _kv.close(got[0], want, 2.0 ** -11 + 2.0 ** -13)
+
+
+# --------------------------------------------------------- the widest heads, in shares
+
+@pytest.mark.parametrize("codes,dtype", [("int8", "fp16"), ("fp8", "bf16")])
+@pytest.mark.parametrize("tokens,starts,counts", [(70, [1900, 3, 0], [70, 41, 0]), (150, [1500, 1990, -7], None)])
+def test_prompt_of_256_dims_in_shares(gpu, tokens, starts, counts, codes, dtype):
+    """Prompts behind held tokens in a cache of 2100 slots: the slots are
+    divided, sequences of one share and of several, padding, rows outside."""
+    q = _kv.rows((3, tokens, 2, 256), dtype, 68)
+    cache = (*_kv.cache(3, 1, 2100, 256, codes, 32, 69), *_kv.cache(3, 1, 2100, 256, codes, 32, 70))
+    want, bound = _kv.attend(q, *cache, starts, counts, 32)
+    _kv.close(_attend(q, cache, starts, counts), want, bound)
