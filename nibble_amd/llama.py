@@ -262,16 +262,17 @@ class LlamaDecoder(torch.nn.Module):
             raise ValueError("an 8-bit kv_cache on the GPU needs head_dim 64, 128 or 256")
         frequencies, rope_factor = rope_frequencies(cfg.head_dim, cfg.rope_theta, cfg.rope_scaling, cfg.max_seq_len)
         # The fused step is HIP-only (CPU runs the torch ops) and built for
-        # head_dim 64 (64, 128 and 256 over an 8-bit cache) and rows of K <= 16384.
+        # head_dim 64 (64, 128 and 256 over an 8-bit cache), rows of K <= 16384
+        # and groups of 128: its GEMVs find the scales of no other size.
         self.fused = (fused and device.type == "cuda" and cfg.head_dim in ((64, 128, 256) if quantized else (64,))
-                      and max(cfg.hidden_size, cfg.intermediate_size) <= 16384)
+                      and max(cfg.hidden_size, cfg.intermediate_size) <= 16384 and cfg.group_size == 128)
         # attention + o projection as one launch (positions < 64): head layouts
         # the kernel supports
         # (over the fp16 cache, rotating by inv_freq alone: without a factor on the tables)
         self.attn_o = (self.fused and fuse_attention_o and not quantized and rope_factor == 1.0
                        and cfg.num_kv_heads in (1, 2, 4, 8)
                        and cfg.num_heads % cfg.num_kv_heads == 0 and cfg.num_heads // cfg.num_kv_heads <= 16
-                       and cfg.num_heads * cfg.head_dim <= 4096 and cfg.group_size == 128)
+                       and cfg.num_heads * cfg.head_dim <= 4096)
         gen = torch.Generator(device=device).manual_seed(seed) if init == "random" else None
         if gen is None:
             table = torch.empty((cfg.vocab_size, cfg.hidden_size), dtype=torch.float16, device=device)
