@@ -85,7 +85,8 @@ int w4a16_rotary(const w4a16_kv_rows* x, void* out, int64_t batch, int64_t token
  * new tokens are taken to be free: they keep their codes, whose values change
  * with the scale (a sequence grows, or is taken back to an earlier length and
  * written on from there). Tokens whose slot lies outside the cache are not
- * written.
+ * written. Rows of codes and of scales share no memory with each other, keys
+ * with values among them (strides that interleave them are fine).
  */
 int w4a16_kv_write(const w4a16_kv_rows* k, const w4a16_kv_rows* v, int64_t tokens, const w4a16_kv_cache* cache,
                    const int64_t* start, const int64_t* counts, int type, void* stream);

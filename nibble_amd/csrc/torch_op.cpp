@@ -158,15 +158,7 @@ int64_t block_of(int64_t slots, int64_t blocks) {
     return 0;
 }
 
-// Whether no two of the rows that a call writes share memory.
-bool disjoint(int64_t batch, int64_t batch_stride, int64_t heads, int64_t head_stride, int64_t row) {
-    if (batch <= 1) return heads <= 1 || head_stride >= row;
-    if (heads <= 1) return batch_stride >= row;
-    if (batch_stride >= head_stride) return head_stride >= row && batch_stride >= (heads - 1) * head_stride + row;
-    return batch_stride >= row && head_stride >= (batch - 1) * batch_stride + row;
-}
-
-w4a16_kv_codes codes_of(const at::Tensor& codes, const at::Tensor& scales, bool written, const char* name) {
+w4a16_kv_codes codes_of(const at::Tensor& codes, const at::Tensor& scales, const char* name) {
     TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), name, " codes and scales must be CUDA tensors");
     TORCH_CHECK(codes.device() == scales.device(), name, " codes and scales must be on the same CUDA device");
     TORCH_CHECK(scales.scalar_type() == at::kFloat, name, " scales must have dtype torch.float32");
@@ -179,15 +171,8 @@ w4a16_kv_codes codes_of(const at::Tensor& codes, const at::Tensor& scales, bool 
     TORCH_CHECK(scales.size(2) <= 1 || scales.stride(2) == 1, name, " scales must be contiguous in blocks");
     TORCH_CHECK(block_of(codes.size(2), scales.size(2)) != 0 || codes.size(2) == 0, name,
                 " scales must hold one scale for every 16, 32, 64 or 128 slots");
-    const w4a16_kv_codes c{codes.data_ptr(), scales.data_ptr<float>(), stride_of(codes, 0), stride_of(codes, 1),
-                           stride_of(scales, 0), stride_of(scales, 1)};
-    if (written) {
-        const int64_t row = codes.size(2) * codes.size(3);
-        TORCH_CHECK(disjoint(codes.size(0), c.batch_stride, codes.size(1), c.head_stride, row) &&
-                        disjoint(codes.size(0), c.scale_batch_stride, codes.size(1), c.scale_head_stride, scales.size(2)),
-                    name, " codes and scales that are written must not overlap themselves");
-    }
-    return c;
+    return {codes.data_ptr(), scales.data_ptr<float>(), stride_of(codes, 0), stride_of(codes, 1),
+            stride_of(scales, 0), stride_of(scales, 1)};
 }
 
 struct Cache {
@@ -196,15 +181,12 @@ struct Cache {
 };
 
 Cache cache_of(const at::Tensor& k_codes, const at::Tensor& k_scales, const at::Tensor& v_codes,
-               const at::Tensor& v_scales, bool written) {
-    const w4a16_kv_codes k = codes_of(k_codes, k_scales, written, "key"), v = codes_of(v_codes, v_scales, written, "value");
+               const at::Tensor& v_scales) {
+    const w4a16_kv_codes k = codes_of(k_codes, k_scales, "key"), v = codes_of(v_codes, v_scales, "value");
     TORCH_CHECK(k_codes.device() == v_codes.device(), "keys and values must be on the same CUDA device");
     TORCH_CHECK(k_codes.scalar_type() == v_codes.scalar_type(), "key and value codes must have the same dtype");
     TORCH_CHECK(k_codes.sizes() == v_codes.sizes() && k_scales.sizes() == v_scales.sizes(),
                 "key and value codes and scales must have the same shapes");
-    TORCH_CHECK(!written || k_codes.numel() == 0 ||
-                    (k_codes.data_ptr() != v_codes.data_ptr() && k_scales.data_ptr() != v_scales.data_ptr()),
-                "keys and values must not share memory");
     return {{k, v, k_codes.size(0), k_codes.size(1), k_codes.size(2), k_codes.size(3),
              block_of(k_codes.size(2), k_scales.size(2)), code_type(k_codes, "codes")},
             k_codes.device()};
@@ -268,7 +250,7 @@ at::Tensor rotary(const at::Tensor& x, const at::Tensor& positions, const at::Te
 
 void kv_write(const at::Tensor& k, const at::Tensor& v, at::Tensor k_codes, at::Tensor k_scales, at::Tensor v_codes,
               at::Tensor v_scales, const at::Tensor& start, const c10::optional<at::Tensor>& counts) {
-    const Cache cache = cache_of(k_codes, k_scales, v_codes, v_scales, true);
+    const Cache cache = cache_of(k_codes, k_scales, v_codes, v_scales);
     TORCH_CHECK(k.dim() == 4, "k must have shape [batch, tokens, heads, head_dim]");
     const w4a16_kv_rows kr = token_rows(k, cache, k.size(1), cache.abi.kv_heads, "k");
     const w4a16_kv_rows vr = token_rows(v, cache, k.size(1), cache.abi.kv_heads, "v");
@@ -285,7 +267,7 @@ at::Tensor rotary_kv_write(const at::Tensor& q, const at::Tensor& k, const at::T
                            const at::Tensor& sin, at::Tensor k_codes, at::Tensor k_scales, at::Tensor v_codes,
                            at::Tensor v_scales, const at::Tensor& start, const c10::optional<at::Tensor>& counts,
                            bool interleaved) {
-    const Cache cache = cache_of(k_codes, k_scales, v_codes, v_scales, true);
+    const Cache cache = cache_of(k_codes, k_scales, v_codes, v_scales);
     TORCH_CHECK(q.dim() == 4, "q must have shape [batch, tokens, heads, head_dim]");
     const int64_t tokens = q.size(1);
     const w4a16_kv_rows qr = token_rows(q, cache, tokens, -1, "q");
@@ -307,7 +289,7 @@ at::Tensor rotary_kv_write(const at::Tensor& q, const at::Tensor& k, const at::T
 }
 
 at::Tensor kv_read(const at::Tensor& codes, const at::Tensor& scales, at::ScalarType dtype) {
-    const w4a16_kv_codes side = codes_of(codes, scales, false, "the");
+    const w4a16_kv_codes side = codes_of(codes, scales, "the");
     const int type = code_type(codes, "codes");
     TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16 || dtype == at::kFloat,
                 "dtype must be torch.float16, torch.bfloat16 or torch.float32");
@@ -325,7 +307,7 @@ at::Tensor kv_read(const at::Tensor& codes, const at::Tensor& scales, at::Scalar
 at::Tensor kv_attention(const at::Tensor& q, const at::Tensor& k_codes, const at::Tensor& k_scales,
                         const at::Tensor& v_codes, const at::Tensor& v_scales, const at::Tensor& start,
                         const c10::optional<at::Tensor>& counts, c10::optional<double> scale) {
-    const Cache cache = cache_of(k_codes, k_scales, v_codes, v_scales, false);
+    const Cache cache = cache_of(k_codes, k_scales, v_codes, v_scales);
     TORCH_CHECK(q.dim() == 4, "q must have shape [batch, tokens, heads, head_dim]");
     const int64_t tokens = q.size(1), heads = q.size(2);
     const w4a16_kv_rows qr = token_rows(q, cache, tokens, -1, "q");

@@ -3,8 +3,10 @@
 // the cache is in w4a16_kv_attn.hip.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
+#include <utility>
 
 #include "w4a16_hip.h"
 #include "w4a16_kv_device.h"
@@ -458,6 +460,79 @@ void launch_write(bool rotate, bool interleaved, int hpt, int upt, const WriteAr
         launch_write_units<TYPE, CODES, true, false, 4>(upt, a, q, items, grid, threads, st);
 }
 
+// Memory that a write call changes: rows of `row` bytes, n[0] groups of n[1]
+// of them, step[0] and step[1] bytes apart, ascending from `base`.
+struct Region {
+    __int128 base, row, step[2];
+    int64_t n[2];
+};
+
+Region region_of(const void* data, int64_t row, int64_t batch, int64_t batch_stride, int64_t heads, int64_t head_stride,
+                 int64_t size) {
+    Region r{(__int128)reinterpret_cast<uintptr_t>(data), (__int128)row * size,
+             {(__int128)batch_stride * size, (__int128)head_stride * size}, {batch, heads}};
+    for (int i = 0; i < 2; ++i) {
+        if (r.n[i] == 1) r.step[i] = 0;
+        if (r.step[i] < 0) {
+            r.base += r.step[i] * (r.n[i] - 1);
+            r.step[i] = -r.step[i];
+        }
+    }
+    if (r.n[0] == 1 || (r.n[1] > 1 && r.step[0] < r.step[1])) {
+        std::swap(r.step[0], r.step[1]);
+        std::swap(r.n[0], r.n[1]);
+    }
+    return r;
+}
+
+__int128 extent(const Region& r) { return r.step[0] * (r.n[0] - 1) + r.step[1] * (r.n[1] - 1) + r.row; }
+
+// Whether no two of its rows share memory.
+bool disjoint(const Region& r) {
+    return (r.n[1] == 1 || r.step[1] >= r.row) && (r.n[0] == 1 || r.step[0] >= r.step[1] * (r.n[1] - 1) + r.row);
+}
+
+// Whether a row of one shares memory with a row of the other, both disjoint in
+// themselves: for each row of `a` the last row of `b` that starts at or before
+// it, and the first that starts behind it.
+bool meet(const Region& a, const Region& b) {
+    if (a.base + extent(a) <= b.base || b.base + extent(b) <= a.base) return false;
+    for (int64_t i = 0; i < a.n[0]; ++i)
+        for (int64_t j = 0; j < a.n[1]; ++j) {
+            const __int128 x = a.base + a.step[0] * i + a.step[1] * j;
+            if (x < b.base) {
+                if (x + a.row > b.base) return true;
+                continue;
+            }
+            const __int128 g = b.n[0] == 1 ? 0 : std::min<__int128>((x - b.base) / b.step[0], b.n[0] - 1);
+            const __int128 group = b.base + g * b.step[0];
+            const __int128 k = b.n[1] == 1 ? 0 : std::min<__int128>((x - group) / b.step[1], b.n[1] - 1);
+            const __int128 before = group + k * b.step[1];
+            if (before + b.row > x) return true;
+            if (k + 1 < b.n[1] ? before + b.step[1] < x + a.row : g + 1 < b.n[0] && group + b.step[0] < x + a.row) return true;
+        }
+    return false;
+}
+
+// Workgroups write their own block each: blocks that share memory would race.
+int check_written(const w4a16_kv_cache& c) {
+    const int64_t blocks = (c.slots + c.block - 1) / c.block;
+    Region r[4];
+    for (int i = 0; i < 2; ++i) {
+        const w4a16_kv_codes& side = i ? c.v : c.k;
+        r[i] = region_of(side.codes, c.slots * c.head_dim, c.batch, side.batch_stride, c.kv_heads, side.head_stride, 1);
+        r[2 + i] = region_of(side.scales, blocks, c.batch, side.scale_batch_stride, c.kv_heads, side.scale_head_stride, 4);
+    }
+    for (int i = 0; i < 4; ++i)
+        if (!disjoint(r[i]))
+            return kv_fail(W4A16_ERR_CONFIG, "codes and scales that are written must not overlap themselves");
+    for (int i = 0; i < 4; ++i)
+        for (int j = i + 1; j < 4; ++j)
+            if (meet(r[i], r[j]))
+                return kv_fail(W4A16_ERR_CONFIG, "keys and values, codes and scales must not share memory");
+    return W4A16_OK;
+}
+
 // Keys and values into the cache, and (q != NULL) the rotation of q and k.
 int write_tokens(const w4a16_kv_rows* q, void* q_out, int64_t heads, const w4a16_kv_rows* k, const w4a16_kv_rows* v,
                  int64_t tokens, const float* cos_table, const float* sin_table, int64_t table_rows, int64_t rot,
@@ -477,6 +552,7 @@ int write_tokens(const w4a16_kv_rows* q, void* q_out, int64_t heads, const w4a16
     if (cache->batch == 0 || tokens == 0) return W4A16_OK;
     if ((rc = check_rows(k, "k")) != W4A16_OK || (rc = check_rows(v, "v")) != W4A16_OK) return rc;
     if (start == nullptr) return kv_fail(W4A16_ERR_NULL, "start must be non-NULL");
+    if ((rc = check_written(*cache)) != W4A16_OK) return rc;
     if (q != nullptr) {
         if ((rc = check_rows(q, "q")) != W4A16_OK) return rc;
         if (q_out == nullptr || cos_table == nullptr || sin_table == nullptr)
