@@ -552,6 +552,18 @@ int write_tokens(const w4a16_kv_rows* q, void* q_out, int64_t heads, const w4a16
     if (cache->batch == 0 || tokens == 0) return W4A16_OK;
     if ((rc = check_rows(k, "k")) != W4A16_OK || (rc = check_rows(v, "v")) != W4A16_OK) return rc;
     if (start == nullptr) return kv_fail(W4A16_ERR_NULL, "start must be non-NULL");
+    const int64_t block = cache->block;
+    const int64_t blocks = (tokens + block - 2) / block + 1;   // most that a sequence's tokens touch
+    const int64_t items = 2 * cache->kv_heads * cache->batch * blocks;
+    // a workgroup's rows: at most a block's; one wavefront while they fit its lanes
+    const int64_t units = (tokens < block ? tokens : block) * cache->head_dim / 16;
+    const int threads = units <= 64 ? 64 : units <= 128 ? 128 : 256;
+    const int upt = (int)((units + threads - 1) / threads);
+    const int hpt = q == nullptr || heads == 0 ? 1 : heads_per_thread(cache->batch, tokens, heads, cache->head_dim);
+    const int64_t head_groups = (heads + hpt - 1) / hpt;
+    const __int128 work = q == nullptr ? 0 : (__int128)cache->batch * tokens * head_groups * (cache->head_dim / 16);
+    const __int128 extra = (work + threads - 1) / threads;
+    if (!launch_fits(items + extra, threads)) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
     if ((rc = check_written(*cache)) != W4A16_OK) return rc;
     if (q != nullptr) {
         if ((rc = check_rows(q, "q")) != W4A16_OK) return rc;
@@ -580,37 +592,24 @@ int write_tokens(const w4a16_kv_rows* q, void* q_out, int64_t heads, const w4a16
     a.dim = (int)cache->head_dim;
     a.block = (int)cache->block;
     a.rot = (int)rot;
-    const int64_t block = cache->block;
-    a.blocks = (int)((tokens + block - 2) / block + 1);
-    const int64_t items = 2 * cache->kv_heads * cache->batch * a.blocks;
-    // a workgroup's rows: at most a block's; one wavefront while they fit its lanes
-    const int64_t units = (tokens < block ? tokens : block) * cache->head_dim / 16;
-    const int threads = units <= 64 ? 64 : units <= 128 ? 128 : 256;
-    const int upt = (int)((units + threads - 1) / threads);
+    a.blocks = (int)blocks;
     RotaryArgs r{};
-    int hpt = 1;
-    int64_t extra = 0;
-    if (q != nullptr && heads > 0) {
+    if (q != nullptr && heads > 0)
         r = RotaryArgs{static_cast<const uint16_t*>(q->data), static_cast<uint16_t*>(q_out), cos_table, sin_table,
                        nullptr, start, counts, q->batch_stride, q->token_stride, q->head_stride, 0, 0, table_rows,
-                       cache->slots, (int)cache->batch, (int)tokens, (int)heads, (int)cache->head_dim, (int)rot, 0};
-        hpt = heads_per_thread(cache->batch, tokens, heads, cache->head_dim);
-        r.head_groups = (int)((heads + hpt - 1) / hpt);
-        const __int128 work = (__int128)cache->batch * tokens * r.head_groups * (cache->head_dim / 16);
-        if (!launch_fits(work / threads, threads)) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
-        extra = ((int64_t)work + threads - 1) / threads;
-    }
-    if (!launch_fits(items + extra, threads)) return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
+                       cache->slots, (int)cache->batch, (int)tokens, (int)heads, (int)cache->head_dim, (int)rot,
+                       (int)head_groups};
+    const int64_t grid = items + (int64_t)extra;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool inter = interleaved != 0;
     if (type == W4A16_FP16 && cache->code_type == W4A16_KV_INT8)
-        launch_write<W4A16_FP16, W4A16_KV_INT8>(q != nullptr, inter, hpt, upt, a, r, (int)items, items + extra, threads, st);
+        launch_write<W4A16_FP16, W4A16_KV_INT8>(q != nullptr, inter, hpt, upt, a, r, (int)items, grid, threads, st);
     else if (type == W4A16_FP16)
-        launch_write<W4A16_FP16, W4A16_KV_FP8>(q != nullptr, inter, hpt, upt, a, r, (int)items, items + extra, threads, st);
+        launch_write<W4A16_FP16, W4A16_KV_FP8>(q != nullptr, inter, hpt, upt, a, r, (int)items, grid, threads, st);
     else if (cache->code_type == W4A16_KV_INT8)
-        launch_write<W4A16_BF16, W4A16_KV_INT8>(q != nullptr, inter, hpt, upt, a, r, (int)items, items + extra, threads, st);
+        launch_write<W4A16_BF16, W4A16_KV_INT8>(q != nullptr, inter, hpt, upt, a, r, (int)items, grid, threads, st);
     else
-        launch_write<W4A16_BF16, W4A16_KV_FP8>(q != nullptr, inter, hpt, upt, a, r, (int)items, items + extra, threads, st);
+        launch_write<W4A16_BF16, W4A16_KV_FP8>(q != nullptr, inter, hpt, upt, a, r, (int)items, grid, threads, st);
     return finish();
 }
 

@@ -8,22 +8,20 @@ import pytest
 
 from nibble_amd import _lib
 
-SLOTS, DIM, BLOCK = 16, 256, 16
+SLOTS, DIM, BLOCK = 16, 64, 16
 ROW = SLOTS * DIM
 
 
 def _write(k, v, batch, heads):
     """A write call's answer about the sides (codes address and strides, scales
-    address and strides): its message, or '' where it is refused only for its
-    size, after all that is asked here (nothing is launched)."""
+    address and strides): its message, or '' where it goes on to the queries,
+    which are misaligned (nothing is launched)."""
     sides = [_lib.KVCodes(c[0], s[0], c[1], c[2], s[1], s[2]) for c, s in (k, v)]
     cache = _lib.KVCache(*sides, batch, heads, SLOTS, DIM, BLOCK, 0)
-    rows = _lib.KVRows(1 << 40, 4096, 256, 64)
-    tokens = 1 << 24   # 2^20 blocks x 2 sides x 16 heads in all x 256 threads: past a launch
-    assert batch * heads >= 16
-    code = _lib.lib().w4a16_kv_write(ctypes.byref(rows), ctypes.byref(rows), tokens, ctypes.byref(cache), 1 << 41, None,
-                                     0, None)
-    if code == _lib.W4A16_ERR_TOO_LARGE:
+    rows, queries = _lib.KVRows(1 << 40, 4096, 256, 64), _lib.KVRows((1 << 40) + 2, 4096, 256, 64)
+    code = _lib.lib().w4a16_rotary_kv_write(ctypes.byref(queries), 1 << 42, 4, ctypes.byref(rows), ctypes.byref(rows), 3,
+                                            1 << 43, 1 << 43, SLOTS, DIM, 0, ctypes.byref(cache), 1 << 41, None, 0, None)
+    if code == _lib.W4A16_ERR_ALIGNMENT:
         return ""
     assert code == _lib.W4A16_ERR_CONFIG
     return _lib.last_error()
