@@ -375,9 +375,14 @@ class LlamaDecoder(torch.nn.Module):
         limit = self.cfg.max_seq_len if streams else min(self.cfg.max_seq_len, FUSED_PREFILL_MAX_TOKENS)
         return self.fused and self.fuse_prefill and 1 <= tokens <= limit
 
+    def _need_slots(self, slots: int, what: str) -> None:
+        """Positions past an 8-bit cache are not written and attend to nothing:
+        refused here, by the host's count, as no launch tells of them."""
+        if self.kv_caches is not None and slots > self.cfg.max_seq_len:
+            raise IndexError(f"{what} longer than the key/value cache ({slots} slots of {self.cfg.max_seq_len})")
+
     def _prefill(self, prompt: torch.Tensor, positions: torch.Tensor) -> None:
-        if self.kv_caches is not None and prompt.numel() > self.cfg.max_seq_len:
-            raise IndexError("the prompt is longer than the key/value cache")
+        self._need_slots(prompt.numel(), "the prompt is")
         if self.fused_prefill(prompt.numel()):
             # no cache reset: every fused attention kernel selects away the
             # slots past the position it attends to, whatever they hold
@@ -496,6 +501,7 @@ class LlamaDecoder(torch.nn.Module):
         prompt is copied into a static buffer before each replay). Sets the
         token and position like a prefill does; the torch-op prefill also
         resets the KV caches."""
+        self._need_slots(prompt_len, "the prompt is")
         device = self.token.device
         # Every tensor the graph reads must outlive it: the token and position
         # buffers are attributes (a local allocated before the capture would be
@@ -583,6 +589,7 @@ class LlamaDecoder(torch.nn.Module):
     @torch.inference_mode()
     def step(self) -> torch.Tensor:
         """One eager decode step; returns the new token."""
+        self._need_slots(self.host_position + 1, "the sequence is")
         self._step()
         self.host_position += 1
         return self.token.clone()
@@ -663,6 +670,7 @@ class LlamaDecoder(torch.nn.Module):
     def replay(self) -> None:
         """One decode step: the captured graph for the current position."""
         assert self.graph is not None, "call capture() first"
+        self._need_slots(self.host_position + 1, "the sequence is")
         if self.graph_short is not None and self.short_step():
             self.graph_short.replay()
         else:
@@ -691,7 +699,9 @@ class LlamaDecoder(torch.nn.Module):
     @torch.inference_mode()
     def generate(self, prompt: torch.Tensor, new_tokens: int, use_graph: bool = True) -> torch.Tensor:
         """Greedy decode: prefill, then new_tokens - 1 decode steps (several per
-        graph replay when capture(tokens_per_replay > 1) recorded them)."""
+        graph replay when capture(tokens_per_replay > 1) recorded them). The
+        last token is returned, not run: prompt and new_tokens - 1 slots."""
+        self._need_slots(prompt.numel() + max(new_tokens - 1, 0), "prompt and new tokens are")
         out = [self.prefill(prompt)]
         left = new_tokens - 1
         while left > 0:
