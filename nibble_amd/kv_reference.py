@@ -59,8 +59,27 @@ def rotary_reference(x, positions, cos, sin, interleaved=False):
     return torch.cat((turned.to(x.dtype), x[..., rot:]), dim=-1)
 
 
+def _check_lengths(x, batch: int, name: str) -> None:
+    if x.dtype != torch.int64:
+        raise TypeError(f"{name} must have dtype torch.int64")
+    if x.shape != (batch,):
+        raise ValueError(f"{name} must have shape [batch]")
+
+
+def _check_rows(x, name: str, codes, tokens: int, heads: int | None = None) -> None:
+    """Rows [batch, tokens, heads, head_dim] that go with a cache's codes, as the GPU ops ask for them."""
+    if x.dim() != 4 or x.shape[0] != codes.shape[0] or x.shape[1] != tokens or x.shape[3] != codes.shape[3] or (
+            heads is not None and x.shape[2] != heads):
+        raise ValueError(f"{name} must have shape [batch, tokens, heads, head_dim] of the cache and of the other rows")
+    if x.requires_grad:
+        raise ValueError(f"{name} must not require grad")
+
+
 def _spans(start, counts, batch: int, tokens: int):
     """(first position, tokens that are no padding) of each sequence."""
+    _check_lengths(start, batch, "start")
+    if counts is not None:
+        _check_lengths(counts, batch, "counts")
     begins = [int(p) for p in start]
     if counts is None:
         return [(p, tokens) for p in begins]
@@ -93,14 +112,22 @@ def _write_side(x, codes, scales, b, start, count):
 
 
 def kv_write_reference(k, v, k_codes, k_scales, v_codes, v_scales, start, counts=None):
-    for b, (first, count) in enumerate(_spans(start, counts, k.shape[0], k.shape[1])):
+    batch, kv_heads = k_codes.shape[:2]
+    for x, name in ((k, "k"), (v, "v")):
+        _check_rows(x, name, k_codes, k.shape[1], kv_heads)
+    for b, (first, count) in enumerate(_spans(start, counts, batch, k.shape[1])):
         _write_side(k[b], k_codes, k_scales, b, first, count)
         _write_side(v[b], v_codes, v_scales, b, first, count)
 
 
 def rotary_kv_write_reference(q, k, v, cos, sin, k_codes, k_scales, v_codes, v_scales, start, counts=None,
                               interleaved=False):
-    tokens, slots = q.shape[1], k_codes.shape[2]
+    tokens, (batch, kv_heads, slots) = q.shape[1], k_codes.shape[:3]
+    for x, name, heads in ((q, "q", None), (k, "k", kv_heads), (v, "v", kv_heads)):
+        _check_rows(x, name, k_codes, tokens, heads)
+    _spans(start, counts, batch, tokens)
+    if cos.shape[0] < slots:
+        raise ValueError("the rotary tables must have a row for every slot")
     positions = start.unsqueeze(1) + torch.arange(tokens)
     outside = torch.full_like(positions, -1)
     positions = torch.where(positions < slots, positions, outside)
@@ -121,12 +148,15 @@ def kv_read_reference(codes, scales, dtype=torch.float16):
 
 
 def kv_attention_reference(q, k_codes, k_scales, v_codes, v_scales, start, counts=None, scale=None):
+    _check_rows(q, "q", k_codes, q.shape[1])
     batch, tokens, heads, dim = q.shape
     kv_heads, slots = k_codes.shape[1], k_codes.shape[2]
-    if heads % kv_heads != 0:
+    if heads == 0 or heads % kv_heads != 0:
         raise ValueError("heads must be a positive multiple of the cache's KV heads")
     group = heads // kv_heads
     scale = dim ** -0.5 if scale is None else scale
+    if not math.isfinite(scale):
+        raise ValueError("scale must be a finite number")
     out = torch.zeros_like(q, memory_format=torch.contiguous_format)
     for b, (first, count) in enumerate(_spans(start, counts, batch, tokens)):
         end = min(max(first + count, 0), slots)
