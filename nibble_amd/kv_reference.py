@@ -41,14 +41,18 @@ def encode(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 def rotary_reference(x, positions, cos, sin, interleaved=False):
     if positions.dtype != torch.int64:
         raise TypeError("positions must have dtype torch.int64")
+    if x.dim() not in (3, 4):
+        raise ValueError("x must have shape [tokens, heads, head_dim] or [batch, tokens, heads, head_dim]")
+    if positions.shape not in (x.shape[-3:-2], x.shape[:-2]):
+        raise ValueError("positions must have shape [tokens] or [batch, tokens]")
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        raise ValueError("cos and sin must have shape [positions, rotated dims / 2]")
     rot = 2 * cos.shape[1]
     if rot < 2 or rot > x.shape[-1]:
         raise ValueError("the rotated part must be an even number of at most head_dim dims")
     known = (positions >= 0) & (positions < cos.shape[0])
-    at = positions.clamp(0, max(cos.shape[0] - 1, 0))
-    nan = torch.tensor(float("nan"))
-    c = torch.where(known.unsqueeze(-1), cos[at], nan).unsqueeze(-2)
-    s = torch.where(known.unsqueeze(-1), sin[at], nan).unsqueeze(-2)
+    at = torch.where(known, positions, cos.shape[0])   # a row of NaN behind the tables
+    c, s = (torch.cat((table, table.new_full((1, rot // 2), float("nan"))))[at].unsqueeze(-2) for table in (cos, sin))
     part = x[..., :rot].float()
     if interleaved:
         x1, x2 = part[..., 0::2], part[..., 1::2]

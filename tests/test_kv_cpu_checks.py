@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from nibble_amd import QuantizedKVCache, rope_tables
+from nibble_amd import QuantizedKVCache, rope_tables, rotary
 from tests import _kv
 
 
@@ -60,3 +60,30 @@ def test_rows_of_another_cache_are_refused(parts):
         with pytest.raises(ValueError, match="must not require grad"):
             call()
     assert all(torch.equal(a, b) for a, b in zip(before, cache.tensors()))
+
+
+def test_rotary_positions_of_another_shape_are_refused():
+    """[1] and [batch, 1] used to be taken for all tokens."""
+    x = _kv.rows((2, 4, 3, 64), "fp16", 4)
+    cos, sin = rope_tables(64, 10)
+    good = torch.tensor([0, 9, 3, 3])
+    assert _kv.same(rotary(x, good, cos, sin), rotary(x, good.expand(2, 4), cos, sin))
+    assert _kv.same(rotary(x[0], good, cos, sin), rotary(x, good, cos, sin)[0])
+    for rows, bad in ((x, good[:1]), (x, good[:2].unsqueeze(1)), (x, good.expand(1, 4)), (x, good[0]), (x[0], good.expand(2, 4)),
+                      (x[0], good.unsqueeze(0))):
+        with pytest.raises(ValueError, match="positions must have shape"):
+            rotary(rows, bad, cos, sin)
+    with pytest.raises(ValueError, match="x must have shape"):
+        rotary(x[0, 0], good[0], cos, sin)
+    for tables in ((cos, sin[:9]), (cos[0], sin[0])):
+        with pytest.raises(ValueError, match="cos and sin"):
+            rotary(x, good, *tables)
+
+
+def test_rotary_without_table_rows():
+    """Every position lies outside: NaN in the rotated dims, as on the GPU."""
+    x = _kv.rows((4, 2, 64), "fp16", 5)
+    cos, sin = rope_tables(16, 0)
+    got = rotary(x, torch.tensor([0, 1, -1, 5]), cos, sin)
+    assert torch.isnan(got[..., :16]).all() and torch.equal(got[..., 16:], x[..., 16:])
+    assert rotary(x[:0], torch.zeros(0, dtype=torch.int64), cos, sin).shape == (0, 2, 64)
