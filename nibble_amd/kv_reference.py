@@ -51,8 +51,11 @@ def rotary_reference(x, positions, cos, sin, interleaved=False):
     if rot < 2 or rot > x.shape[-1]:
         raise ValueError("the rotated part must be an even number of at most head_dim dims")
     known = (positions >= 0) & (positions < cos.shape[0])
-    at = torch.where(known, positions, cos.shape[0])   # a row of NaN behind the tables
-    c, s = (torch.cat((table, table.new_full((1, rot // 2), float("nan"))))[at].unsqueeze(-2) for table in (cos, sin))
+    if cos.shape[0] == 0:
+        c = s = torch.full((*positions.shape, 1, rot // 2), float("nan"))
+    else:
+        at, nan = positions.clamp(0, cos.shape[0] - 1), torch.tensor(float("nan"))
+        c, s = (torch.where(known.unsqueeze(-1), table[at], nan).unsqueeze(-2) for table in (cos, sin))
     part = x[..., :rot].float()
     if interleaved:
         x1, x2 = part[..., 0::2], part[..., 1::2]
