@@ -175,18 +175,22 @@ def _rope_scaling(hf_config: dict) -> dict | None:
 def decoder_config(hf_config: dict, max_seq_len: int = 2048, kv_cache: str = "fp16", rope_scaling: bool = False):
     """``LlamaConfig`` of ``nibble_amd.llama`` from a Hugging Face Llama config
     dict; ``kv_cache`` "int8" or "fp8" keeps the keys and values in 8 bits,
-    ``rope_scaling`` takes the config's scaling of the rotary positions over
-    (positions stay unscaled without it; the decoder refuses a kind that it
-    does not know)."""
+    ``rope_scaling`` takes the config's scaling of the rotary positions over,
+    and a theta that stands in the same dict (``rope_parameters``, where newer
+    configs have both). Without it positions stay unscaled and theta is the
+    config's own entry or 10000. The decoder refuses a kind that it does not know."""
     from nibble_amd.llama import LlamaConfig
 
     heads = hf_config["num_attention_heads"]
+    theta = hf_config.get("rope_theta", 10000.0)
+    if rope_scaling and "rope_theta" not in hf_config:
+        theta = (hf_config.get("rope_parameters") or {}).get("rope_theta", theta)
     return LlamaConfig(
         vocab_size=hf_config["vocab_size"], hidden_size=hf_config["hidden_size"],
         intermediate_size=hf_config["intermediate_size"], num_layers=hf_config["num_hidden_layers"],
         num_heads=heads, num_kv_heads=hf_config.get("num_key_value_heads", heads),
         head_dim=hf_config.get("head_dim") or hf_config["hidden_size"] // heads,
-        rms_norm_eps=hf_config.get("rms_norm_eps", 1e-6), rope_theta=hf_config.get("rope_theta", 10000.0),
+        rms_norm_eps=hf_config.get("rms_norm_eps", 1e-6), rope_theta=theta,
         max_seq_len=max_seq_len, kv_cache=kv_cache,
         rope_scaling=_rope_scaling(hf_config) if rope_scaling else None,
     )
