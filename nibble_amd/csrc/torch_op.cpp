@@ -162,7 +162,7 @@ w4a16_kv_codes codes_of(const at::Tensor& codes, const at::Tensor& scales, const
     TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), name, " codes and scales must be CUDA tensors");
     TORCH_CHECK(codes.device() == scales.device(), name, " codes and scales must be on the same CUDA device");
     TORCH_CHECK(scales.scalar_type() == at::kFloat, name, " scales must have dtype torch.float32");
-    TORCH_CHECK(!scales.requires_grad(), name, " scales must not require grad");
+    TORCH_CHECK(!codes.requires_grad() && !scales.requires_grad(), name, " codes and scales must not require grad");
     TORCH_CHECK(codes.dim() == 4, name, " codes must have shape [batch, kv_heads, slots, head_dim]");
     TORCH_CHECK(scales.dim() == 3 && scales.size(0) == codes.size(0) && scales.size(1) == codes.size(1), name,
                 " scales must have shape [batch, kv_heads, blocks]");

@@ -4,7 +4,7 @@ work, layouts that overlap are refused before a launch."""
 import pytest
 import torch
 
-from nibble_amd import kv_write_cuda, rotary_kv_write_cuda
+from nibble_amd import kv_attention_cuda, kv_read_cuda, kv_write_cuda, rotary_kv_write_cuda
 from tests import _kv
 
 pytestmark = pytest.mark.gpu
@@ -47,3 +47,16 @@ def test_overlapping_views_are_refused(gpu):
             rotary_kv_write_cuda(k, k, k, cos, sin, *cache, start)
     torch.cuda.synchronize()
     assert _kv.same(codes, before)
+
+
+def test_codes_that_require_grad_are_refused(gpu):
+    """e4m3 codes can: the attention would return outputs without a gradient."""
+    k = _kv.rows((2, 4, 3, 64), "fp16", 75).cuda()
+    start = torch.zeros(2, dtype=torch.int64, device="cuda")
+    codes, scales = (t.cuda() for t in _kv.cache(2, 3, 50, 64, "fp8", 16, 76))
+    other, own = codes.clone(), scales.clone()
+    leaf = codes.clone().requires_grad_()
+    for call in (lambda: kv_attention_cuda(k, codes, scales, leaf, own, start), lambda: kv_read_cuda(leaf, scales),
+                 lambda: kv_write_cuda(k, k, leaf, scales, other, own, start)):
+        with pytest.raises(RuntimeError, match="must not require grad"):
+            call()
