@@ -199,7 +199,7 @@ struct WriteArgs {
     const int64_t *start, *counts;
     const float *cos_table, *sin_table;   // of the keys, or NULL
     int64_t slots;
-    int tokens, kv_heads, batch, dim, block, blocks, rot;   // blocks: most that a sequence's tokens touch
+    int tokens, kv_heads, batch, dim, block, rot;
 };
 
 template <int TYPE, int CODES, bool ROTATE, bool INTERLEAVED, int UPT>
@@ -348,7 +348,6 @@ read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales,
         raw[i] = src[u];
         scale[i] = sc[(u / (dim >> 3)) >> block_log];
     }
-    constexpr float most = OUT == W4A16_FP16 ? 65504.0f : 3.3895313892515355e38f;
 #pragma unroll
     for (int i = 0; i < kReadVectors; ++i) {
         const int64_t u = first + 256 * i;
@@ -372,7 +371,7 @@ read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales,
             if constexpr (OUT == W4A16_FP16) {   // bf16 holds every code * scale's magnitude
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    x[e] = __builtin_fabsf(x[e]) > most ? __builtin_copysignf(most, x[e]) : x[e];
+                    x[e] = __builtin_fabsf(x[e]) > 65504.0f ? __builtin_copysignf(65504.0f, x[e]) : x[e];
             }
             static_cast<u32x4*>(out)[at] = narrow8<OUT>(x);
         }
@@ -592,7 +591,6 @@ int write_tokens(const w4a16_kv_rows* q, void* q_out, int64_t heads, const w4a16
     a.dim = (int)cache->head_dim;
     a.block = (int)cache->block;
     a.rot = (int)rot;
-    a.blocks = (int)blocks;
     RotaryArgs r{};
     if (q != nullptr && heads > 0)
         r = RotaryArgs{static_cast<const uint16_t*>(q->data), static_cast<uint16_t*>(q_out), cos_table, sin_table,

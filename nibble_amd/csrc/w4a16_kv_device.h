@@ -95,17 +95,6 @@ __device__ __forceinline__ u32x4 load8(const uint16_t* p, bool vec) {
     for (int i = 0; i < 4; ++i) r[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
     return r;
 }
-__device__ __forceinline__ void store8(uint16_t* p, u32x4 v, bool vec) {
-    if (vec) {
-        *reinterpret_cast<u32x4*>(p) = v;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        p[2 * i] = (uint16_t)v[i];
-        p[2 * i + 1] = (uint16_t)(v[i] >> 16);
-    }
-}
 template <int TYPE>
 __device__ __forceinline__ void widen8(u32x4 v, float (&x)[8]) {
 #pragma unroll
