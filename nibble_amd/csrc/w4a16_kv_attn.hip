@@ -612,7 +612,7 @@ __device__ __forceinline__ void attend_row(const AttnArgs& a, const Seen& seen, 
 // Bound: the matrix cores and the softmax's vector instructions together (4 dim
 // flops a pair of row and slot; 4096 tokens of 32/8 heads of 128: 151 us, 912
 // TFLOP/s, two thirds of what an 8192^3 product reaches; the counters show the
-// matrix cores busy 36% of the time, the vector unit 42%, LDS 31%: two
+// matrix cores busy 45% of the time, the vector unit 54%, LDS 31%: two
 // wavefronts a SIMD, which the registers allow, do not cover each other's
 // waits). Tiles of 64 slots (32 with head_dim 256): their codes are requested
 // into registers a tile and a half ahead, decoded to fp16 once for the
@@ -1026,6 +1026,9 @@ AttnPlan plan_attention(int64_t batch, int64_t tokens, int64_t heads, int64_t kv
     p.waves = dim <= 128 && batch * kv_heads * ((rows + 255) / 256) >= 512 ? 8 : 4;
     p.rows_per = p.prompt ? 32 * p.waves : 16 * p.column_tiles;
     p.row_tiles = (rows + p.rows_per - 1) / p.rows_per;
+    // The rules below know the cache's capacity, not the sequences' lengths, which
+    // are on the device: a short prompt in a long cache is planned as a long one.
+    // It uses one share then, but the merge is launched and returns at once.
     // Shares of the slots, where the rows alone leave the chip empty. Each writes
     // fp32 outputs and all bring the merge's launch (3 us, 5 to 8 with a prompt's
     // rows).

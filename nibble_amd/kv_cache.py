@@ -2,8 +2,8 @@
 
 Codes are int8 or e4m3 (``dtype`` "int8" / "fp8"), one byte a value, with a
 power-of-two fp32 scale for each ``block_size`` slots of a sequence's KV head.
-int8 keeps an absolute step per block (at most 1/127 of its largest value, at
-least half of that), e4m3 a relative one (2^-4). Half of the bytes of an fp16
+int8 keeps an absolute step per block (at least 1/127 of its largest value and
+less than 2/127), e4m3 a relative one (2^-3). Half of the bytes of an fp16
 cache, so half of what a decode step reads of it.
 
 GPU tensors run the HIP kernels (``torch.ops.w4a16.kv_write`` and so on; head

@@ -87,3 +87,12 @@ def test_rotary_without_table_rows():
     got = rotary(x, torch.tensor([0, 1, -1, 5]), cos, sin)
     assert torch.isnan(got[..., :16]).all() and torch.equal(got[..., 16:], x[..., 16:])
     assert rotary(x[:0], torch.zeros(0, dtype=torch.int64), cos, sin).shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_gradient_is_the_rotation_back(interleaved):
+    cos, sin = rope_tables(16, 10)
+    x = _kv.rows((4, 2, 24), "fp32", 6).requires_grad_()
+    weights, at = _kv.rows((4, 2, 24), "fp32", 7), torch.tensor([0, 9, 3, 3])
+    (rotary(x, at, cos, sin, interleaved) * weights).sum().backward()
+    assert torch.allclose(x.grad, rotary(weights, at, cos, -sin, interleaved), rtol=0, atol=4 * 2.0 ** -24 * 20)
