@@ -127,6 +127,46 @@ def test_large_scores(gpu, tokens, power, codes, dim, dtype):
     assert checked > 2 * tokens
 
 
+@pytest.mark.parametrize("codes,dim,heads,kv_heads", [("int8", 64, 4, 1), ("fp8", 128, 4, 2), ("int8", 128, 32, 8),
+                                                      ("fp8", 256, 2, 1)])
+@pytest.mark.parametrize("slots", [700, 2500])
+def test_large_scores_of_ragged_prompts(gpu, slots, codes, dim, heads, kv_heads):
+    """Large and ordinary scores side by side, in shares of the slots and in
+    groups of wavefronts: padding rows, rows outside the cache, sequences of one
+    share and of several."""
+    tokens, block = 90, 32
+    starts, counts = [slots - 80, 3, 0, -4, slots // 2], [tokens, 41, 0, tokens, tokens]
+    q = _kv.rows((5, tokens, heads, dim), "bf16", 77)
+    q[:, ::3] *= 2.0 ** 30
+    kc, ks = _kv.cache(5, kv_heads, slots, dim, codes, block, 78)
+    vc, vs = _kv.cache(5, kv_heads, slots, dim, codes, block, 79)
+    want, bound = _kv.attend(q, kc, ks, vc, vs, starts, counts, block)
+    got = _attend(q, (kc, ks, vc, vs), starts, counts)
+    large = torch.zeros(q.shape, dtype=torch.bool)
+    large[:, ::3] = True
+    keep = ~large.numpy()
+    assert np.array_equal(np.isnan(_kv.numbers(got)), np.isnan(want))
+    _kv.close(got.cpu().masked_fill(large, 0.0), np.where(keep, want, 0.0), np.where(keep, bound, 0.0))
+    # large scores: the first by far takes all
+    group, checked = heads // kv_heads, 0
+    keys, values, rows, out = _kv.values(kc, ks, block), _kv.values(vc, vs, block), _kv.numbers(q), _kv.numbers(got)
+    for b, (start, count) in enumerate(zip(starts, counts)):
+        for t in range(0, tokens, 3):
+            if t >= count:
+                assert (out[b, t] == 0).all()
+            elif 0 <= start + t < slots:
+                for h in range(heads):
+                    kk, vv = keys[b, h // group, :start + t + 1], values[b, h // group, :start + t + 1]
+                    s = kk @ rows[b, t, h] * dim ** -0.5
+                    slip = (dim + 4) * 2.0 ** -24 * (np.abs(kk) @ np.abs(rows[b, t, h])).max() * dim ** -0.5
+                    first, *rest = np.sort(s)[::-1][:2]
+                    if not rest or first - rest[0] > 2 * slip + 40:
+                        best = vv[int(np.argmax(s))]
+                        assert (np.abs(out[b, t, h] - best) <= (2.0 ** -11 + 1.01 * 2.0 ** -8) * np.abs(best) + 1e-7).all()
+                        checked += 1
+    assert checked > 50
+
+
 @pytest.mark.parametrize("scale", [1e-30, -1e-30, 1e-38])
 @pytest.mark.parametrize("tokens", [2, 80])
 def test_tiny_scale(gpu, tokens, scale):
