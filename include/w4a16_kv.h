@@ -1,6 +1,7 @@
 /*
  * w4a16_kv.h -- C ABI of the 8-bit key/value cache: rotary positions, writing
- * keys and values into the cache, reading it back, and attention over it.
+ * keys and values into the cache, reading it back, attention over it (also
+ * behind shared prefixes), and copying its sequences.
  * The conventions of w4a16_hip.h hold (device pointers, return codes,
  * w4a16_last_error(), work enqueued on `stream`, nothing allocated or
  * synchronised, so every call may be captured in a HIP graph).
@@ -135,6 +136,48 @@ int64_t w4a16_kv_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_
 int w4a16_kv_attention(const w4a16_kv_rows* q, void* out, int64_t tokens, int64_t heads, const w4a16_kv_cache* cache,
                        const int64_t* start, const int64_t* counts, float scale, int type, void* workspace,
                        int64_t workspace_bytes, void* stream);
+
+/*
+ * The same where the sequences share prefixes, which another cache holds: of
+ * `prefix` with G sequences and `cache` with B, a multiple of G, sequence b
+ * stands behind prefix g = b / (B / G). Token t of sequence b sees the prefix's
+ * slots 0 .. prefix_lengths[g] - 1 and its own slots 0 .. start[b] + t (its
+ * position in the sequence is prefix_lengths[g] + start[b] + t, which is the row
+ * of the rotary tables to rotate it by). Both caches have the same kv_heads,
+ * head_dim and code_type; slots and blocks may differ. prefix_lengths is device
+ * int64 [G], from 0 (an empty prefix) to the prefix's slots; rows behind a
+ * length outside of that come out NaN, as those at positions outside `cache` do.
+ * The rows of all sequences behind a prefix attend it together, so its keys and
+ * values are read once for them; a row's value is that of attention over one
+ * cache with both, up to the rounding. Everything else as w4a16_kv_attention.
+ */
+int64_t w4a16_kv_shared_attention_workspace_bytes(int64_t groups, int64_t prefix_slots, int64_t batch, int64_t tokens,
+                                                  int64_t heads, int64_t kv_heads, int64_t slots, int64_t head_dim);
+int w4a16_kv_shared_attention(const w4a16_kv_rows* q, void* out, int64_t tokens, int64_t heads,
+                              const w4a16_kv_cache* prefix, const int64_t* prefix_lengths, const w4a16_kv_cache* cache,
+                              const int64_t* start, const int64_t* counts, float scale, int type, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/*
+ * Copies sequences of one cache into another: sequence b of `to` becomes what
+ * sequence source[b] of `from` holds, its first lengths[source[b]] slots (at most
+ * as many as both caches have) with the scales of their blocks. source is device
+ * int64 [to->batch]; a sequence whose source lies outside `from` stays as it is.
+ * lengths is device int64 [from->batch], below 0 as 0. Codes behind the copied
+ * slots stay as they are (their values change with a shared block's scale: they
+ * are free). The caches have the same kv_heads, head_dim, block and code_type and
+ * share no memory; the rows of `to` share none with each other.
+ */
+int w4a16_kv_fork(const w4a16_kv_cache* from, const w4a16_kv_cache* to, const int64_t* source, const int64_t* lengths,
+                  void* stream);
+
+/*
+ * The same within one cache: every sequence b becomes what sequence source[b]
+ * held before the call (beams that live on, finished sequences whose place
+ * another takes). lengths [batch] are those before the call. At most 262144 /
+ * head_dim sequences.
+ */
+int w4a16_kv_reorder(const w4a16_kv_cache* cache, const int64_t* source, const int64_t* lengths, void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,17 +11,22 @@ from nibble_amd.cuda import (
     cuda_extension_available,
     dequantize_cuda,
     kv_attention_cuda,
+    kv_fork_cuda,
     kv_read_cuda,
+    kv_reorder_cuda,
+    kv_shared_attention_cuda,
     kv_write_cuda,
     linear_cuda,
     rotary_cuda,
     rotary_kv_write_cuda,
+    sample_cuda,
 )
 from nibble_amd.integration import load_packed_state_dict, replace_linear_layers
 from nibble_amd.kv_cache import QuantizedKVCache
 from nibble_amd.linear import Int4Linear, QuantizedLinear
 from nibble_amd.quantization import pack_int4, quantize_and_pack_weights, quantize_groupwise, unpack_int4
 from nibble_amd.rope import rope_frequencies, rope_tables, rotary
+from nibble_amd.sampling import sample
 
 __all__ = [
     "QuantizedLinear",
@@ -46,4 +51,9 @@ __all__ = [
     "rotary_kv_write_cuda",
     "kv_read_cuda",
     "kv_attention_cuda",
+    "kv_shared_attention_cuda",
+    "kv_fork_cuda",
+    "kv_reorder_cuda",
+    "sample",
+    "sample_cuda",
 ]

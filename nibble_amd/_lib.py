@@ -152,6 +152,25 @@ KV_SIGNATURES = {
     "w4a16_kv_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "w4a16_kv_attention": (ctypes.c_int, [_rows_p, _vp, _i64, _i64, _cache_p, _vp, _vp, ctypes.c_float, ctypes.c_int,
                                           _vp, _i64, _vp]),
+    "w4a16_kv_shared_attention_workspace_bytes": (_i64, [_i64] * 8),
+    "w4a16_kv_shared_attention": (ctypes.c_int, [_rows_p, _vp, _i64, _i64, _cache_p, _vp, _cache_p, _vp, _vp,
+                                                 ctypes.c_float, ctypes.c_int, _vp, _i64, _vp]),
+    "w4a16_kv_fork": (ctypes.c_int, [_cache_p, _cache_p, _vp, _vp, _vp]),
+    "w4a16_kv_reorder": (ctypes.c_int, [_cache_p, _vp, _vp, _vp]),
+}
+
+
+# include/w4a16_sample.h
+class SampleSettings(ctypes.Structure):
+    """w4a16_sample_settings"""
+
+    _fields_ = [("temperature", ctypes.c_double), ("top_k", _i64), ("top_p", ctypes.c_double),
+                ("min_p", ctypes.c_double), ("temperatures", _vp), ("top_ks", _vp), ("top_ps", _vp), ("min_ps", _vp)]
+
+
+SAMPLE_SIGNATURES = {
+    "w4a16_sample": (ctypes.c_int, [_vp, _i64, _i64, _i64, ctypes.c_int, _vp, ctypes.POINTER(SampleSettings), _vp,
+                                    _vp]),
 }
 
 _lib = None
@@ -172,7 +191,8 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`"
             )
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (restype, argtypes) in {**SIGNATURES, **DECODE_SIGNATURES, **KV_SIGNATURES}.items():
+        for name, (restype, argtypes) in {**SIGNATURES, **DECODE_SIGNATURES, **KV_SIGNATURES,
+                                          **SAMPLE_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.restype = restype
             fn.argtypes = argtypes

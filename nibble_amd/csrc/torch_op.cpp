@@ -5,7 +5,8 @@
 // PyTorch-ROCm), and exposes an empty Python module so that importing the
 // extension registers the ops (reference csrc/int4_linear.cpp:30). The ops of
 // the 8-bit key/value cache (w4a16::rotary, kv_write, rotary_kv_write,
-// kv_read, kv_attention) map tensors onto w4a16_kv.h in the same way.
+// kv_read, kv_attention, kv_shared_attention, kv_fork, kv_reorder) map tensors
+// onto w4a16_kv.h and w4a16::sample onto w4a16_sample.h in the same way.
 //
 // Tensor-level checks use the reference's messages (reference
 // csrc/int4_linear_kernel.cu:646-691, :809-841); shape relations and launches
@@ -20,9 +21,11 @@
 #include <torch/library.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "w4a16_hip.h"
 #include "w4a16_kv.h"
+#include "w4a16_sample.h"
 
 namespace {
 
@@ -329,6 +332,110 @@ at::Tensor kv_attention(const at::Tensor& q, const at::Tensor& k_codes, const at
     return out;
 }
 
+at::Tensor kv_shared_attention(const at::Tensor& q, const at::Tensor& prefix_k_codes, const at::Tensor& prefix_k_scales,
+                               const at::Tensor& prefix_v_codes, const at::Tensor& prefix_v_scales,
+                               const at::Tensor& prefix_lengths, const at::Tensor& k_codes, const at::Tensor& k_scales,
+                               const at::Tensor& v_codes, const at::Tensor& v_scales, const at::Tensor& start,
+                               const c10::optional<at::Tensor>& counts, c10::optional<double> scale) {
+    const Cache prefix = cache_of(prefix_k_codes, prefix_k_scales, prefix_v_codes, prefix_v_scales);
+    const Cache cache = cache_of(k_codes, k_scales, v_codes, v_scales);
+    TORCH_CHECK(prefix.device == cache.device, "the prefix must be on the cache's CUDA device");
+    TORCH_CHECK(q.dim() == 4, "q must have shape [batch, tokens, heads, head_dim]");
+    const int64_t tokens = q.size(1), heads = q.size(2);
+    const w4a16_kv_rows qr = token_rows(q, cache, tokens, -1, "q");
+    const int type = row_type(q, "q");
+    const int64_t* lengths = lengths_of(prefix_lengths, prefix.abi.batch, cache.device, "prefix_lengths");
+    const int64_t* first = lengths_of(start, cache.abi.batch, cache.device, "start");
+    const c10::DeviceGuard guard(cache.device);
+    at::Tensor out = at::empty(q.sizes(), q.options(), at::MemoryFormat::Contiguous);
+    // the shares of both sides, from the caching allocator (graph-capture safe)
+    const int64_t ws_bytes = w4a16_kv_shared_attention_workspace_bytes(
+        prefix.abi.batch, prefix.abi.slots, cache.abi.batch, tokens, heads, cache.abi.kv_heads, cache.abi.slots,
+        cache.abi.head_dim);
+    at::Tensor workspace;
+    if (ws_bytes > 0) workspace = at::empty({(ws_bytes + 3) / 4}, q.options().dtype(at::kFloat));
+    const int rc = w4a16_kv_shared_attention(
+        &qr, out.data_ptr(), tokens, heads, &prefix.abi, lengths, &cache.abi, first,
+        counts_of(counts, cache.abi.batch, cache.device),
+        (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)cache.abi.head_dim)), type,
+        ws_bytes > 0 ? workspace.data_ptr() : nullptr, ws_bytes, current_stream(cache.device));
+    TORCH_CHECK(rc == W4A16_OK, w4a16_last_error());
+    return out;
+}
+
+void kv_fork(const at::Tensor& k_codes, const at::Tensor& k_scales, const at::Tensor& v_codes,
+             const at::Tensor& v_scales, at::Tensor to_k_codes, at::Tensor to_k_scales, at::Tensor to_v_codes,
+             at::Tensor to_v_scales, const at::Tensor& source, const at::Tensor& lengths) {
+    Cache from = cache_of(k_codes, k_scales, v_codes, v_scales);
+    Cache to = cache_of(to_k_codes, to_k_scales, to_v_codes, to_v_scales);
+    TORCH_CHECK(from.device == to.device, "both caches must be on the same CUDA device");
+    // slots that one scale covers may be of any block that holds them: the other cache tells which
+    if (k_scales.size(2) == 1 && from.abi.slots <= to.abi.block) from.abi.block = to.abi.block;
+    if (to_k_scales.size(2) == 1 && to.abi.slots <= from.abi.block) to.abi.block = from.abi.block;
+    const int64_t* rows = lengths_of(source, to.abi.batch, to.device, "source");
+    const int64_t* held = lengths_of(lengths, from.abi.batch, to.device, "lengths");
+    const c10::DeviceGuard guard(to.device);
+    const int rc = w4a16_kv_fork(&from.abi, &to.abi, rows, held, current_stream(to.device));
+    TORCH_CHECK(rc == W4A16_OK, w4a16_last_error());
+}
+
+void kv_reorder(at::Tensor k_codes, at::Tensor k_scales, at::Tensor v_codes, at::Tensor v_scales,
+                const at::Tensor& source, const at::Tensor& lengths) {
+    const Cache cache = cache_of(k_codes, k_scales, v_codes, v_scales);
+    const int64_t* rows = lengths_of(source, cache.abi.batch, cache.device, "source");
+    const int64_t* held = lengths_of(lengths, cache.abi.batch, cache.device, "lengths");
+    const c10::DeviceGuard guard(cache.device);
+    const int rc = w4a16_kv_reorder(&cache.abi, rows, held, current_stream(cache.device));
+    TORCH_CHECK(rc == W4A16_OK, w4a16_last_error());
+}
+
+// ------------------------------------------------------------ sampling
+
+// One value a row, or none.
+template <typename T>
+const T* row_values(const c10::optional<at::Tensor>& x, int64_t rows, const at::Device& device, const char* name) {
+    if (!x.has_value() || !x->defined()) return nullptr;
+    constexpr bool whole = std::is_same<T, int64_t>::value;
+    TORCH_CHECK(x->is_cuda() && x->device() == device, name, " must be on the same CUDA device as the logits");
+    TORCH_CHECK(!x->requires_grad(), name, " must not require grad");
+    TORCH_CHECK(x->scalar_type() == (whole ? at::kLong : at::kFloat), name, " must have dtype ",
+                whole ? "torch.int64" : "torch.float32");
+    TORCH_CHECK(x->dim() == 1 && x->size(0) == rows && x->is_contiguous(), name,
+                " must be contiguous with shape [rows]");
+    return x->template data_ptr<T>();
+}
+
+at::Tensor sample(const at::Tensor& logits, const at::Tensor& random, double temperature, int64_t top_k, double top_p,
+                  double min_p, const c10::optional<at::Tensor>& temperatures,
+                  const c10::optional<at::Tensor>& top_ks, const c10::optional<at::Tensor>& top_ps,
+                  const c10::optional<at::Tensor>& min_ps) {
+    TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+    TORCH_CHECK(logits.scalar_type() == at::kHalf || logits.scalar_type() == at::kBFloat16 ||
+                    logits.scalar_type() == at::kFloat,
+                "logits must have dtype torch.float16, torch.bfloat16 or torch.float32");
+    TORCH_CHECK(!logits.requires_grad(), "logits must not require grad");
+    TORCH_CHECK(logits.dim() == 2, "logits must have shape [rows, vocabulary]");
+    TORCH_CHECK(logits.size(1) <= 1 || logits.stride(1) == 1, "logits must be contiguous in their last dimension");
+    const int64_t rows = logits.size(0);
+    const at::Device device = logits.device();
+    const float* numbers = row_values<float>(random, rows, device, "random");
+    TORCH_CHECK(numbers != nullptr || rows == 0, "random must have a value for every row");
+    const w4a16_sample_settings settings{temperature, top_k, top_p, min_p,
+                                         row_values<float>(temperatures, rows, device, "temperature"),
+                                         row_values<int64_t>(top_ks, rows, device, "top_k"),
+                                         row_values<float>(top_ps, rows, device, "top_p"),
+                                         row_values<float>(min_ps, rows, device, "min_p")};
+    const c10::DeviceGuard guard(device);
+    at::Tensor tokens = at::empty({rows}, logits.options().dtype(at::kLong));
+    const int type = logits.scalar_type() == at::kHalf       ? W4A16_FP16
+                     : logits.scalar_type() == at::kBFloat16 ? W4A16_BF16
+                                                             : W4A16_FP32;
+    const int rc = w4a16_sample(logits.data_ptr(), rows, logits.size(1), stride_of(logits, 0), type, numbers, &settings,
+                                tokens.data_ptr<int64_t>(), current_stream(device));
+    TORCH_CHECK(rc == W4A16_OK, w4a16_last_error());
+    return tokens;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(w4a16, m) {
@@ -344,6 +451,16 @@ TORCH_LIBRARY(w4a16, m) {
     m.def("kv_read(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor");
     m.def("kv_attention(Tensor q, Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor start, "
           "Tensor? counts=None, float? scale=None) -> Tensor");
+    m.def("kv_shared_attention(Tensor q, Tensor prefix_k_codes, Tensor prefix_k_scales, Tensor prefix_v_codes, "
+          "Tensor prefix_v_scales, Tensor prefix_lengths, Tensor k_codes, Tensor k_scales, Tensor v_codes, "
+          "Tensor v_scales, Tensor start, Tensor? counts=None, float? scale=None) -> Tensor");
+    m.def("kv_fork(Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor(a!) to_k_codes, "
+          "Tensor(b!) to_k_scales, Tensor(c!) to_v_codes, Tensor(d!) to_v_scales, Tensor source, Tensor lengths) -> ()");
+    m.def("kv_reorder(Tensor(a!) k_codes, Tensor(b!) k_scales, Tensor(c!) v_codes, Tensor(d!) v_scales, "
+          "Tensor source, Tensor lengths) -> ()");
+    m.def("sample(Tensor logits, Tensor random, float temperature=1.0, int top_k=0, float top_p=1.0, "
+          "float min_p=0.0, Tensor? temperatures=None, Tensor? top_ks=None, Tensor? top_ps=None, "
+          "Tensor? min_ps=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(w4a16, CUDA, m) {
@@ -355,6 +472,10 @@ TORCH_LIBRARY_IMPL(w4a16, CUDA, m) {
     m.impl("rotary_kv_write", &rotary_kv_write);
     m.impl("kv_read", &kv_read);
     m.impl("kv_attention", &kv_attention);
+    m.impl("kv_shared_attention", &kv_shared_attention);
+    m.impl("kv_fork", &kv_fork);
+    m.impl("kv_reorder", &kv_reorder);
+    m.impl("sample", &sample);
 }
 
 static PyModuleDef w4a16_module = {PyModuleDef_HEAD_INIT, "_C", "W4A16 torch ops (registered on import)", -1,

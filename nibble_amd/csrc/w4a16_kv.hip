@@ -513,15 +513,24 @@ bool meet(const Region& a, const Region& b) {
     return false;
 }
 
-// Workgroups write their own block each: blocks that share memory would race.
-int check_written(const w4a16_kv_cache& c) {
+// The memory of a cache's codes and scales: keys' and values' codes, then their scales.
+void regions_of(const w4a16_kv_cache& c, Region (&r)[4]) {
     const int64_t blocks = (c.slots + c.block - 1) / c.block;
-    Region r[4];
     for (int i = 0; i < 2; ++i) {
         const w4a16_kv_codes& side = i ? c.v : c.k;
         r[i] = region_of(side.codes, c.slots * c.head_dim, c.batch, side.batch_stride, c.kv_heads, side.head_stride, 1);
         r[2 + i] = region_of(side.scales, blocks, c.batch, side.scale_batch_stride, c.kv_heads, side.scale_head_stride, 4);
     }
+}
+
+}  // namespace
+
+namespace w4a16_internal {
+
+// Workgroups write their own block each: blocks that share memory would race.
+int check_written(const w4a16_kv_cache& c) {
+    Region r[4];
+    regions_of(c, r);
     for (int i = 0; i < 4; ++i)
         if (!disjoint(r[i]))
             return kv_fail(W4A16_ERR_CONFIG, "codes and scales that are written must not overlap themselves");
@@ -531,6 +540,22 @@ int check_written(const w4a16_kv_cache& c) {
                 return kv_fail(W4A16_ERR_CONFIG, "keys and values, codes and scales must not share memory");
     return W4A16_OK;
 }
+
+int check_apart(const w4a16_kv_cache& read, const w4a16_kv_cache& written) {
+    Region r[4], w[4];
+    regions_of(read, r);
+    regions_of(written, w);
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j)
+            if (meet(r[i], w[j])) return kv_fail(W4A16_ERR_CONFIG, "the two caches must not share memory");
+    return W4A16_OK;
+}
+
+}  // namespace w4a16_internal
+
+namespace {
+
+using w4a16_internal::check_written;
 
 // Keys and values into the cache, and (q != NULL) the rotation of q and k.
 int write_tokens(const w4a16_kv_rows* q, void* q_out, int64_t heads, const w4a16_kv_rows* k, const w4a16_kv_rows* v,

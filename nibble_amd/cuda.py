@@ -1,6 +1,7 @@
 """Python wrappers of the torch ops ``w4a16::linear``, ``w4a16::dequantize``,
-``w4a16::quantize`` and of the ops of the 8-bit key/value cache (``rotary``,
-``kv_write``, ``rotary_kv_write``, ``kv_read``, ``kv_attention``).
+``w4a16::quantize``, of the ops of the 8-bit key/value cache (``rotary``,
+``kv_write``, ``rotary_kv_write``, ``kv_read``, ``kv_attention``,
+``kv_shared_attention``, ``kv_fork``, ``kv_reorder``) and of ``sample``.
 
 Mirrors reference ``w4a16/cuda.py``: importing the compiled extension
 (``nibble_amd._C``, here a thin libtorch shim over the HIP C ABI) registers
@@ -65,6 +66,26 @@ if _EXTENSION_LOAD_ERROR is None:
     @torch.library.register_fake("w4a16::kv_attention")
     def _kv_attention_fake(q, k_codes, k_scales, v_codes, v_scales, start, counts=None, scale=None):
         return q.new_empty(q.shape)
+
+
+    @torch.library.register_fake("w4a16::kv_shared_attention")
+    def _kv_shared_attention_fake(q, prefix_k_codes, prefix_k_scales, prefix_v_codes, prefix_v_scales, prefix_lengths,
+                                  k_codes, k_scales, v_codes, v_scales, start, counts=None, scale=None):
+        return q.new_empty(q.shape)
+
+    @torch.library.register_fake("w4a16::kv_fork")
+    def _kv_fork_fake(k_codes, k_scales, v_codes, v_scales, to_k_codes, to_k_scales, to_v_codes, to_v_scales, source,
+                      lengths):
+        return None
+
+    @torch.library.register_fake("w4a16::kv_reorder")
+    def _kv_reorder_fake(k_codes, k_scales, v_codes, v_scales, source, lengths):
+        return None
+
+    @torch.library.register_fake("w4a16::sample")
+    def _sample_fake(logits, random, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, temperatures=None, top_ks=None,
+                     top_ps=None, min_ps=None):
+        return logits.new_empty((logits.shape[0],), dtype=torch.int64)
 
 
 def cuda_extension_available() -> bool:
@@ -225,3 +246,93 @@ def kv_attention_cuda(
     padding and come out zero. ``scale`` defaults to head_dim ** -0.5."""
     _require_extension()
     return torch.ops.w4a16.kv_attention.default(q, k_codes, k_scales, v_codes, v_scales, start, counts, scale)
+
+
+def kv_shared_attention_cuda(
+    q: torch.Tensor,
+    prefix_k_codes: torch.Tensor,
+    prefix_k_scales: torch.Tensor,
+    prefix_v_codes: torch.Tensor,
+    prefix_v_scales: torch.Tensor,
+    prefix_lengths: torch.Tensor,
+    k_codes: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_codes: torch.Tensor,
+    v_scales: torch.Tensor,
+    start: torch.Tensor,
+    counts: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """``kv_attention_cuda`` of a batch whose sequences share prefixes: a cache
+    of G prefixes and one of the B sequences' own slots, B a multiple of G;
+    token t of sequence b sees the slots 0 .. prefix_lengths[g] - 1 of prefix g
+    = b // (B // G) and its own slots 0 .. start[b] + t. A prefix is read once
+    for all of its sequences."""
+    _require_extension()
+    return torch.ops.w4a16.kv_shared_attention.default(
+        q, prefix_k_codes, prefix_k_scales, prefix_v_codes, prefix_v_scales, prefix_lengths, k_codes, k_scales,
+        v_codes, v_scales, start, counts, scale)
+
+
+def kv_fork_cuda(
+    k_codes: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_codes: torch.Tensor,
+    v_scales: torch.Tensor,
+    to_k_codes: torch.Tensor,
+    to_k_scales: torch.Tensor,
+    to_v_codes: torch.Tensor,
+    to_v_scales: torch.Tensor,
+    source: torch.Tensor,
+    lengths: torch.Tensor,
+) -> None:
+    """Copies sequences of one 8-bit cache into another: sequence b of the
+    second becomes what sequence source[b] of the first holds, lengths[source[b]]
+    slots of it (int64 tensors); it stays as it is where source[b] is outside
+    the first. The caches have the same KV heads, head_dim, block and codes and
+    share no memory."""
+    _require_extension()
+    torch.ops.w4a16.kv_fork.default(k_codes, k_scales, v_codes, v_scales, to_k_codes, to_k_scales, to_v_codes,
+                                    to_v_scales, source, lengths)
+
+
+def kv_reorder_cuda(
+    k_codes: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_codes: torch.Tensor,
+    v_scales: torch.Tensor,
+    source: torch.Tensor,
+    lengths: torch.Tensor,
+) -> None:
+    """The sequences of an 8-bit cache in another order, in place: every
+    sequence b becomes what sequence source[b] held before, its first
+    lengths[source[b]] slots (int64 [batch]); one whose source is outside the
+    batch stays as it is."""
+    _require_extension()
+    torch.ops.w4a16.kv_reorder.default(k_codes, k_scales, v_codes, v_scales, source, lengths)
+
+
+def sample_cuda(
+    logits: torch.Tensor,
+    random: torch.Tensor,
+    temperature: float | torch.Tensor = 1.0,
+    top_k: int | torch.Tensor = 0,
+    top_p: float | torch.Tensor = 1.0,
+    min_p: float | torch.Tensor = 0.0,
+) -> torch.Tensor:
+    """A token (int64 [rows]) from each row of logits fp16, bf16 or fp32 [rows,
+    vocabulary], drawn by the uniform numbers ``random`` (float32 [rows], in
+    [0, 1)): temperature first (0: the largest logit), then the ``top_k`` most
+    likely tokens (0: all), of those the most likely ones that hold ``top_p`` of
+    the probability together (1: all), and of those the ones at least ``min_p``
+    times as likely as the first. The token is the first by index at which the
+    running sum of the kept probabilities exceeds ``random`` times their sum.
+    Each setting is a number for all rows or a tensor with one a row (float32,
+    ``top_k`` int64). At most 524288 logits a row."""
+    _require_extension()
+    single, rows = [], []
+    for value, unset in ((temperature, 1.0), (top_k, 0), (top_p, 1.0), (min_p, 0.0)):
+        tensor = isinstance(value, torch.Tensor)
+        single.append(unset if tensor else value)
+        rows.append(value if tensor else None)
+    return torch.ops.w4a16.sample.default(logits, random, *single, *rows)

@@ -20,7 +20,15 @@ from __future__ import annotations
 import torch
 
 from nibble_amd import kv_reference
-from nibble_amd.cuda import kv_attention_cuda, kv_read_cuda, kv_write_cuda, rotary_kv_write_cuda
+from nibble_amd.cuda import (
+    kv_attention_cuda,
+    kv_fork_cuda,
+    kv_read_cuda,
+    kv_reorder_cuda,
+    kv_shared_attention_cuda,
+    kv_write_cuda,
+    rotary_kv_write_cuda,
+)
 
 CODE_TYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 
@@ -93,6 +101,37 @@ class QuantizedKVCache:
         start[b] + t over the cache, which holds the tokens already."""
         call = kv_attention_cuda if self.k_codes.is_cuda else kv_reference.kv_attention_reference
         return call(q, *self.tensors(), start, counts, scale)
+
+    def attend_shared(
+        self,
+        q: torch.Tensor,
+        prefix: QuantizedKVCache,
+        prefix_lengths: torch.Tensor,
+        start: torch.Tensor,
+        counts: torch.Tensor | None = None,
+        scale: float | None = None,
+    ) -> torch.Tensor:
+        """``attend`` where this cache holds what its sequences have for
+        themselves and ``prefix``, of which each sequence stands behind the same
+        number of this one's, what comes before: token t of sequence b sees the
+        first prefix_lengths[g] slots of prefix g and its own slots 0 ..
+        start[b] + t. Its position, for the rotary tables, is prefix_lengths[g] +
+        start[b] + t: with one prefix length, the tables from its row on."""
+        call = kv_shared_attention_cuda if self.k_codes.is_cuda else kv_reference.kv_shared_attention_reference
+        return call(q, *prefix.tensors(), prefix_lengths, *self.tensors(), start, counts, scale)
+
+    def fork_from(self, other: QuantizedKVCache, source: torch.Tensor, lengths: torch.Tensor) -> None:
+        """Every sequence b becomes what sequence source[b] of another cache
+        holds, lengths[source[b]] slots of it (int64 tensors of this and of the
+        other cache's batch); a source outside the other leaves b as it is."""
+        call = kv_fork_cuda if self.k_codes.is_cuda else kv_reference.kv_fork_reference
+        call(*other.tensors(), *self.tensors(), source, lengths)
+
+    def reorder(self, source: torch.Tensor, lengths: torch.Tensor) -> None:
+        """Every sequence b becomes what sequence source[b] held before, its
+        first lengths[source[b]] slots (int64 [batch] both)."""
+        call = kv_reorder_cuda if self.k_codes.is_cuda else kv_reference.kv_reorder_reference
+        call(*self.tensors(), source, lengths)
 
     def read(self, slots: int | None = None, dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values [batch, kv_heads, slots, head_dim] of the first

@@ -177,3 +177,81 @@ def kv_attention_reference(q, k_codes, k_scales, v_codes, v_scales, start, count
         row[~inside] = float("nan")
         out[b, :count] = row.to(q.dtype)
     return out
+
+
+def kv_shared_attention_reference(q, prefix_k_codes, prefix_k_scales, prefix_v_codes, prefix_v_scales, prefix_lengths,
+                                  k_codes, k_scales, v_codes, v_scales, start, counts=None, scale=None):
+    """Sequence by sequence over the prefix's values and the own ones in one tensor."""
+    groups, kv_heads, held = prefix_k_codes.shape[:3]
+    _check_rows(q, "q", k_codes, q.shape[1])
+    batch, tokens, heads, dim = q.shape
+    if (kv_heads, prefix_k_codes.shape[3], prefix_k_codes.dtype) != (k_codes.shape[1], dim, k_codes.dtype):
+        raise ValueError("the prefix and the cache must have the same KV heads, head_dim and codes")
+    if groups == 0 or batch % groups != 0:
+        raise ValueError("the cache's sequences must be a multiple of the prefixes")
+    if heads == 0 or heads % kv_heads != 0:
+        raise ValueError("heads must be a positive multiple of the cache's KV heads")
+    scale = dim ** -0.5 if scale is None else scale
+    if not math.isfinite(scale):
+        raise ValueError("scale must be a finite number")
+    _check_lengths(prefix_lengths, groups, "prefix_lengths")
+    slots, group = k_codes.shape[2], heads // kv_heads
+    out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+    for b, (first, count) in enumerate(_spans(start, counts, batch, tokens)):
+        g = b // (batch // groups)
+        before = int(prefix_lengths[g])
+        known = 0 <= before <= held
+        before = before if known else 0
+        end = min(max(first + count, 0), slots)
+        k, v = (torch.cat((kv_read_reference(pc[g:g + 1], ps[g:g + 1], torch.float32)[0, :, :before],
+                           kv_read_reference(c[b:b + 1], s[b:b + 1], torch.float32)[0, :, :end]), dim=1)
+                .repeat_interleave(group, dim=0)
+                for pc, ps, c, s in ((prefix_k_codes, prefix_k_scales, k_codes, k_scales),
+                                     (prefix_v_codes, prefix_v_scales, v_codes, v_scales)))
+        position = first + torch.arange(count)
+        scores = torch.matmul(q[b, :count].float().transpose(0, 1), k.transpose(1, 2)) * scale
+        scores = scores.masked_fill(torch.arange(-before, end) > position.clamp(min=-1).unsqueeze(1), float("-inf"))
+        row = torch.matmul(torch.softmax(scores, dim=-1), v).transpose(0, 1)
+        row[~((position >= 0) & (position < slots) & known)] = float("nan")
+        out[b, :count] = row.to(q.dtype)
+    return out
+
+
+def _check_moved(tensors, to_tensors, source, lengths) -> int:
+    """The slots of a block of both caches; (k_codes, k_scales, v_codes, v_scales) each."""
+    blocks = []
+    for k, ks, v, vs in (tensors, to_tensors):
+        if k.shape != v.shape or ks.shape != vs.shape or k.dtype != v.dtype:
+            raise ValueError("key and value codes and scales must have the same shapes and dtype")
+        blocks.append((block_size(k.shape[2], ks.shape[2]), ks.shape[2] == 1, k.shape[2]))
+    (block, one, slots), (to_block, to_one, to_slots) = blocks
+    if one and slots <= to_block:      # slots that one scale covers may be of any block that holds them
+        block = to_block
+    if to_one and to_slots <= block:
+        to_block = block
+    codes, to_codes = tensors[0], to_tensors[0]
+    if (codes.shape[1], codes.shape[3], codes.dtype, block) != (to_codes.shape[1], to_codes.shape[3], to_codes.dtype,
+                                                                to_block):
+        raise ValueError("the two caches must have the same KV heads, head_dim, block and codes")
+    _check_lengths(source, to_codes.shape[0], "source")
+    _check_lengths(lengths, codes.shape[0], "lengths")
+    return block
+
+
+def kv_fork_reference(k_codes, k_scales, v_codes, v_scales, to_k_codes, to_k_scales, to_v_codes, to_v_scales, source,
+                      lengths):
+    tensors = (k_codes, k_scales, v_codes, v_scales)
+    to_tensors = (to_k_codes, to_k_scales, to_v_codes, to_v_scales)
+    block = _check_moved(tensors, to_tensors, source, lengths)
+    most = min(k_codes.shape[2], to_k_codes.shape[2])
+    for b, j in enumerate(source.tolist()):
+        if not 0 <= j < k_codes.shape[0]:
+            continue
+        slots = min(max(int(lengths[j]), 0), most)
+        for x, to, n in zip(tensors, to_tensors, (slots, -(-slots // block)) * 2):
+            to[b, :, :n] = x[j, :, :n]
+
+
+def kv_reorder_reference(k_codes, k_scales, v_codes, v_scales, source, lengths):
+    tensors = (k_codes, k_scales, v_codes, v_scales)
+    kv_fork_reference(*(x.clone() for x in tensors), *tensors, source, lengths)

@@ -12,7 +12,7 @@ import nibble_amd as _impl
 from nibble_amd import *  # noqa: F401,F403
 from nibble_amd import __all__  # noqa: F401
 
-for _name in ("quantization", "reference", "cuda", "linear", "integration", "checkpoint", "kv_cache", "rope"):
+for _name in ("quantization", "reference", "cuda", "linear", "integration", "checkpoint", "kv_cache", "rope", "sampling"):
     _module = _importlib.import_module(f"nibble_amd.{_name}")
     _sys.modules[f"{__name__}.{_name}"] = _module
     globals()[_name] = _module
