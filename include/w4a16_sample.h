@@ -44,9 +44,9 @@ typedef struct w4a16_sample_settings {
  *   the token is the first, by index, at which the running sum of the kept
  *   weights exceeds random[r] times their sum.
  * A number below 0 or NaN reads as 0, one of 1 or more gives the last token of a
- * weight. Weights are rounded to whole multiples of 2^-44 of the largest one
- * (smaller ones count as 0), their sums are exact: the same call gives the same
- * tokens. A row with NaN gives the first NaN's index and a row of -inf token 0,
+ * weight. Weights are held to 2^-38 of themselves and rounded to whole multiples
+ * of 2^-44 of the largest one (smaller ones count as 0), their sums are exact: the
+ * same call gives the same tokens. A row with NaN gives the first NaN's index and a row of -inf token 0,
  * as argmax does; where logits are +inf, those alone have weight.
  * tokens share no memory with the other arguments.
  */

@@ -7,9 +7,10 @@ import torch
 
 
 def tokens(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> set[int]:
-    """The tokens that a row may give. A weight is held to 2^-45 of the largest
-    and has a relative error below 2^-44 besides; so sums of n weights are off by
-    less than n 2^-43, and a border that lies so near may fall on either side."""
+    """The tokens that a row may give. A weight is held to 2^-45 of the largest one
+    and to 2^-38 of itself; so sums of n weights are off by less than 2^-38 of
+    themselves and n 2^-45, each of two that are compared, and a border that lies
+    so near may fall on either side."""
     x = np.asarray(x, dtype=np.float64)
     if np.isnan(x).any():
         return {int(np.argmax(np.isnan(x)))}
@@ -19,7 +20,7 @@ def tokens(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> set[int]:
     with np.errstate(invalid="ignore"):
         w = np.exp((x - top) / temperature)
     w[x == top], w[x == -np.inf] = 1.0, 0.0
-    slack = len(x) * 2.0 ** -43
+    slack = len(x) * 2.0 ** -44 + w.sum() * 2.0 ** -37
     order = np.lexsort((np.arange(len(x)), -x))
     if top_k > 0:
         order = order[:top_k]
@@ -32,7 +33,7 @@ def tokens(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> set[int]:
             keep[0] = True
             kept = kept[keep]
         for side_m in (-1, 1):
-            least = min(min_p if min_p > 0.0 else 0.0, 1.0) * (1 + side_m * 2.0 ** -40)   # NaN: none
+            least = min(min_p if min_p > 0.0 else 0.0, 1.0) * (1 + side_m * 2.0 ** -37)   # NaN: none
             chosen = kept[(w[kept] >= least) | (w[kept] == 1.0)]
             mask = np.zeros(len(x), dtype=bool)
             mask[chosen] = True

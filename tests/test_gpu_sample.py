@@ -173,3 +173,21 @@ def test_compiled(gpu):
     logits, random = _sample.logits(2, 999, torch.float16, 71).cuda(), _sample.numbers(2, 72).cuda()
     got = torch.compile(draw, backend="aot_eager", fullgraph=True)(logits, random)
     assert torch.equal(got, draw(logits, random))
+
+
+@pytest.mark.parametrize("settings", [{}, {"top_k": 400}, {"top_p": 0.9}, {"top_p": 0.5, "top_k": 3000}, {"min_p": 0.3},
+                                      {"temperature": 1e-6, "top_p": 0.9}, {"temperature": 30.0, "top_p": 0.99}])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_values_near_zero(gpu, dtype, settings):
+    """Logits around 0 and below 2^-20: few and many, zeros, of both signs, as the largest and among larger ones."""
+    g = torch.Generator().manual_seed(3)
+    n = 9000
+    rows = []
+    for share, spread, shift in [(0.001, 1.0, 0.0), (0.001, 1e-3, 0.0), (0.5, 1.0, 0.0), (1.0, 1.0, 0.0), (0.004, 2.0, -5.0),
+                                 (0.02, 0.5, -1.5)]:
+        row = spread * torch.randn(n, generator=g) + shift
+        tiny = torch.rand(n, generator=g) < share
+        rows.append(torch.where(tiny, torch.randn(n, generator=g) * 2.0 ** -22, row))
+        rows[-1][torch.rand(n, generator=g) < 0.01] = 0.0
+        rows[-1][torch.rand(n, generator=g) < 0.01] = -0.0
+    _check(torch.stack(rows).to(dtype), _sample.numbers(len(rows), 4), **settings)
