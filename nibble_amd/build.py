@@ -53,7 +53,8 @@ def _run(cmd: list[str], verbose: bool) -> None:
 HIP_SOURCES = ["w4a16_hip.hip", "w4a16_decode.hip", "w4a16_pair.hip", "w4a16_stream.hip", "w4a16_gemm.hip",
                "w4a16_pair_ring.hip", "w4a16_quant.hip",
                "w4a16_group.hip", "w4a16_kv.hip", "w4a16_kv_attn.hip",
-               "w4a16_kv_shared.hip", "w4a16_kv_move.hip", "w4a16_sample.hip"]
+               "w4a16_kv_shared.hip", "w4a16_kv_shared_64.hip", "w4a16_kv_shared_128.hip", "w4a16_kv_shared_256.hip",
+               "w4a16_kv_move.hip", "w4a16_sample.hip"]
 
 
 def build_hip(verbose: bool = False) -> str:

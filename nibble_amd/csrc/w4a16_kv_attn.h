@@ -50,20 +50,24 @@ struct AttnArgs {
     int tokens, heads, kv_heads, group, block_log, splits, least, row_tiles;
     bool vec;
     bool early;   // shares request their first chunk before `start` has arrived
-    // of the forms that write shares alone (Prefix, Own): a row's states, and
-    // which of them the first share's is; Prefix: sequences of a group and their
-    // tokens (`tokens` counts those of all together)
+    // of the other modes: a row's states, and which of them the first share's is;
+    // sequences of a group and their tokens (Prefix: `tokens` counts those of all
+    // together)
     int pitch, share0, sequences, sequence_tokens;
+    // Last: the launch over the prefixes
+    const int64_t* prefix_lengths;
+    int64_t prefix_slots;
+    int prefix_unit, prefix_splits, prefix_least;
 };
 
 // What a launch attends. Alone: causally over the cache, and writes outputs
 // (or shares, where there are several). Own: the same, always as shares. Prefix:
 // the rows of a group's sequences together over all start[group] slots of their
-// prefix, as shares.
-enum Mode { Alone, Own, Prefix };
+// prefix, as shares. Last: as Alone in one share, joined with those of the prefix.
+enum Mode { Alone, Own, Prefix, Last };
 template <Mode MODE>
 __device__ __forceinline__ int64_t state_at(const AttnArgs& a, int64_t row, int split) {
-    return MODE == Alone ? row * a.splits + split : row * a.pitch + a.share0 + split;
+    return MODE == Alone ? row * a.splits + split : row * a.pitch + (MODE == Last ? 0 : a.share0) + split;
 }
 
 // The sequence and the token that row token t of batch entry b is.
@@ -149,6 +153,16 @@ __host__ __device__ __forceinline__ Shares shares_of(int parts, int splits, int 
     const int even = (parts + splits - 1) / splits;
     const int size = parts <= 3 * least ? (parts > 0 ? parts : 1) : even > least ? even : least;
     return {size, (parts + size - 1) / size};
+}
+
+// Last: whether the prefix of sequence b has a length that its cache holds, and its shares.
+__device__ __forceinline__ bool prefix_known(const AttnArgs& a, int b) {
+    const int64_t n = a.prefix_lengths[b / a.sequences];
+    return n >= 0 && n <= a.prefix_slots;
+}
+__device__ __forceinline__ int prefix_shares(const AttnArgs& a, int b) {
+    const int64_t n = a.prefix_lengths[b / a.sequences];
+    return shares_of((int)((n + a.prefix_unit - 1) / a.prefix_unit), a.prefix_splits, a.prefix_least).count;
 }
 
 // A query row's 16-bit values -> fp16, with the power of two that was divided
@@ -258,21 +272,26 @@ constexpr int kDecodeWaves = 4;
 // with two); two with more rows (20 rows over 131072 slots of int8: 63 us against 73).
 constexpr int chunk_tiles(int dim, int column_tiles) { return dim == 256 || column_tiles > 1 ? 2 : 4; }
 
-template <int D, int NT, int CODES, int TYPE, Mode MODE = Alone>
-__global__ void __launch_bounds__(64 * kDecodeWaves, D * NT > 256 || D == 256 ? 1 : 2)
-decode_kernel(const AttnArgs a) {
+constexpr int decode_dims(int dim) { return dim > 128 ? 128 : dim; }   // joined at a time
+template <int D, int NT>
+struct DecodeLds {
+    float row_max[kDecodeWaves][16 * NT], row_sum[kDecodeWaves][16 * NT];
+    __align__(16) float joined[kDecodeWaves][16][decode_dims(D) + 4];
+};
+
+template <int D, int NT, int CODES, int TYPE, Mode MODE>
+__device__ __forceinline__ void decode_body(const AttnArgs& a, int item, DecodeLds<D, NT>& lds) {
     constexpr int W = kDecodeWaves;
     constexpr int M = chunk_tiles(D, NT), C = 16 * M;
     constexpr int J = D / 64;                    // 16-byte loads of a key row's quarter; words of a value load
-    constexpr int PARTS = D > 128 ? D / 128 : 1;
-    constexpr int DP = D / PARTS;
-    __shared__ float row_max[W][16 * NT], row_sum[W][16 * NT];
-    __shared__ __align__(16) float joined[W][16][DP + 4];
+    constexpr int DP = decode_dims(D), PARTS = D / DP;
+    auto& row_max = lds.row_max;
+    auto& row_sum = lds.row_sum;
+    auto& joined = lds.joined;
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int c = lane & 15, h = lane >> 4;
-    int item = blockIdx.x;
     const int split = item % a.splits;
     item /= a.splits;
     const int tile = item % a.row_tiles;
@@ -517,7 +536,7 @@ decode_kernel(const AttnArgs a) {
                     : (D / 16) * (4 * (q / (4 / PARTS)) + part * (4 / PARTS) + q % (4 / PARTS)) + col % (D / 16);
                 const int t = r / a.group, g = r - t * a.group;
                 const int64_t at = ((int64_t)b * a.tokens + t) * a.heads + hk * a.group + g;
-                if (MODE != Alone || shares.count > 1) {
+                if (MODE != Alone || shares.count > 1) {   // (no Last among these)
                     const int64_t sp = state_at<MODE>(a, at, split);
                     *reinterpret_cast<f32x4*>(a.partial + sp * D + dim) = o;
                     if (col == 0 && part == 0) a.states[sp] = make_float2(t0, l);
@@ -535,6 +554,15 @@ decode_kernel(const AttnArgs a) {
             }
         }
     }
+}
+
+// (three row tiles of 128 dims take the registers of two wavefronts a SIMD as two do)
+constexpr int decode_workgroups(int dim, int column_tiles) { return dim * column_tiles > 384 || dim == 256 ? 1 : 2; }
+
+template <int D, int NT, int CODES, int TYPE>
+__global__ void __launch_bounds__(64 * kDecodeWaves, D * NT > 256 || D == 256 ? 1 : 2) decode_kernel(const AttnArgs a) {
+    __shared__ DecodeLds<D, NT> lds;
+    decode_body<D, NT, CODES, TYPE, Alone>(a, blockIdx.x, lds);
 }
 
 // The shares of an output row joined by a workgroup: out = sum_s acc_s 2^(R_s
@@ -669,6 +697,19 @@ __device__ __forceinline__ void attend_row(const AttnArgs& a, const Seen& seen, 
         if (lane == 0) a.states[sp] = make_float2(top, sum);
         return;
     }
+    if constexpr (MODE == Last) {
+        const int count = inside && prefix_known(a, b) ? prefix_shares(a, b) : 0;
+        for (int s = 0; s < count; ++s) {
+            const float2 state = a.states[at * a.pitch + s];
+            const float mx = fmaxf(top, state.x);
+            if (mx == -__builtin_inff()) continue;
+            const float own = __builtin_amdgcn_exp2f(top - mx), f = __builtin_amdgcn_exp2f(state.x - mx);
+            top = mx;
+            sum = sum * own + state.y * f;
+            for (int i = 0; i < E; ++i) o[i] = o[i] * own + a.partial[(at * a.pitch + s) * D + lane * E + i] * f;
+        }
+        if (!prefix_known(a, b)) sum = __builtin_nanf("");
+    }
     const float inv = t >= seen.count ? 0.0f : inside ? 1.0f / sum : __builtin_nanf("");
     for (int i = 0; i < E; ++i) a.out[at * D + lane * E + i] = (uint16_t)narrow16<TYPE>(o[i] * inv);
 }
@@ -699,10 +740,16 @@ __device__ __forceinline__ float half_pair_sum(float v) {
     return __builtin_bit_cast(float, (uint32_t)x[0]) + __builtin_bit_cast(float, (uint32_t)x[1]);
 }
 
-// head_dim 256 keeps its outputs and queries in 512 registers, one wavefront a SIMD
-template <int D, int W, int KS, int CODES, int TYPE, Mode MODE = Alone>
-__global__ void __launch_bounds__(64 * W * KS, D == 256 ? 1 : 2)
-prompt_kernel(const AttnArgs a) {
+// head_dim 256 keeps its outputs and queries in 512 registers, one wavefront a SIMD.
+// OWN (own.NT > 0): with the workgroups from prefix_blocks on, which attend `own` in
+// the decode form (Prefix with Own in one launch; not a body of its own beside the
+// decode form's: so the compiler keeps the arguments in too many registers).
+struct OwnArgs {
+    AttnArgs args;
+    int prefix_blocks;
+};
+template <int D, int W, int KS, int CODES, int TYPE, Mode MODE = Alone, int NT = 0, typename... Beside>
+__global__ void __launch_bounds__(64 * W * KS, D == 256 ? 1 : 2) prompt_kernel(const AttnArgs a, const Beside... beside) {
     constexpr int KT = D == 256 ? 32 : 64;   // slots of a tile
     constexpr int KN = KT / 32;
     constexpr int KROW = D + 8;              // fp16 values of a key row in LDS
@@ -713,6 +760,15 @@ prompt_kernel(const AttnArgs a) {
     constexpr int VW = KT * D / 32 / 64;                  // and values: the last ones
     constexpr int KSIZE = KT * KROW, VSIZE = D * VROW;
     __shared__ __align__(16) f16 staged[KS][2 * (KSIZE + VSIZE)];
+    if constexpr (NT > 0) {
+        static_assert(64 * W * KS == 64 * kDecodeWaves && sizeof(DecodeLds<D, NT>) <= sizeof(staged), "one launch for both");
+        const OwnArgs& own = (beside, ...);
+        if ((int)blockIdx.x >= own.prefix_blocks) {
+            decode_body<D, NT, CODES, TYPE, Own>(own.args, (int)blockIdx.x - own.prefix_blocks,
+                                                 *reinterpret_cast<DecodeLds<D, NT>*>(staged));
+            return;
+        }
+    }
 
     // KS groups of W wavefronts attend the same rows, each every KS-th tile
     const int group = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * W));
@@ -1022,7 +1078,7 @@ prompt_kernel(const AttnArgs a) {
     if (__any(fabsf(run_max) < __builtin_inff() && (fabsf(run_max) >= kLarge || finite != 0.0f))) {
         for (int row = wave0; row < min(wave0 + 32, rows); ++row)
             attend_row<D, CODES, TYPE, MODE>(a, seen, b, hk, row, (int64_t)split * shares.size * KT,
-                                             (int64_t)stop * KT, MODE != Alone || shares.count > 1 ? split : -1);
+                                             (int64_t)stop * KT, MODE == Own || MODE == Prefix || shares.count > 1 ? split : -1);
         return;
     }
     if (wave0 + n >= rows) return;
@@ -1041,7 +1097,37 @@ prompt_kernel(const AttnArgs a) {
         }
         return x;
     };
-    if (MODE != Alone || shares.count > 1) {
+    if constexpr (MODE == Last) {
+        // joined with the shares of the prefix, of which a lane reads the dims that it holds
+        const bool known = prefix_known(a, b);
+        const int count = inside && known ? prefix_shares(a, b) : 0;
+        const float2* states = a.states + at * a.pitch;
+        float top = run_max;
+        for (int s = 0; s < count; ++s) top = fmaxf(top, states[s].x);
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+        const float own = __builtin_amdgcn_exp2f(run_max - base);
+        run_sum *= own;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= own;
+        for (int s = 0; s < count; ++s) {
+            const float2 state = states[s];
+            const float f = __builtin_amdgcn_exp2f(state.x - base);
+            run_sum = __builtin_fmaf(state.y, f, run_sum);
+            const float* part = a.partial + (at * a.pitch + s) * D;
+#pragma unroll
+            for (int v = 0; v < D / 8; ++v) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(part + dim_of(v));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = place(v) + e * (D / 4);
+                    const int i = 4 * ((row >> 3) & 3) + (row & 3);
+                    acc[row >> 5][i] = __builtin_fmaf(x[e], f, acc[row >> 5][i]);
+                }
+            }
+        }
+        if (!known && !(t >= seen.count)) run_sum = __builtin_nanf("");
+    }
+    if (MODE == Own || MODE == Prefix || (MODE == Alone && shares.count > 1)) {
         const int64_t sp = state_at<MODE>(a, at, split);
         if (h == 0) a.states[sp] = make_float2(run_max, run_sum);
         float* o = a.partial + sp * D;

@@ -34,20 +34,34 @@ __device__ __forceinline__ int64_t moved_slots(const MoveArgs& a, int64_t source
     return source < 0 || source >= a.held ? 0 : min(max(a.lengths[source], (int64_t)0), a.slots);
 }
 
+// A store of 16 bytes; past the caches where much is moved.
+template <bool FAR>
+__device__ __forceinline__ void put(u32x4* to, u32x4 v) {
+    if constexpr (FAR)
+        __builtin_nontemporal_store(v, to);
+    else
+        *to = v;
+}
+
 // ---------------------------------------------------------------------------
 // Between two caches: a workgroup copies a chunk of a head of one sequence, 16
 // bytes a lane and load, the blocks that start in it with their scales.
+//
+// Bound: memory (3 sequences of up to 4001 tokens, 8 KV heads of 128, into 24: 30
+// us for 91 MB written; 61 with the sequences of a chunk one after the other and
+// stores that stay in the caches, 40 and 50 with one of the two).
 // ---------------------------------------------------------------------------
-constexpr int kForkUnits = 4;   // of a thread
+constexpr int kForkUnits = 2;   // of a thread: 30 us, with four 32, with one 51
 
+template <bool FAR>
 __global__ void __launch_bounds__(256) fork_kernel(const MoveArgs a) {
     int item = blockIdx.x;
-    const int b = item % a.batch;
-    item /= a.batch;
+    const int64_t slot0 = (int64_t)(item % a.chunks) * a.chunk;
+    item /= a.chunks;
     const int h = item % a.kv_heads;
     item /= a.kv_heads;
     const MoveSide& s = a.side[item & 1];
-    const int64_t slot0 = (int64_t)(item >> 1) * a.chunk;
+    const int b = item >> 1;
     const int64_t source = a.source[b];
     const int64_t slots = moved_slots(a, source);
     if (slot0 >= slots) return;
@@ -66,15 +80,19 @@ __global__ void __launch_bounds__(256) fork_kernel(const MoveArgs a) {
 #pragma unroll
     for (int i = 0; i < kForkUnits; ++i) {
         const int u = (int)threadIdx.x + 256 * i;
-        if (u < n * a.units) to[u] = v[i];
+        if (u < n * a.units) put<FAR>(to + u, v[i]);
     }
 }
 
 // ---------------------------------------------------------------------------
 // Within a cache: a workgroup holds the same slots of a head of all sequences in
 // registers, U units a thread, and writes none before all are read.
+//
+// Bound: memory (beams of 32 sequences of up to 2000 tokens, 8 KV heads of 128: 33
+// us for 75 MB written; 51 with stores that stay in the caches, 60 with 16 units a
+// thread).
 // ---------------------------------------------------------------------------
-template <int T, int U>
+template <int T, int U, bool FAR>
 __global__ void __launch_bounds__(T) reorder_kernel(const MoveArgs a) {
     int item = blockIdx.x;
     const int h = item % a.kv_heads;
@@ -119,7 +137,7 @@ __global__ void __launch_bounds__(T) reorder_kernel(const MoveArgs a) {
     for (int i = 0; i < U; ++i) {
         const int u = (int)threadIdx.x + T * i;
         const int b = u / row, at = u - b * row;
-        if (moves[i]) reinterpret_cast<u32x4*>(s.to + b * s.tb + h * s.th)[slot0 * a.units + at] = v[i];
+        if (moves[i]) put<FAR>(reinterpret_cast<u32x4*>(s.to + b * s.tb + h * s.th) + slot0 * a.units + at, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < S; ++i) {
@@ -158,6 +176,11 @@ MoveArgs args_of(const w4a16_kv_cache& from, const w4a16_kv_cache& to, const int
     return a;
 }
 
+// Whether a cache is too large to stay in the device's caches between calls.
+bool is_far(const w4a16_kv_cache& c) {
+    return (__int128)2 * c.batch * c.kv_heads * c.slots * c.head_dim > (32 << 20);
+}
+
 int finish() {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return kv_fail(W4A16_ERR_LAUNCH, std::string("kernel launch failed: ") + hipGetErrorString(e));
@@ -184,7 +207,12 @@ int w4a16_kv_fork(const w4a16_kv_cache* from, const w4a16_kv_cache* to, const in
     if (!w4a16_internal::launch_fits(grid, 256)) return kv_fail(W4A16_ERR_TOO_LARGE, "too many sequences for one launch");
     if ((rc = w4a16_internal::check_written(*to)) != W4A16_OK) return rc;
     if ((rc = w4a16_internal::check_apart(*from, *to)) != W4A16_OK) return rc;
-    hipLaunchKernelGGL(fork_kernel, dim3((unsigned)grid), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    const dim3 g((unsigned)grid), t(256);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (is_far(*to))
+        hipLaunchKernelGGL((fork_kernel<true>), g, t, 0, st, a);
+    else
+        hipLaunchKernelGGL((fork_kernel<false>), g, t, 0, st, a);
     return finish();
 }
 
@@ -207,11 +235,13 @@ int w4a16_kv_reorder(const w4a16_kv_cache* cache, const int64_t* source, const i
     const dim3 g((unsigned)grid), t((unsigned)threads);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (threads == 1024)
-        hipLaunchKernelGGL((reorder_kernel<1024, 16>), g, t, 0, st, a);
+        hipLaunchKernelGGL((reorder_kernel<1024, 16, true>), g, t, 0, st, a);
     else if (units == 16)
-        hipLaunchKernelGGL((reorder_kernel<256, 16>), g, t, 0, st, a);
+        hipLaunchKernelGGL((reorder_kernel<256, 16, true>), g, t, 0, st, a);
+    else if (is_far(*cache))
+        hipLaunchKernelGGL((reorder_kernel<256, 4, true>), g, t, 0, st, a);
     else
-        hipLaunchKernelGGL((reorder_kernel<256, 4>), g, t, 0, st, a);
+        hipLaunchKernelGGL((reorder_kernel<256, 4, false>), g, t, 0, st, a);
     return finish();
 }
 

@@ -1,193 +1,81 @@
 // Attention of a batch whose sequences share a prefix (include/w4a16_kv.h): the
-// plan, the launches and the joining of their shares. The attending kernels are
-// those of w4a16_kv_attn.h.
-//
-// Mathematics. The softmax over a prefix and a sequence's own slots is that over
-// the two apart, joined by their states: with R, l, o of each share s,
-//     out = sum_s o_s 2^(R_s - R) / sum_s l_s 2^(R_s - R).
-// So the rows of all sequences behind one prefix attend it together, as the rows
-// of one long sequence would, and a key or value of the prefix is read once for
-// all of them.
+// checks and the plan. The kernels are in w4a16_kv_shared.h.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
 #include <string>
 
 #include "w4a16_hip.h"
-#include "w4a16_kv_attn.h"
 #include "w4a16_kv_host.h"
-
-namespace w4a16 {
-
-// The shares of an output row joined, by W wavefronts (a workgroup of 256
-// threads joins 4 / W rows). Lane s holds share s's state (at most 64): those of
-// the prefix first, then the sequence's own. `unit` slots a chunk or tile of the
-// launches before, `own_rows` rows a workgroup of the own slots' launch: they give
-// the shares that were written.
-template <int D, int TYPE, int W>
-__global__ void __launch_bounds__(256) join_kernel(const AttnArgs prefix, const AttnArgs own, int prefix_unit,
-                                                   int own_unit, int own_rows, int64_t rows) {
-    constexpr int E = D / 64;   // dims a lane
-    constexpr int F = 4;        // shares of a wavefront in flight
-    __shared__ float parts[W][D];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W, lane = threadIdx.x & 63;
-    const int64_t row = blockIdx.x * (int64_t)(4 / W) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
-    if (row >= rows) return;   // W == 1 alone: a wavefront for itself
-    const float* part = own.partial + row * own.pitch * D + lane * E;
-    float v[F][E];
-    auto load = [&](int s0) {
-#pragma unroll
-        for (int x = 0; x < F; ++x)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[x][e] = part[(int64_t)min(s0 + W * x, own.pitch - 1) * D + e];
-    };
-    // requested before the lengths tell which of them were written
-    load(wave);
-    float2 state = own.states[row * own.pitch + min(lane, own.pitch - 1)];
-    const int64_t bt = row / own.heads;
-    const int head = (int)(row - bt * own.heads);
-    const int b = (int)(bt / own.tokens), t = (int)(bt - (int64_t)b * own.tokens);
-    const Seen seen = seen_of(own, b);
-    const int r = t * own.group + head % own.group;
-    const int end = seen_end(own, seen, r - r % own_rows, own_rows);
-    const int own_count = shares_of((end + own_unit - 1) / own_unit, own.splits, own.least).count;
-    const int64_t n = prefix.start[b / prefix.sequences];
-    const bool known = n >= 0 && n <= prefix.slots;
-    const int prefix_count =
-        known ? shares_of((int)((n + prefix_unit - 1) / prefix_unit), prefix.splits, prefix.least).count : 0;
-    const int64_t p = seen.start + t;
-    const bool padding = t >= seen.count;
-    const bool inside = !padding && known && p >= 0 && p < own.slots;
-    // what was not written may be anything
-    const int s = lane - own.share0;
-    if (!inside || !(s < 0 ? lane < prefix_count : s < own_count)) state = make_float2(-__builtin_inff(), 0.0f);
-    float o[E] = {};
-    const float top = wave_max(state.x);
-    const float f = state.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.x - top);
-    if (inside) {
-        for (int s0 = wave; s0 < own.pitch; s0 += W * F) {
-#pragma unroll
-            for (int x = 0; x < F; ++x) {
-                const int at = s0 + W * x;
-                const bool written = at < own.pitch && (at < own.share0 ? at < prefix_count : at - own.share0 < own_count);
-                const float fs = __builtin_bit_cast(
-                    float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(at, own.pitch - 1)));
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = written ? __builtin_fmaf(v[x][e], fs, o[e]) : o[e];
-            }
-            if (s0 + W * F < own.pitch) load(s0 + W * F);
-        }
-    }
-    if constexpr (W > 1) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) parts[wave][lane * E + e] = o[e];
-        __syncthreads();
-        if (wave != 0) return;
-#pragma unroll
-        for (int w = 1; w < W; ++w)
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += parts[w][lane * E + e];
-    }
-    const float inv = padding ? 0.0f : inside ? 1.0f / wave_sum(state.y * f) : __builtin_nanf("");
-    uint16_t* out = own.out + row * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) out[e] = (uint16_t)narrow16<TYPE>(o[e] * inv);
-}
-
-}  // namespace w4a16
+#include "w4a16_kv_shared.h"
 
 namespace {
 
 using namespace w4a16;
 using w4a16_internal::kv_fail;
 
-// How one side (a prefix, or the sequences' own slots) is launched.
-struct SidePlan {
-    bool prompt;
-    int column_tiles;   // NT of the decode form
-    int rows_per;
-    int64_t row_tiles;
-    int unit;           // slots of a chunk or tile
-    int splits, least;
-    int threads;
-};
-
 constexpr int kMostPrefixShares = 48, kMostOwnShares = 16;
 
-SidePlan plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t slots, int64_t dim, int most_shares) {
-    SidePlan p;
-    p.prompt = rows > 64;
-    p.column_tiles = rows <= 16 ? 1 : rows <= 32 || dim == 256 ? 2 : 4;
-    p.rows_per = p.prompt ? 128 : 16 * p.column_tiles;
+// Rows a workgroup, and the slots' shares: at most `most_shares`, and so many that
+// `workgroups` are launched.
+SidePlan plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t slots, int64_t dim, int most_shares,
+                   int64_t workgroups, SidePlan p) {
+    p.rows_per = p.prompt ? 32 * p.waves : 16 * p.column_tiles;
     p.row_tiles = (rows + p.rows_per - 1) / p.rows_per;
     p.unit = p.prompt ? (dim == 256 ? 32 : 64) : 16 * chunk_tiles((int)dim, p.column_tiles);
-    p.least = p.prompt ? 2 : 4;
-    p.threads = p.prompt && dim <= 128 ? 512 : 256;
+    p.threads = p.prompt ? 64 * p.waves * p.groups : 64 * kDecodeWaves;
     const int64_t groups = batch * kv_heads * p.row_tiles;
-    int64_t splits = groups > 0 ? 256 / groups : 1;
+    int64_t splits = groups > 0 ? (workgroups + groups - 1) / groups : 1;
     const int64_t most = shares_of((int)((slots + p.unit - 1) / p.unit), most_shares, p.least).count;
     if (splits > most) splits = most;
     p.splits = splits < 1 ? 1 : (int)splits;
     return p;
 }
 
-struct Plan {
-    SidePlan prefix, own;
-    int pitch;
-};
-
-Plan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
-                 int64_t slots, int64_t dim) {
-    const int64_t group = heads / kv_heads;
-    Plan p;
-    p.prefix = plan_side(groups, batch / groups * tokens * group, kv_heads, prefix_slots, dim, kMostPrefixShares);
-    p.own = plan_side(batch, tokens * group, kv_heads, slots, dim, kMostOwnShares);
-    p.pitch = p.prefix.splits + p.own.splits;
+SharedPlan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int64_t tokens, int64_t heads,
+                       int64_t kv_heads, int64_t slots, int64_t dim) {
+    const int64_t group = heads / kv_heads, rows = tokens * group, all = batch / groups * rows;
+    SharedPlan p{};
+    SidePlan prefix{}, own{};
+    prefix.waves = own.waves = 4;
+    prefix.groups = own.groups = 1;
+    own.prompt = rows > 64;
+    own.column_tiles = rows <= 16 ? 1 : 2;
+    // The rules below know the caches' capacities, not the lengths, which are on the device.
+    if (own.prompt) {
+        // Two launches, the second of which joins the prefix's shares unless its own
+        // rows leave the chip empty. Workgroups of 256 rows of the prefix (4 x 500
+        // tokens, 32/8 heads of 128, behind 6000: 196 us, of 128 rows 218), of a
+        // sequence's own rows as attention over one cache has them (202 with 256).
+        prefix.prompt = true;
+        prefix.waves = dim <= 128 ? 8 : 4;
+        own.waves = dim <= 128 && batch * kv_heads * ((rows + 255) / 256) >= 512 ? 8 : 4;
+        prefix.least = own.least = 8;
+        p.prefix = plan_side(groups, all, kv_heads, prefix_slots, dim, kMostPrefixShares, 256, prefix);
+        p.own = plan_side(batch, rows, kv_heads, slots, dim, kMostOwnShares, 256, own);
+        p.last = p.own.splits == 1;
+    } else {
+        // One launch for both, and one that joins. The prefix in the decode form up
+        // to 64 rows, 128 over short prefixes (128 rows of 128 dims over 3000 slots: 19
+        // us, in the prompt form 23; over 8192 slots the other way round): of 48 rows a workgroup where these are the fewest (42 rows over
+        // 4 x 30001 slots: 42 us, of 32 rows 47), two of them a compute unit from 17
+        // rows on over long prefixes (32 rows over 100000 slots: 52 us, one 54; 16
+        // rows 53, one 47). In the prompt form, which has the matrix cores to do,
+        // fewer workgroups where the sequences' own slots, which have the memory,
+        // take as long (64 sequences of up to 1024 slots behind 8192: 160 workgroups
+        // 37 us, 256 of them 44; of up to 64 behind 32768: 63, and 128 of them 95).
+        prefix.prompt = all > (dim == 128 && prefix_slots <= 4096 ? 128 : 64);
+        prefix.column_tiles = all <= 16 ? 1 : all <= 32 || dim == 256 ? 2 : dim == 64 ? 4 : all <= 48 ? 3 : 2;
+        if (prefix.column_tiles < own.column_tiles) prefix.column_tiles = own.column_tiles;
+        prefix.least = prefix.prompt ? 2 : 4;
+        own.least = 4;
+        const int64_t workgroups = prefix.prompt ? (batch / groups * slots >= 4 * prefix_slots ? 160 : 256)
+                                   : prefix.column_tiles >= 2 && all <= 48 && dim <= 128 && prefix_slots >= 8192 ? 512 : 256;
+        p.prefix = plan_side(groups, all, kv_heads, prefix_slots, dim, kMostPrefixShares, workgroups, prefix);
+        p.own = plan_side(batch, rows, kv_heads, slots, dim, kMostOwnShares, 256, own);
+    }
+    p.pitch = p.prefix.splits + (p.last ? 0 : p.own.splits);
     return p;
-}
-
-template <int D, int CODES, int TYPE, Mode MODE>
-void launch_side(const SidePlan& p, const AttnArgs& a, int64_t grid, hipStream_t st) {
-    const dim3 g((unsigned)grid), threads((unsigned)p.threads);
-    if (p.prompt)
-        hipLaunchKernelGGL((prompt_kernel<D, 4, D == 256 ? 1 : 2, CODES, TYPE, MODE>), g, threads, 0, st, a);
-    else if (p.column_tiles == 1)
-        hipLaunchKernelGGL((decode_kernel<D, 1, CODES, TYPE, MODE>), g, threads, 0, st, a);
-    else if (p.column_tiles == 2)
-        hipLaunchKernelGGL((decode_kernel<D, 2, CODES, TYPE, MODE>), g, threads, 0, st, a);
-    else if constexpr (D <= 128)
-        hipLaunchKernelGGL((decode_kernel<D, 4, CODES, TYPE, MODE>), g, threads, 0, st, a);
-}
-
-struct Call {
-    Plan plan;
-    AttnArgs prefix, own;
-    int64_t prefix_grid, own_grid, rows;
-    hipStream_t stream;
-};
-
-template <int D, int CODES, int TYPE>
-void launch(const Call& c) {
-    launch_side<D, CODES, TYPE, Prefix>(c.plan.prefix, c.prefix, c.prefix_grid, c.stream);
-    launch_side<D, CODES, TYPE, Own>(c.plan.own, c.own, c.own_grid, c.stream);
-    if (c.plan.pitch > 8)
-        hipLaunchKernelGGL((join_kernel<D, TYPE, 4>), dim3((unsigned)c.rows), dim3(256), 0, c.stream, c.prefix, c.own,
-                           c.plan.prefix.unit, c.plan.own.unit, c.plan.own.rows_per, c.rows);
-    else
-        hipLaunchKernelGGL((join_kernel<D, TYPE, 1>), dim3((unsigned)((c.rows + 3) / 4)), dim3(256), 0, c.stream,
-                           c.prefix, c.own, c.plan.prefix.unit, c.plan.own.unit, c.plan.own.rows_per, c.rows);
-}
-
-template <int D>
-void launch_dim(const Call& c, int code_type, int type) {
-    if (code_type == W4A16_KV_INT8 && type == W4A16_FP16)
-        launch<D, W4A16_KV_INT8, W4A16_FP16>(c);
-    else if (code_type == W4A16_KV_INT8)
-        launch<D, W4A16_KV_INT8, W4A16_BF16>(c);
-    else if (type == W4A16_FP16)
-        launch<D, W4A16_KV_FP8, W4A16_FP16>(c);
-    else
-        launch<D, W4A16_KV_FP8, W4A16_BF16>(c);
 }
 
 bool sizes_fit(int64_t groups, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads) {
@@ -229,7 +117,7 @@ int64_t w4a16_kv_shared_attention_workspace_bytes(int64_t groups, int64_t prefix
                                                   int64_t heads, int64_t kv_heads, int64_t slots, int64_t head_dim) {
     if (!sizes_fit(groups, batch, tokens, heads, kv_heads) || prefix_slots < 1 || slots < 1 || batch == 0 || tokens == 0)
         return 0;
-    const Plan p = plan_shared(groups, prefix_slots, batch, tokens, heads, kv_heads, slots, head_dim);
+    const SharedPlan p = plan_shared(groups, prefix_slots, batch, tokens, heads, kv_heads, slots, head_dim);
     return batch * tokens * heads * p.pitch * (4 * head_dim + 8);
 }
 
@@ -256,7 +144,7 @@ int w4a16_kv_shared_attention(const w4a16_kv_rows* q, void* out, int64_t tokens,
     if ((reinterpret_cast<uintptr_t>(q->data) & 1u) != 0 || (reinterpret_cast<uintptr_t>(out) & 15u) != 0)
         return kv_fail(W4A16_ERR_ALIGNMENT, "q must be 2-byte and out 16-byte aligned");
     const int64_t dim = cache->head_dim, batch = cache->batch, groups = prefix->batch;
-    Call c{};
+    SharedCall c{};
     c.plan = plan_shared(groups, prefix->slots, batch, tokens, heads, cache->kv_heads, cache->slots, dim);
     c.rows = batch * tokens * heads;
     if (workspace == nullptr || workspace_bytes < c.rows * c.plan.pitch * (4 * dim + 8))
@@ -265,8 +153,7 @@ int w4a16_kv_shared_attention(const w4a16_kv_rows* q, void* out, int64_t tokens,
         return kv_fail(W4A16_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
     c.prefix_grid = groups * cache->kv_heads * c.plan.prefix.row_tiles * c.plan.prefix.splits;
     c.own_grid = batch * cache->kv_heads * c.plan.own.row_tiles * c.plan.own.splits;
-    if (!w4a16_internal::launch_fits(c.prefix_grid, c.plan.prefix.threads) ||
-        !w4a16_internal::launch_fits(c.own_grid, c.plan.own.threads) || !w4a16_internal::launch_fits(c.rows, 256))
+    if (!w4a16_internal::launch_fits((__int128)c.prefix_grid + c.own_grid, 512) || !w4a16_internal::launch_fits(c.rows, 256))
         return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
     AttnArgs a{};
     a.q = static_cast<const uint16_t*>(q->data);
@@ -295,15 +182,20 @@ int w4a16_kv_shared_attention(const w4a16_kv_rows* q, void* out, int64_t tokens,
     c.own.start = start;
     c.own.tokens = (int)tokens;
     c.own.share0 = c.plan.prefix.splits;
+    c.own.prefix_lengths = prefix_lengths;
+    c.own.prefix_slots = prefix->slots;
+    c.own.prefix_unit = c.plan.prefix.unit;
+    c.own.prefix_splits = c.plan.prefix.splits;
+    c.own.prefix_least = c.plan.prefix.least;
     set_cache(c.own, *cache);
     set_plan(c.own, c.plan.own, batch, dim);
     c.stream = static_cast<hipStream_t>(stream);
     if (dim == 64)
-        launch_dim<64>(c, cache->code_type, type);
+        launch_shared<64>(c, cache->code_type, type);
     else if (dim == 128)
-        launch_dim<128>(c, cache->code_type, type);
+        launch_shared<128>(c, cache->code_type, type);
     else
-        launch_dim<256>(c, cache->code_type, type);
+        launch_shared<256>(c, cache->code_type, type);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return kv_fail(W4A16_ERR_LAUNCH, std::string("kernel launch failed: ") + hipGetErrorString(e));
     return W4A16_OK;
