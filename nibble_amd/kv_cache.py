@@ -65,6 +65,15 @@ class QuantizedKVCache:
         """(k_codes, k_scales, v_codes, v_scales)."""
         return self.k_codes, self.k_scales, self.v_codes, self.v_scales
 
+    def first(self, batch: int) -> QuantizedKVCache:
+        """The first ``batch`` sequences as a cache of their own, in the same memory."""
+        if not 0 < batch <= self.k_codes.shape[0]:
+            raise ValueError("batch must be between 1 and the cache's")
+        part = object.__new__(QuantizedKVCache)
+        part.k_codes, part.k_scales, part.v_codes, part.v_scales = (t[:batch] for t in self.tensors())
+        part.block_size = self.block_size
+        return part
+
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in self.tensors())
 

@@ -46,7 +46,9 @@ the projections take dequantize + hipBLASLt. The attention launch holds up
 to 256 cache slots in LDS and streams longer prompts through it in 256-slot
 blocks where query heads per KV head are a power of two up to 64; other
 head layouts run prompts past 256 tokens as torch ops around the same op. ``capture_prefill(T)`` records
-a T-token prefill in a HIP graph. ``Decoder.capture()`` records one decode step -- embedding, 22 blocks,
+a T-token prefill in a HIP graph. ``sample`` draws tokens by temperature, top-k,
+top-p and min-p, and with an 8-bit cache several sequences for one prompt, which
+share its keys and values (``attend_shared``). ``Decoder.capture()`` records one decode step -- embedding, 22 blocks,
 lm_head, greedy argmax, KV-cache write and position increment -- in a HIP
 graph, so generating a token is one ``graph.replay()``.
 """
@@ -65,6 +67,7 @@ from nibble_amd.kv_cache import QuantizedKVCache
 from nibble_amd.linear import QuantizedLinear
 from nibble_amd.quantization import quantize_and_pack_weights
 from nibble_amd.rope import rope_frequencies, rope_tables
+from nibble_amd.sampling import sample
 
 # Longest prompt the fused prefill takes where the prefill attention cannot
 # stream the caches (query heads per KV head not a power of two up to 64:
@@ -81,6 +84,14 @@ NATIVE_PREFILL_MAX_ROWS = 256
 # 1.1B prefill (one HIP graph): 1024 tokens 4.31 ms with the op against 4.88
 # with dequantize + hipBLASLt from 513 rows; 2048 tokens 7.65 against 7.53.
 FUSED_PREFILL_NATIVE_MAX_ROWS = 1024
+# Most bytes of a layer's cache that `sample` fills with copies of the prompt, one
+# for each sequence; longer prompts are attended to once for all of them. Measured
+# on steps of the 1.1B model (graph, sequences x prompt): 16 x 1024 tokens 955 us
+# with copies, 1010 without; 16 x 3000 (25 MB) 1042 and 1046, 32 x 3000 1413 and
+# 1399.
+FORK_BYTES_MAX = 24 << 20
+# Steps of `sample` between two looks at which sequences have ended.
+EOS_STRIDE = 16
 
 
 @dataclass
@@ -391,6 +402,7 @@ class LlamaDecoder(torch.nn.Module):
         self.k_cache.zero_()
         self.v_cache.zero_()
         logits = self._forward(prompt, positions)
+        self.logits.copy_(logits)
         self.token.copy_(torch.argmax(logits).view(1))
         self.position.fill_(prompt.numel())
         if self.fused:
@@ -713,3 +725,172 @@ class LlamaDecoder(torch.nn.Module):
                 out.append(self.step())
                 left -= 1
         return torch.cat(out)
+
+    def _check_sampling(self, prompt, new_tokens, sequences, random) -> None:
+        if sequences < 1 or new_tokens < 1:
+            raise ValueError("sequences and new_tokens must be greater than zero")
+        if sequences > 1 and self.kv_caches is None:
+            raise ValueError("several sequences need an 8-bit kv_cache")
+        if random is not None and random.shape != (sequences, new_tokens):
+            raise ValueError("random must have shape [sequences, new_tokens]")
+        slots = prompt.numel() + new_tokens - 1
+        if slots > self.cfg.max_seq_len:
+            raise IndexError(f"prompt and new tokens are longer than the key/value cache ({slots} slots of "
+                             f"{self.cfg.max_seq_len})")
+
+    @torch.inference_mode()
+    def sample(self, prompt: torch.Tensor, new_tokens: int, sequences: int = 1, temperature: float = 1.0,
+               top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, random: torch.Tensor | None = None,
+               generator: torch.Generator | None = None, eos: int | None = None,
+               use_graph: bool = True) -> torch.Tensor:
+        """Tokens drawn after the prompt (int64 [T]): int64 [sequences,
+        new_tokens], each by one of the uniform numbers ``random`` (float32
+        [sequences, new_tokens]; drawn with ``generator`` if None) and the
+        settings of ``nibble_amd.sample``.
+
+        One sequence runs the decode step of ``generate`` (its captured graph
+        with use_graph, if ``capture`` recorded one) and continues in the
+        decoder's own state. Several need an 8-bit cache. The prompt is run once;
+        its keys and values are copied into each sequence's cache up to
+        FORK_BYTES_MAX in all and attended to by all sequences together from
+        there on; the decoder's own state stays at the end of the prompt. Their
+        step is recorded in a HIP graph with use_graph.
+
+        With ``eos`` a sequence that has drawn it is filled up with it. When half
+        of the running ones have ended, the others move up and the step goes on
+        with them alone (looked at every EOS_STRIDE tokens)."""
+        self._check_sampling(prompt, new_tokens, sequences, random)
+        if random is None:
+            random = torch.rand((sequences, new_tokens), device=self.token.device, generator=generator)
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        self.prefill(prompt)
+        if sequences == 1:
+            out = self._sample_one(random[0], settings, eos, use_graph).unsqueeze(0)
+        else:
+            out = self._sample_several(prompt.numel(), random, settings, eos, use_graph)
+        if eos is not None:   # nothing counts behind a sequence's first eos
+            ended = (out == eos).cumsum(dim=1) > 0
+            out = torch.where(ended, eos, out)
+        return out
+
+    def _sample_one(self, random: torch.Tensor, settings: dict, eos: int | None, use_graph: bool) -> torch.Tensor:
+        """[new_tokens] from the logits of the prefill on; each step's own greedy
+        token is replaced by the drawn one."""
+        steps = random.numel()
+        out = torch.full((steps,), 0 if eos is None else eos, dtype=torch.int64, device=random.device)
+        for i in range(steps):
+            if i > 0:
+                if use_graph and self.graph is not None:
+                    self.replay()
+                else:
+                    self._step()
+                    self.host_position += 1
+            self.token.copy_(sample(self.logits.unsqueeze(0), random[i:i + 1].contiguous(), **settings))
+            if self.fused:
+                _lib.embedding_f16(self.embed, self.token, self.x_buf)
+            out[i:i + 1] = self.token
+            if eos is not None and i % EOS_STRIDE == EOS_STRIDE - 1 and bool((out[:i + 1] == eos).any()):
+                break
+        return out
+
+    def _sample_several(self, length: int, random: torch.Tensor, settings: dict, eos: int | None,
+                        use_graph: bool) -> torch.Tensor:
+        """[sequences, new_tokens] behind a prompt of `length` tokens, which the decoder's caches hold."""
+        cfg, device = self.cfg, random.device
+        n, steps = random.shape
+        first_logits = self.logits.unsqueeze(0).expand(n, -1)
+        if steps == 1:
+            return sample(first_logits, random[:, 0].contiguous(), **settings).unsqueeze(1)
+        fork = n * length * 2 * cfg.num_kv_heads * cfg.head_dim <= FORK_BYTES_MAX
+        whole = lambda value, rows: torch.full((rows,), value, dtype=torch.int64, device=device)  # noqa: E731
+        lengths = whole(length, 1)
+        caches = [QuantizedKVCache(n, cfg.num_kv_heads, steps - 1 + (length if fork else 0), cfg.head_dim,
+                                   cfg.kv_cache, cfg.kv_block, device) for _ in self.layers]
+        if fork:
+            source = whole(0, n)
+            for cache, held in zip(caches, self.kv_caches):
+                cache.fork_from(held, source, lengths)
+        first = 0 if fork else length       # the row of the rotary tables of the caches' first slot
+        cos, sin = self.cos[first:], self.sin[first:]
+        state = {"token": whole(0, n), "random": torch.empty((n,), dtype=torch.float32, device=device),
+                 "held": whole(length if fork else 0, n), "caches": caches}
+
+        def step():
+            logits = self._rows_forward(state["token"], state["caches"], state["held"], cos, sin,
+                                        None if fork else lengths)
+            state["token"].copy_(sample(logits, state["random"], **settings))
+            state["held"].add_(1)
+
+        out = torch.full((n, steps), 0 if eos is None else eos, dtype=torch.int64, device=device)
+        rows = torch.arange(n, device=device)     # which sequences run
+        state["token"].copy_(sample(first_logits, random[:, 0].contiguous(), **settings))
+        out[:, 0] = state["token"]
+        graph = None
+        for i in range(1, steps):
+            if eos is not None and i % EOS_STRIDE == 0:
+                running = ~(out[rows, :i] == eos).any(dim=1)
+                live = int(running.sum())
+                if live == 0:
+                    break
+                if 2 * live <= rows.numel():      # the others move up
+                    keep = running.nonzero().squeeze(1)
+                    source = torch.cat((keep, whole(-1, rows.numel() - live)))
+                    for cache in state["caches"]:
+                        cache.reorder(source, state["held"])
+                    rows = rows[keep]
+                    state = {"token": state["token"][keep], "random": state["random"][:live].clone(),
+                             "held": state["held"][keep], "caches": [c.first(live) for c in state["caches"]]}
+                    graph = None
+            state["random"].copy_(random[rows, i])
+            if graph is not None:
+                graph.replay()
+            else:
+                step()
+                if use_graph and self.fused and steps - i > 4:   # the steps from the next one on
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        step()
+            out[rows, i] = state["token"]
+        return out
+
+    def _rows_forward(self, tokens: torch.Tensor, caches: list[QuantizedKVCache], held: torch.Tensor,
+                      cos: torch.Tensor, sin: torch.Tensor, prefix_lengths: torch.Tensor | None) -> torch.Tensor:
+        """Logits [n, vocab] of one token of each of n sequences, at the slots
+        `held` of `caches`; with prefix_lengths behind the prompt in the
+        decoder's own caches."""
+        cfg = self.cfg
+        n, width, split = tokens.numel(), cfg.num_heads * cfg.head_dim, [cfg.num_heads, cfg.num_kv_heads, cfg.num_kv_heads]
+
+        def attend(i, qkv):
+            q, k, v = qkv.view(n, 1, -1, cfg.head_dim).split(split, dim=2)
+            q = caches[i].rotary_write(q, k, v, cos, sin, held)
+            if prefix_lengths is None:
+                return caches[i].attend(q, held).view(n, width)
+            return caches[i].attend_shared(q, self.kv_caches[i], prefix_lengths, held).view(n, width)
+
+        x = self.embed[tokens]
+        if not self.fused:
+            for i, b in enumerate(self.layers):
+                h = b.input_norm(x)
+                x = x + b.o_proj(attend(i, torch.cat((b.q_proj(h), b.k_proj(h), b.v_proj(h)), dim=1)))
+                h = b.post_norm(x)
+                x = x + b.down_proj(F.silu(b.gate_proj(h)) * b.up_proj(h))
+            return self.lm_head(self.norm(x))
+        h = torch.empty_like(x)
+        mlp = torch.empty((n, cfg.intermediate_size), dtype=torch.float16, device=x.device)
+        first = self.layers[0].input_norm
+        _lib.rmsnorm_f16(x, first.weight, first.eps, h)
+        for i, b in enumerate(self.layers):
+            o = self._prefill_linear(attend(i, self._prefill_linear(h, *self.qkv[i])), b.o_proj.packed_weights,
+                                     b.o_proj.scales)
+            _lib.add_rmsnorm_f16(x, o, b.post_norm.weight, b.post_norm.eps, x, h)
+            nxt = self.layers[i + 1].input_norm if i + 1 < len(self.layers) else self.norm
+            if n <= FUSED_PREFILL_NATIVE_MAX_ROWS:
+                _lib.linear_silu_f16(h, *self.gate_up[i], mlp, cfg.group_size)
+                _lib.linear_add_rmsnorm_f16(mlp, b.down_proj.packed_weights, b.down_proj.scales, x, nxt.weight, nxt.eps,
+                                            x, h, cfg.group_size)
+            else:
+                _lib.silu_mul_f16(self._prefill_linear(h, *self.gate_up[i]), mlp)
+                _lib.add_rmsnorm_f16(x, self._prefill_linear(mlp, b.down_proj.packed_weights, b.down_proj.scales),
+                                     nxt.weight, nxt.eps, x, h)
+        return self._prefill_linear(h, self.lm_head.packed_weights, self.lm_head.scales)
