@@ -612,6 +612,10 @@ struct Places {
         const uint32_t bits = at == 0 ? 0u : at > 0 ? (uint32_t)(at + kSmall) : (uint32_t)(kSmall - at) | 0x8000u;
         return __builtin_bit_cast(float, bits << 16);
     }
+    // the smaller of `least` and the bits of two logits' magnitudes less 1 (0: none)
+    static __device__ __forceinline__ u16x2 smaller(u16x2 least, uint32_t word) {
+        return __builtin_elementwise_min(least, (__builtin_bit_cast(u16x2, word) & (u16x2)(0x7FFF)) - (u16x2)(1));
+    }
     __device__ __forceinline__ u16x2 of(uint32_t word) const {   // of two logits, at most `end`
         const u16x2 bits = __builtin_bit_cast(u16x2, word);
         const u16x2 size = __builtin_elementwise_sub_sat(bits & (u16x2)(0x7FFF), (u16x2)((uint16_t)kSmall));
@@ -660,11 +664,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
     r.template each4<true>([&](int, const u32x4& v) {
         if constexpr (TYPE == W4A16_BF16) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t word = v[e];
-                smallest = __builtin_elementwise_min(
-                    smallest, (__builtin_bit_cast(Places::u16x2, word) & (Places::u16x2)(0x7FFF)) - (Places::u16x2)(1));
-            }
+            for (int e = 0; e < 4; ++e) smallest = Places::smaller(smallest, v[e]);
         }
 #pragma unroll
         for (int e = 0; e < R::VE; ++e) {
@@ -759,19 +759,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
             if (end <= kValues && (some || nucleus || a.n > end) && !(tiny && places.top <= 0)) {
                 places.end = (Places::u16x2)((uint16_t)(end + (tid & 31)));
                 const int small = places.top >= 0 ? places.top : -1;   // the place of magnitudes below 2^-20
-                for (int i = tid; i < end + 32; i += kThreads) s.value_counts[i] = 0;
-                __syncthreads();
-                r.each4([&](int, const u32x4& v) {
+                const bool counted = some || nucleus;   // else min_p alone gives a limit
+                if (counted) {
+                    for (int i = tid; i < end + 32; i += kThreads) s.value_counts[i] = 0;
+                    __syncthreads();
+                    r.each4([&](int, const u32x4& v) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const Places::u16x2 at = places.of(v[e]);
-                        atomicAdd(&s.value_counts[at.x], 1u);
-                        atomicAdd(&s.value_counts[at.y], 1u);
-                    }
-                });
+                        for (int e = 0; e < 4; ++e) {
+                            const Places::u16x2 at = places.of(v[e]);
+                            atomicAdd(&s.value_counts[at.x], 1u);
+                            atomicAdd(&s.value_counts[at.y], 1u);
+                        }
+                    });
+                }
                 __syncthreads();
                 for (int i = tid; i < end; i += kThreads)
-                    if (s.value_counts[i] != 0) s.value_weights[i] = weights.of(places.value(i));
+                    if (!counted || s.value_counts[i] != 0) s.value_weights[i] = weights.of(places.value(i));
                 __syncthreads();
                 // magnitudes between 0 and 2^-20, which share a place with 0: the few that there
                 // may be have their weights added apart
@@ -779,7 +782,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                 if (tiny) {
                     if (tid == 0) s.tinies = 0;
                     __syncthreads();
-                    r.each([&](int j, const u32x4& v) {
+                    r.each4([&](int j, const u32x4& v) {
+                        Places::u16x2 own = (Places::u16x2)(0xFFFF);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) own = Places::smaller(own, v[e]);
+                        if (min(own.x, own.y) >= Places::kSmall) return;
 #pragma unroll
                         for (int e = 0; e < R::VE; ++e) {
                             const float x = R::value(v, e);
@@ -821,13 +828,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                 // a limit there, or too many of them: the other way
                 if (!tiny || (!among && last != small && s.tinies <= kTiny)) {
                     limited = true;
-                    const uint32_t count = s.value_counts[last];
                     limit = {places.value(last), (int64_t)min(ties, (uint64_t)a.n)};
-                    tie = count != 0 ? s.value_weights[last] : 0;
+                    tie = !counted || s.value_counts[last] != 0 ? s.value_weights[last] : 0;
                     // each value's weight is looked up, 0 of the limit and below
                     __syncthreads();
                     for (int i = tid; i < end + 32; i += kThreads)
-                        if (i >= last || s.value_counts[i] == 0) s.value_weights[i] = 0;
+                        if (i >= last || (counted && s.value_counts[i] == 0)) s.value_weights[i] = 0;
                     __syncthreads();
                     const uint16_t last16 = (uint16_t)last;
                     places.end = (Places::u16x2)((uint16_t)(last + 1 + (tid & 31)));   // zeros of many banks
