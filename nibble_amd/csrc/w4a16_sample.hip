@@ -821,9 +821,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                     const uint64_t w = max(s.value_weights[last], (uint64_t)1);
                     ties = (target - f.before + w - 1) / w;
                 }
-                if (least > -__builtin_inff() && places.of(least) < last) {
+                if (least > places.value(last)) {
                     last = places.of(least);
-                    ties = ~0ull;
+                    ties = least > places.value(last) ? 0 : ~0ull;   // a bound between 0 and 2^-20 keeps no 0
                 }
                 // a limit there, or too many of them: the other way
                 if (!tiny || (!among && last != small && s.tinies <= kTiny)) {

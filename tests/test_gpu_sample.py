@@ -1,5 +1,7 @@
 """Sampling on the GPU against the 64-bit oracle of tests/_sample.py."""
 
+import math
+
 import pytest
 import torch
 
@@ -191,3 +193,18 @@ def test_values_near_zero(gpu, dtype, settings):
         rows[-1][torch.rand(n, generator=g) < 0.01] = 0.0
         rows[-1][torch.rand(n, generator=g) < 0.01] = -0.0
     _check(torch.stack(rows).to(dtype), _sample.numbers(len(rows), 4), **settings)
+
+
+@pytest.mark.parametrize("settings", [{}, {"top_p": 0.97}, {"top_k": 2500}])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_min_p_between_zero_and_small_values(gpu, dtype, sign, settings):
+    """Logits of 0 beside a bound that is nearer to 0 than 2^-20: kept below it (sign -1), not above."""
+    n = 3000
+    logits = torch.full((6, n), -1.0)
+    logits[:, ::7] = 0.0
+    logits[:, 700] = -0.0
+    logits[:, 1500] = 2.0 ** -18          # the largest: 0 weighs e^-3.8
+    temperature = 1e-6
+    min_p = math.exp(-(2.0 ** -18 - sign * 2.0 ** -22) / temperature)
+    _check(logits.to(dtype), _sample.numbers(6, 5), temperature=temperature, min_p=min_p, **settings)
