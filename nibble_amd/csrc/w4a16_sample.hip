@@ -326,24 +326,6 @@ struct Weights {
 };
 __device__ __forceinline__ uint64_t whole(double parts) { return (uint64_t)(parts * (double)kOne); }
 
-__device__ __forceinline__ double wave_total(double v) {   // in lane 63
-#define PLUS_DPP(CTRL, ROWS)                                                                                       \
-    {                                                                                                              \
-        const uint64_t b = __builtin_bit_cast(uint64_t, v);                                                        \
-        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xF, false);              \
-        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xF, false);      \
-        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);                                                  \
-    }
-    PLUS_DPP(0x111, 0xF)
-    PLUS_DPP(0x112, 0xF)
-    PLUS_DPP(0x114, 0xF)
-    PLUS_DPP(0x118, 0xF)
-    PLUS_DPP(0x142, 0xA)
-    PLUS_DPP(0x143, 0xC)
-#undef PLUS_DPP
-    return v;
-}
-
 // The largest value of the workgroup; NaN if a thread brings `strange`. `flag`: of any thread.
 __device__ __forceinline__ float block_max(Shared& s, float v, bool strange, bool& flag) {
     v = wave_max(v);
@@ -470,10 +452,13 @@ __device__ __forceinline__ bool select(Shared& s, Keys keys, uint64_t target, fl
 // Appends indices to s.near, N a lane at most; past kMostNear they are only counted.
 template <int N, typename Index>
 __device__ __forceinline__ void list_near(Shared& s, const bool (&has)[N], Index index) {
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) any |= has[e];
+    if (!__any(any)) return;
     int total = 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) total += __builtin_popcountll(__ballot(has[e]));
-    if (total == 0) return;
     int at = 0;
     if ((threadIdx.x & 63) == 0) at = atomicAdd(&s.listed, total);
     at = __builtin_amdgcn_readfirstlane(at);
@@ -880,7 +865,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                     in_last = (uint64_t)top_k - f.before;
                     uint64_t rest = 0;
                     // few kept tokens are listed all, else those of the last bin
-                    const int from = top_k <= kMostNear * 3 / 4 ? 0 : last_bin;
+                    const int from = top_k <= kMostNear * 7 / 8 ? 0 : last_bin;
                     if (tid == 0) s.listed = 0;
                     __syncthreads();
                     r.each([&](int j, const u32x4& v) {
@@ -959,11 +944,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                     const uint64_t n = i < last_bin ? s.counts[i] : i == last_bin ? min((uint64_t)s.counts[i], in_last) : 0;
                     return (uint64_t)((double)n * (double)kOne * (double)__builtin_amdgcn_exp2f(-(i + 1.01f) / kBinsPerOctave));
                 };
+                // so for each bin the share up to it, and the share behind it, are known to 1.02
                 const Found f0 = find(s, kBins, least_weight, [&](uint64_t total) {
-                    return (uint64_t)fmax(top_p / 1.02 * (double)total, 1.0);
+                    return (uint64_t)fmax(fmax(top_p / 1.02, 1.0 - 1.02 * (1.0 - top_p)) * (double)total, 1.0);
                 });
                 const Found f1 = find(s, kBins, least_weight, [&](uint64_t total) {
-                    return (uint64_t)fmax(top_p * 1.02 * (double)total, 1.0);
+                    return (uint64_t)fmax(fmin(1.02 * top_p, 1.0 - (1.0 - top_p) / 1.02) * (double)total, 1.0);
                 });
                 int first_bin = max(f0.index, 0), end_bin = f1.index >= 0 ? f1.index : kBins - 1;
                 const Limit by_count = limit;
