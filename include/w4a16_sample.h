@@ -46,8 +46,8 @@ typedef struct w4a16_sample_settings {
  * A number below 0 or NaN reads as 0, one of 1 or more gives the last token of a
  * weight. Weights are held to 2^-38 of themselves and rounded to whole multiples
  * of 2^-44 of the largest one (smaller ones count as 0), their sums are exact: the
- * same call gives the same tokens. A row with NaN gives the first NaN's index and a row of -inf token 0,
- * as argmax does; where logits are +inf, those alone have weight.
+ * same call gives the same tokens. A row with NaN gives the first NaN's index and a
+ * row of -inf token 0, as argmax does; where logits are +inf, those alone have weight.
  * tokens share no memory with the other arguments.
  */
 int w4a16_sample(const void* logits, int64_t rows, int64_t n, int64_t row_stride, int type, const float* random,

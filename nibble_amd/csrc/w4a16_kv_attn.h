@@ -741,9 +741,11 @@ __device__ __forceinline__ float half_pair_sum(float v) {
 }
 
 // head_dim 256 keeps its outputs and queries in 512 registers, one wavefront a SIMD.
-// OWN (own.NT > 0): with the workgroups from prefix_blocks on, which attend `own` in
-// the decode form (Prefix with Own in one launch; not a body of its own beside the
-// decode form's: so the compiler keeps the arguments in too many registers).
+// NT > 0: Prefix with Own in one launch, the latter in the decode form by the
+// workgroups from prefix_blocks on (64 sequences of up to 800 slots behind 8192, 8 KV
+// heads of 128: 32 us for 97 MB, 3.0 TB/s). The prompt form is the kernel itself: as a
+// function beside the decode form's it had its arguments in more scalar registers than
+// there are.
 struct OwnArgs {
     AttnArgs args;
     int prefix_blocks;

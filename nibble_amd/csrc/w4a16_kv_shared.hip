@@ -23,7 +23,7 @@ SidePlan plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t slots,
     p.rows_per = p.prompt ? 32 * p.waves : 16 * p.column_tiles;
     p.row_tiles = (rows + p.rows_per - 1) / p.rows_per;
     p.unit = p.prompt ? (dim == 256 ? 32 : 64) : 16 * chunk_tiles((int)dim, p.column_tiles);
-    p.threads = p.prompt ? 64 * p.waves * p.groups : 64 * kDecodeWaves;
+    p.threads = 64 * (p.prompt ? p.waves : kDecodeWaves);
     const int64_t groups = batch * kv_heads * p.row_tiles;
     int64_t splits = groups > 0 ? (workgroups + groups - 1) / groups : 1;
     const int64_t most = shares_of((int)((slots + p.unit - 1) / p.unit), most_shares, p.least).count;
@@ -38,7 +38,6 @@ SharedPlan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int6
     SharedPlan p{};
     SidePlan prefix{}, own{};
     prefix.waves = own.waves = 4;
-    prefix.groups = own.groups = 1;
     own.prompt = rows > 64;
     own.column_tiles = rows <= 16 ? 1 : 2;
     // The rules below know the caches' capacities, not the lengths, which are on the device.
@@ -57,13 +56,14 @@ SharedPlan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int6
     } else {
         // One launch for both, and one that joins. The prefix in the decode form up
         // to 64 rows, 128 over short prefixes (128 rows of 128 dims over 3000 slots: 19
-        // us, in the prompt form 23; over 8192 slots the other way round): of 48 rows a workgroup where these are the fewest (42 rows over
-        // 4 x 30001 slots: 42 us, of 32 rows 47), two of them a compute unit from 17
-        // rows on over long prefixes (32 rows over 100000 slots: 52 us, one 54; 16
-        // rows 53, one 47). In the prompt form, which has the matrix cores to do,
-        // fewer workgroups where the sequences' own slots, which have the memory,
-        // take as long (64 sequences of up to 1024 slots behind 8192: 160 workgroups
-        // 37 us, 256 of them 44; of up to 64 behind 32768: 63, and 128 of them 95).
+        // us, in the prompt form 23; over 8192 slots the other way round): of 48 rows a
+        // workgroup where these are the fewest (42 rows over 4 x 30001 slots: 41 us, of
+        // 32 rows 47), two of them a compute unit from 17 rows on over long prefixes
+        // (32 rows over 100000 slots: 52 us, one 54; 16 rows 53, one 47). In the prompt
+        // form, which has the matrix cores to do, fewer workgroups where the sequences'
+        // own slots, which have the memory, take as long (64 sequences of up to 1024
+        // slots behind 8192: 160 workgroups 37 us, 256 of them 44; of up to 64 behind
+        // 32768: 63, and 128 of them 95).
         prefix.prompt = all > (dim == 128 && prefix_slots <= 4096 ? 128 : 64);
         prefix.column_tiles = all <= 16 ? 1 : all <= 32 || dim == 256 ? 2 : dim == 64 ? 4 : all <= 48 ? 3 : 2;
         if (prefix.column_tiles < own.column_tiles) prefix.column_tiles = own.column_tiles;
@@ -81,7 +81,8 @@ SharedPlan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int6
 bool sizes_fit(int64_t groups, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads) {
     return groups >= 1 && batch >= 0 && batch % groups == 0 && tokens >= 0 && heads >= 1 && kv_heads >= 1 &&
            heads % kv_heads == 0 && batch <= (1 << 24) && tokens <= (1 << 24) && heads <= (1 << 16) &&
-           (__int128)(batch / groups) * tokens * (heads / kv_heads) <= (1 << 28);
+           (__int128)(batch / groups) * tokens * (heads / kv_heads) <= (1 << 28) &&
+           (__int128)batch * tokens * heads <= ((int64_t)1 << 40);
 }
 
 void set_cache(AttnArgs& a, const w4a16_kv_cache& c) {
@@ -153,7 +154,8 @@ int w4a16_kv_shared_attention(const w4a16_kv_rows* q, void* out, int64_t tokens,
         return kv_fail(W4A16_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
     c.prefix_grid = groups * cache->kv_heads * c.plan.prefix.row_tiles * c.plan.prefix.splits;
     c.own_grid = batch * cache->kv_heads * c.plan.own.row_tiles * c.plan.own.splits;
-    if (!w4a16_internal::launch_fits((__int128)c.prefix_grid + c.own_grid, 512) || !w4a16_internal::launch_fits(c.rows, 256))
+    if (!w4a16_internal::launch_fits((__int128)c.prefix_grid + c.own_grid, 512) ||
+        (!c.plan.last && !w4a16_internal::launch_fits(c.rows, 256)))
         return kv_fail(W4A16_ERR_TOO_LARGE, "too many rows for one launch");
     AttnArgs a{};
     a.q = static_cast<const uint16_t*>(q->data);

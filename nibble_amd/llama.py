@@ -92,6 +92,8 @@ FUSED_PREFILL_NATIVE_MAX_ROWS = 1024
 FORK_BYTES_MAX = 24 << 20
 # Steps of `sample` between two looks at which sequences have ended.
 EOS_STRIDE = 16
+# Sequences times head_dim that `QuantizedKVCache.reorder` takes.
+REORDER_VALUES_MAX = 262144
 
 
 @dataclass
@@ -832,7 +834,8 @@ class LlamaDecoder(torch.nn.Module):
                 live = int(running.sum())
                 if live == 0:
                     break
-                if 2 * live <= rows.numel():      # the others move up
+                # the others move up (of no more sequences than a cache is reordered with)
+                if 2 * live <= rows.numel() <= REORDER_VALUES_MAX // cfg.head_dim:
                     keep = running.nonzero().squeeze(1)
                     source = torch.cat((keep, whole(-1, rows.numel() - live)))
                     for cache in state["caches"]:

@@ -217,6 +217,38 @@ def test_captured_streams_and_runs(gpu):
         _kv.close(eager, ref, bound)
 
 
+@pytest.mark.parametrize("codes,dtype", [("int8", "fp16"), ("fp8", "bf16")])
+def test_two_graphs_of_prompts_and_tokens(gpu, codes, dtype):
+    """Prompts and single tokens behind the same prefixes, captured apart and replayed in turn, one in a stream of its own."""
+    q, prefix, own = _shared.case(2, 2, 70, 8, 2, 64, 500, 200, codes, dtype)
+    token = _kv.rows((4, 1, 8, 64), dtype, 77)
+    q, token, prefix, own = q.cuda(), token.cuda(), [x.cuda() for x in prefix], [x.cuda() for x in own]
+    lengths, start, counts = _ints([500, 31]), _ints([0, 9, 100, 130]), _ints([70, 33, 0, 70])
+    calls = [lambda: kv_shared_attention_cuda(q, *prefix, lengths, *own, start, counts),
+             lambda: kv_shared_attention_cuda(token, *prefix, lengths, *own, start)]
+    graphs, outs = [], []
+    for call in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(call())
+    stream = torch.cuda.Stream()
+    for i in range(4):
+        q.copy_(_kv.rows(q.shape, dtype, 80 + i))
+        token.copy_(_kv.rows(token.shape, dtype, 90 + i))
+        lengths.copy_(_ints([500 - 150 * i, 31 + 100 * i]))
+        start.copy_(_ints([i, 9 * i, 100 - i, 130]))
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            graphs[i % 2].replay()
+        graphs[1 - i % 2].replay()
+        torch.cuda.synchronize()
+        for out, call in zip(outs, calls):
+            assert _kv.same(out, call())
+        ref, bound = _shared.attend(q.cpu(), [x.cpu() for x in prefix], lengths.tolist(), [x.cpu() for x in own],
+                                    start.tolist(), counts.tolist(), 64, 32)
+        _kv.close(outs[0], ref, bound)
+
+
 def test_prompt_then_answers(gpu):
     """A prompt, forked into answers or shared by them, then their tokens: the run that a sampled batch makes."""
     heads, kv, dim, n, length = 8, 2, 64, 3, 70

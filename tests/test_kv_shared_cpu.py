@@ -81,6 +81,8 @@ def test_refusals_of_the_c_abi():
     assert call(workspace=None) == call(size=4 * 4 * 64) == _lib.W4A16_ERR_CONFIG
     assert call(workspace=(1 << 44) + 8) == _lib.W4A16_ERR_ALIGNMENT
     assert call(tokens=1 << 25) == call(cache=_cache(1 << 32, batch=1 << 24), tokens=1 << 10) == _lib.W4A16_ERR_TOO_LARGE
+    many = dict(prefix=_cache(1 << 30, batch=1 << 24), cache=_cache(1 << 32, batch=1 << 24))
+    assert call(tokens=1 << 20, **many) == _lib.W4A16_ERR_TOO_LARGE
     assert call(tokens=0) == call(cache=_cache(1 << 32, batch=0)) == _lib.W4A16_OK
     size = _lib.lib().w4a16_kv_shared_attention_workspace_bytes
     assert size(1, 100, 8, 1, 4, 2, 40, 64) > 0 and size(3, 100, 8, 1, 4, 2, 40, 64) == 0

@@ -84,6 +84,19 @@ def test_eos(shared, sequences, monkeypatch):
     assert sequences == 1 or calls
 
 
+def test_eos_of_more_sequences_than_a_cache_is_reordered_with(monkeypatch):
+    """The ended ones run on beside the others."""
+    monkeypatch.setattr(llama, "EOS_STRIDE", 2)
+    model = LlamaDecoder(_cfg(), device="cpu", seed=3)
+    numbers = _numbers(6, 12)
+    free = model.sample(_prompt(9), 12, sequences=6, top_k=3, random=numbers)
+    eos = int(free.flatten().mode().values)
+    want = model.sample(_prompt(9), 12, sequences=6, top_k=3, random=numbers, eos=eos)
+    monkeypatch.setattr(llama, "REORDER_VALUES_MAX", 5 * model.cfg.head_dim)
+    monkeypatch.setattr(llama.QuantizedKVCache, "reorder", None)
+    assert torch.equal(model.sample(_prompt(9), 12, sequences=6, top_k=3, random=numbers, eos=eos), want)
+
+
 def test_refusals():
     model = LlamaDecoder(_cfg(max_seq_len=16), device="cpu")
     plain = LlamaDecoder(_cfg(kv_cache="fp16", max_seq_len=16), device="cpu")
