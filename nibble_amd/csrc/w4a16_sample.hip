@@ -291,7 +291,7 @@ struct Row {
 // before each step otherwise (half of the weights' time).
 __device__ __forceinline__ double fma_scalar(double a, double b, double c) {
     double r;
-    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    asm volatile("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
     return r;
 }
 
@@ -300,28 +300,51 @@ struct Weights {
     double top, factor, lowest;   // lowest: -60 / factor
     // 2^y of y = (x - top) factor <= 0: the whole part joins the exponent, 2^f with
     // |f| <= 1/2 is 1 + f times a polynomial through 8 points, off by 2^-38.7. What
-    // lies far below gives 2^-60.
-    __device__ __forceinline__ double weight(float x) const {
-        const double d = __builtin_fmax((double)x - top, lowest);
+    // lies far below gives 2^-60. N of them step by step together: an operation in 64
+    // bits waits for the one before, which four wavefronts a SIMD do not cover (a
+    // pass over 50257 logits: one by one 12 us).
+    template <int N>
+    __device__ __forceinline__ void weights(const float (&x)[N], double (&w)[N]) const {
         constexpr double round = 0x1.8p52;
-        const double t = __builtin_fma(d, factor, round);
-        const double f = __builtin_fma(d, factor, round - t);
-        double q = 1.325080551750225e-06;
-        q = fma_scalar(q, f, 1.5303700711365693e-05);
-        q = fma_scalar(q, f, 0.00015403475186530786);
-        q = fma_scalar(q, f, 0.0013333478473685416);
-        q = fma_scalar(q, f, 0.00961812913523614);
-        q = fma_scalar(q, f, 0.055504109063258665);
-        q = fma_scalar(q, f, 0.24022650695888503);
-        q = fma_scalar(q, f, 0.6931471805568324);
-        q = __builtin_fma(q, f, 1.0);
-        return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, q) + (__builtin_bit_cast(uint64_t, t) << 52));
+        double t[N], f[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = __builtin_fmax((double)x[i] - top, lowest);
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = __builtin_fma(f[i], factor, round);
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = __builtin_fma(f[i], factor, round - t[i]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = 1.325080551750225e-06;
+        constexpr double terms[7] = {1.5303700711365693e-05, 0.00015403475186530786, 0.0013333478473685416,
+                                     0.00961812913523614, 0.055504109063258665, 0.24022650695888503, 0.6931471805568324};
+#pragma unroll
+        for (int k = 0; k < 7; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = fma_scalar(w[i], f[i], terms[k]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            w[i] = __builtin_fma(w[i], f[i], 1.0);
+            w[i] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, w[i]) + (__builtin_bit_cast(uint64_t, t[i]) << 52));
+        }
+    }
+    __device__ __forceinline__ double weight(float x) const {
+        const float one[1] = {x};
+        double w[1];
+        weights(one, w);
+        return w[0];
     }
     // round(2^44 w): the last bits of 2^8 + w
-    __device__ __forceinline__ uint64_t of(float x) const {
-        return __builtin_bit_cast(uint64_t, weight(x) + 0x1p8) & 0xFFFFFFFFFFFFFull;
+    __device__ __forceinline__ static uint64_t rounded(double w) {
+        return __builtin_bit_cast(uint64_t, w + 0x1p8) & 0xFFFFFFFFFFFFFull;
     }
-    // the same as a double, a multiple of 2^-44: sums below 2^9 of such are exact
+    __device__ __forceinline__ uint64_t of(float x) const { return rounded(weight(x)); }
+    // the same as doubles, multiples of 2^-44: sums below 2^9 of such are exact
+    template <int N>
+    __device__ __forceinline__ void parts(const float (&x)[N], double (&w)[N]) const {
+        weights(x, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = (w[i] + 0x1p8) - 0x1p8;
+    }
     __device__ __forceinline__ double part(float x) const { return (weight(x) + 0x1p8) - 0x1p8; }
 };
 __device__ __forceinline__ uint64_t whole(double parts) { return (uint64_t)(parts * (double)kOne); }
@@ -965,7 +988,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                 const Limit by_count = limit;
                 const uint64_t beside =
                     by_count.value == -__builtin_inff() ? 0 : weights.of(by_count.value) * (uint64_t)by_count.ties;
-                while (true) {
+                // Where min_p keeps none but of the bins before, all of which top_p keeps, the
+                // sum is of no use (where the bins tell the weights: the share behind them
+                // by far more than what 2^19 roundings of a weight make).
+                const bool known = first_bin > 0 && top_p <= 0.999 && factor > 1e-30 && factor < 1e30 &&
+                                   least > limit.value && least >= R::of_key(keys_of<R>(bins, first_bin, end_bin).high);
+                while (!known) {
                     // what lies between, by value; from `high` on it is certain to be kept
                     const Keys keys = keys_of<R>(bins, first_bin, end_bin);
                     const float high = first_bin > 0 ? R::of_key(keys.high) : __builtin_inff(), low = R::of_key(keys.low);
@@ -973,17 +1001,25 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                     __syncthreads();
                     double all = 0.0, above = 0.0, group = 0.0;
                     r.each([&](int j, const u32x4& v) {
-                        bool between[R::VE];
 #pragma unroll
-                        for (int e = 0; e < R::VE; ++e) {
-                            const float x = R::value(v, e);
-                            double w = weights.part(x);
-                            w = x > by_count.value ? w : 0.0;
-                            all += w;
-                            group += x > high ? w : 0.0;
-                            between[e] = x <= high && x >= low && x > by_count.value;
+                        for (int e0 = 0; e0 < R::VE; e0 += 4) {
+                            float x[4];
+                            double w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = R::value(v, e0 + e);
+                            weights.parts(x, w);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const bool counts = x[e] > by_count.value;
+                                w[e] = counts ? w[e] : 0.0;
+                                all += w[e];
+                                group += x[e] > high ? w[e] : 0.0;
+                                if (counts && x[e] <= high && x[e] >= low) {   // few
+                                    const int i = atomicAdd(&s.listed, 1);
+                                    if (i < kMostNear) s.near[i] = r.index(j, e0 + e);
+                                }
+                            }
                         }
-                        list_near<R::VE>(s, between, [&](int e) { return r.index(j, e); });
                         if (!r.ends_group(j)) return;
                         put_entry(s, j, whole(group), 0);
                         above += group;
@@ -1060,23 +1096,32 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
         double sum = 0.0;
         int equal = 0;
         r.each([&](int j, const u32x4& v) {
-            float most = R::value(v, 0);
+            if (all) {
 #pragma unroll
-            for (int e = 1; e < R::VE; ++e) most = fmaxf(most, R::value(v, e));
-            if (all || __any(most >= limit.value)) {
+                for (int e0 = 0; e0 < R::VE; e0 += 4) {
+                    float x[4];
+                    double w[4];
 #pragma unroll
-                for (int e = 0; e < R::VE; ++e) {
-                    const float x = R::value(v, e);
-                    if (all) {
-                        sum += weights.part(x);
-                        continue;
+                    for (int e = 0; e < 4; ++e) x[e] = R::value(v, e0 + e);
+                    weights.parts(x, w);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum += w[e];
+                }
+            } else {
+                float most = R::value(v, 0);
+#pragma unroll
+                for (int e = 1; e < R::VE; ++e) most = fmaxf(most, R::value(v, e));
+                if (__any(most >= limit.value)) {
+#pragma unroll
+                    for (int e = 0; e < R::VE; ++e) {
+                        const float x = R::value(v, e);
+                        const bool above = x > limit.value;
+                        if (__any(above)) {
+                            const double w = weights.part(x);
+                            sum += above ? w : 0.0;
+                        }
+                        equal += __builtin_popcountll(__ballot(x == limit.value));
                     }
-                    const bool above = x > limit.value;
-                    if (__any(above)) {
-                        const double w = weights.part(x);
-                        sum += above ? w : 0.0;
-                    }
-                    equal += __builtin_popcountll(__ballot(x == limit.value));
                 }
             }
             if (!r.ends_group(j)) return;

@@ -208,3 +208,13 @@ def test_min_p_between_zero_and_small_values(gpu, dtype, sign, settings):
     temperature = 1e-6
     min_p = math.exp(-(2.0 ** -18 - sign * 2.0 ** -22) / temperature)
     _check(logits.to(dtype), _sample.numbers(6, 5), temperature=temperature, min_p=min_p, **settings)
+
+
+@pytest.mark.parametrize("min_p", [0.7, 0.1, 0.02, 0.004, 1e-4])
+@pytest.mark.parametrize("top_p", [0.3, 0.8, 0.97, 0.9995])
+@pytest.mark.parametrize("top_k", [0, 250, 9000])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_min_p_beside_top_p(gpu, dtype, top_k, top_p, min_p):
+    """Either of them the narrower one, by much and by little."""
+    _check(_sample.logits(4, 20011, dtype, 91), _sample.numbers(4, 92), top_k=top_k, top_p=top_p, min_p=min_p,
+           temperature=torch.tensor([0.5, 1.0, 1.6, 1e-3]))
