@@ -300,9 +300,8 @@ struct Weights {
     double top, factor, lowest;   // lowest: -60 / factor
     // 2^y of y = (x - top) factor <= 0: the whole part joins the exponent, 2^f with
     // |f| <= 1/2 is 1 + f times a polynomial through 8 points, off by 2^-38.7. What
-    // lies far below gives 2^-60. N of them step by step together: an operation in 64
-    // bits waits for the one before, which four wavefronts a SIMD do not cover (a
-    // pass over 50257 logits: one by one 12 us).
+    // lies far below gives 2^-60. N of them step by step together, as each operation
+    // waits for the one before (a pass over 50257 logits 11.2 us, one by one 12).
     template <int N>
     __device__ __forceinline__ void weights(const float (&x)[N], double (&w)[N]) const {
         constexpr double round = 0x1.8p52;
@@ -650,12 +649,13 @@ struct Places {
 // Bound: the instructions of one compute unit, as a row is a workgroup's: an
 // instruction for every logit is 0.85 us of 128000, and a weight takes about twenty,
 // most of them in 64 bits. One row of 32000 fp16 logits with top_k 50 and top_p:
-// 9.8 us, of which 1.5 read it. fp32 rows of 50257 logits: without limits 16 us, by
-// top_p 32 to 35 (2.5 to read, 4.5 to count, 2.5 for the bracket, 20 for the weights,
-// 3.5 near the limit). bf16 rows by value: 16 of 32000 without limits 15 us, 256 of
-// 128000 by top_p 46 us (65 MB once: 13). Not kept: a row in registers (their
-// spills), several workgroups a row (their launches or a wait for each other cost
-// what they save up to 50257 logits).
+// 9.4 us, of which 1.5 read it. fp32 rows of 50257 logits: without limits 15 us, by
+// top_p 33 to 35 (2.5 to read, 4.5 to count, 2.5 for the bracket, 19 for the weights,
+// 4 near the limit), by a narrower min_p 20. bf16 rows by value: 16 of 32000 without
+// limits 15 us, 256 of 128000 by top_p 47 us (65 MB once: 13). Not kept: a row in
+// registers (their spills), weights eight at a time (the same), several workgroups a
+// row (their launches, or a wait for each other, cost what they save up to 50257
+// logits).
 // ---------------------------------------------------------------------------
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
