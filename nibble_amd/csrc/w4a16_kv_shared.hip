@@ -16,8 +16,10 @@ using w4a16_internal::kv_fail;
 
 constexpr int kMostPrefixShares = 48, kMostOwnShares = 16;
 
-// Rows a workgroup, and the slots' shares: at most `most_shares`, and so many that
-// `workgroups` are launched.
+// Rows a workgroup, and the slots' shares: at most `most_shares`, and so many that up to
+// `workgroups` are launched, as one more on a compute unit than on the others is waited
+// for (42 rows behind each of 3 prefixes of 30001 slots, 8 KV heads of 128: 504 of 512
+// workgroups 52 us, 528 67).
 SidePlan plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t slots, int64_t dim, int most_shares,
                    int64_t workgroups, SidePlan p) {
     p.rows_per = p.prompt ? 32 * p.waves : 16 * p.column_tiles;
@@ -25,11 +27,32 @@ SidePlan plan_side(int64_t batch, int64_t rows, int64_t kv_heads, int64_t slots,
     p.unit = p.prompt ? (dim == 256 ? 32 : 64) : 16 * chunk_tiles((int)dim, p.column_tiles);
     p.threads = 64 * (p.prompt ? p.waves : kDecodeWaves);
     const int64_t groups = batch * kv_heads * p.row_tiles;
-    int64_t splits = groups > 0 ? (workgroups + groups - 1) / groups : 1;
+    int64_t splits = groups > 0 ? workgroups / groups : 1;
+    // two fit a compute unit (4 rows behind each of 17 prefixes of 4000 slots: a share 46
+    // us, three 39)
+    if (splits < 2 && groups <= 256 && p.threads <= 256) splits = groups > 128 ? 512 / groups : 2;
     const int64_t most = shares_of((int)((slots + p.unit - 1) / p.unit), most_shares, p.least).count;
     if (splits > most) splits = most;
     p.splits = splits < 1 ? 1 : (int)splits;
     return p;
+}
+
+// Workgroups of a prefix's prompt form, of which a compute unit holds one, for `groups`
+// of them a share: the number of shares with the shortest rounds over the chip. In tiles,
+// a round takes its share and about 5, a share of 256 workgroups about 8 to write and
+// join (32/8 heads of 128, us with 1 to 5 shares: 1200 tokens behind 8000 246, 273, 207,
+// 244, 223; 800 behind 3000 103, 72, 97, 90, 94; 2500 behind 6000 393, 337, 325, 341, -).
+int64_t prompt_workgroups(int64_t groups, int64_t slots, int64_t dim) {
+    const int64_t tiles = (slots + (dim == 256 ? 31 : 63)) / (dim == 256 ? 32 : 64);
+    int64_t best = 0, shares = 1;
+    for (int64_t s = 1; s <= kMostPrefixShares; ++s) {
+        const int64_t cost = 30 * ((groups * s + 255) / 256) * ((tiles + s - 1) / s + 5) + s * groups;
+        if (s == 1 || cost < best) {
+            best = cost;
+            shares = s;
+        }
+    }
+    return groups * shares;
 }
 
 SharedPlan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int64_t tokens, int64_t heads,
@@ -50,7 +73,10 @@ SharedPlan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int6
         prefix.waves = dim <= 128 ? 8 : 4;
         own.waves = dim <= 128 && batch * kv_heads * ((rows + 255) / 256) >= 512 ? 8 : 4;
         prefix.least = own.least = 8;
-        p.prefix = plan_side(groups, all, kv_heads, prefix_slots, dim, kMostPrefixShares, 256, prefix);
+        p.prefix = plan_side(groups, all, kv_heads, prefix_slots, dim, kMostPrefixShares,
+                             prompt_workgroups(groups * kv_heads * ((all + 32 * prefix.waves - 1) / (32 * prefix.waves)),
+                                               prefix_slots, dim),
+                             prefix);
         p.own = plan_side(batch, rows, kv_heads, slots, dim, kMostOwnShares, 256, own);
         p.last = p.own.splits == 1;
     } else {
