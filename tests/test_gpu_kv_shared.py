@@ -83,6 +83,21 @@ def test_shares_of_long_prefixes(gpu, per, tokens, heads, dim):
     _check(q, prefix, [5001], own, [(b * 523) % 2099 for b in range(per)])
 
 
+@pytest.mark.parametrize("groups,per,tokens", [(1, 3, 40), (2, 1, 90), (1, 20, 17)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("codes,dtype", [("int8", "fp16"), ("fp8", "bf16")])
+def test_prompts_behind_long_prefixes(gpu, codes, dtype, dim, groups, per, tokens):
+    """Several shares of a prefix, joined by the launch over the sequences' own slots or by one of its own."""
+    q, prefix, own = _shared.case(groups, per, tokens, 8, 2, dim, 3001, 1100 if tokens == 40 else 130, codes, dtype)
+    batch = groups * per
+    lengths, start = [2999 - 1700 * g for g in range(groups)], [(37 * b) % (131 - tokens) for b in range(batch)]
+    counts = [max(tokens - 29 * b, 0) for b in range(batch)]
+    _check(q, prefix, lengths, own, start, counts)
+    big = [x * 2.0 ** 16 if i == 1 else x for i, x in enumerate(prefix)]     # attended to row by row
+    got = _check(q, big, lengths, own, start, counts)
+    assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("tokens", [1, 3, 40])
 @pytest.mark.parametrize("codes", ["int8", "fp8"])
 def test_what_lies_behind(gpu, codes, tokens):
