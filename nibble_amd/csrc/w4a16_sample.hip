@@ -168,10 +168,12 @@ struct Row {
     struct __attribute__((packed, aligned(2))) Loose {
         uint32_t w[4];
     };
-    __device__ __forceinline__ int vector(int j) const {
+    __device__ __forceinline__ int vector(int j, int wave) const {   // of another wavefront's lane
         const int group = j & ~3, each = min(4, rounds - group);
-        return (group * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * each + (j & 3)) * 64 +
-               (int)(threadIdx.x & 63);
+        return (group * kWaves + wave * each + (j & 3)) * 64 + (int)(threadIdx.x & 63);
+    }
+    __device__ __forceinline__ int vector(int j) const {
+        return vector(j, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
     }
     // The entry of the sums that a vector belongs to: a wavefront's of a group.
     __device__ __forceinline__ int entry(int index) const {
@@ -179,8 +181,7 @@ struct Row {
         return group * kWaves + (v - group * 4 * kWaves) / each;
     }
     __device__ __forceinline__ bool ends_group(int j) const { return (j & 3) == 3 || j + 1 == rounds; }
-    __device__ __forceinline__ u32x4 read(int j) const {
-        const int v = vector(j);
+    __device__ __forceinline__ u32x4 read(int v) const {
         constexpr uint32_t lowest = TYPE == W4A16_FP32 ? 0xFF800000u : TYPE == W4A16_FP16 ? 0xFC00FC00u : 0xFF80FF80u;
         u32x4 x = {lowest, lowest, lowest, lowest};
         if ((v + 1) * VE <= n) {
@@ -202,7 +203,11 @@ struct Row {
     }
     __device__ __forceinline__ u32x4 fetch(int j) const {
         if (j < kStaged) return staged[j * kThreads + threadIdx.x];
-        return read(min(j, rounds - 1));
+        return read(vector(min(j, rounds - 1)));
+    }
+    __device__ __forceinline__ u32x4 fetch(int j, int wave) const {
+        if (j < kStaged) return staged[j * kThreads + wave * 64 + (threadIdx.x & 63)];
+        return read(vector(j, wave));
     }
     // f(j, vector) for the thread's vectors, every lane taking part
     template <typename F>
@@ -232,7 +237,7 @@ struct Row {
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = read(min(4 * group + i, rounds - 1));
+            for (int i = 0; i < 4; ++i) v[i] = read(vector(min(4 * group + i, rounds - 1)));
         }
     }
     // the same; FIRST: the pass that brings the row in
@@ -1152,45 +1157,55 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
         const double at = (u > 0.0f ? (double)u : 0.0) * (double)total;   // NaN as 0
         return target = at < (double)total ? min((uint64_t)at, total - 1) + 1 : total;
     });
-    if (f.index % kWaves != wave) return;
-    // and there the vector, and the lane
-    uint64_t before = f.before;
-    int64_t ties = tie != 0 ? (int64_t)s.ties[f.index] : 0;
-    const int j0 = f.index / kWaves * 4;
-#pragma unroll 1
-    for (int j = j0; j < min(j0 + 4, r.rounds) && before < target; ++j) {
-        const u32x4 v = r.fetch(j);
-        uint64_t own[R::VE], sum = 0;
-        int64_t at = ties;
-        if (tie != 0) {
-            int equal = 0;
+    // and there the vector, a wavefront each, and the lane: what lies above the limit first
+    const int owner = f.index % kWaves, j = f.index / kWaves * 4 + wave;
+    const bool works = f.index >= 0 && wave < 4 && j < r.rounds;
+    float x[R::VE];
+    uint64_t own[R::VE], sum = 0, upto = 0;
+    int equal = 0, equal_upto = 0;
+    if (works) {
+        const u32x4 v = r.fetch(j, owner);
 #pragma unroll
-            for (int e = 0; e < R::VE; ++e) equal += R::value(v, e) == limit.value ? 1 : 0;
-            const uint64_t upto = wave_scan((uint64_t)equal);
-            at += (int64_t)upto - equal;
-            ties += (int64_t)lane_of(upto, 63);
-        }
+        for (int e = 0; e < R::VE; ++e) x[e] = R::value(v, e);
 #pragma unroll
-        for (int e = 0; e < R::VE; ++e) {
-            const float x = R::value(v, e);
-            own[e] = 0;
-            if (x > limit.value) own[e] = weights.of(x);
-            if (x == limit.value && tie != 0) own[e] = at++ < limit.ties ? tie : 0;
-            sum += own[e];
-        }
-        const uint64_t upto = before + wave_scan(sum);
-        uint64_t below = upto - sum;
-        if (below < target && upto >= target) {
-            int e = 0;
+        for (int e0 = 0; e0 < R::VE; e0 += 4) {
+            const float y[4] = {x[e0], x[e0 + 1], x[e0 + 2], x[e0 + 3]};
+            double w[4];
+            weights.weights(y, w);
 #pragma unroll
-            for (int i = 0; i < R::VE; ++i) {
-                below += own[i];
-                if (below < target) e = i + 1;
+            for (int e = 0; e < 4; ++e) {
+                own[e0 + e] = y[e] > limit.value ? Weights::rounded(w[e]) : 0;
+                sum += own[e0 + e];
+                equal += tie != 0 && y[e] == limit.value ? 1 : 0;
             }
-            a.tokens[row] = r.index(j, e);
         }
-        before = lane_of(upto, 63);
+        upto = wave_scan(sum);
+        if (tie != 0) equal_upto = (int)wave_scan((uint64_t)equal);
+        if (lane == 63) {
+            s.sums[wave] = upto;
+            s.firsts[wave] = equal_upto;
+        }
     }
+    __syncthreads();
+    if (!works) return;
+    uint64_t before = f.before;
+    int64_t left = tie != 0 ? limit.ties - (int64_t)s.ties[f.index] : 0;   // ties that are kept from here on
+    auto kept_of = [&](int n) { return tie * (uint64_t)min(max(left, (int64_t)0), (int64_t)n); };
+    for (int w = 0; w < wave; ++w) {
+        before += s.sums[w] + kept_of(s.firsts[w]);
+        left -= s.firsts[w];
+    }
+    uint64_t below = before + upto - sum + kept_of(equal_upto - equal);
+    if (below >= target || before + upto + kept_of(equal_upto) < target) return;
+    left -= equal_upto - equal;
+    int e = 0;
+#pragma unroll
+    for (int i = 0; i < R::VE; ++i) {
+        if (tie != 0 && x[i] == limit.value && left-- > 0) own[i] = tie;
+        below += own[i];
+        if (below < target) e = i + 1;
+    }
+    a.tokens[row] = r.vector(j, owner) * R::VE + e;
 }
 
 }  // namespace w4a16
