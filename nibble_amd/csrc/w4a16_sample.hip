@@ -33,7 +33,7 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kMostEntries = 512;    // sums of places: 2^19 fp32 logits
 constexpr int kList = 256;           // candidates that are compared with each other
-constexpr int kMostNear = 4096;      // logits near a limit that are listed
+constexpr int kMostNear = 4096;      // logits near a limit that are listed, with places that stay empty
 constexpr int kStaged = 4;           // vectors of a thread that stay in LDS: a group, 64 KB
 constexpr int kTiny = 64;            // bf16 logits between 0 and 2^-20 that are listed
 constexpr int kValues = 7168;        // bf16 values that a row's weights may take
@@ -476,27 +476,43 @@ __device__ __forceinline__ bool select(Shared& s, Keys keys, uint64_t target, fl
     return true;
 }
 
-// Appends indices to s.near, N a lane at most; past kMostNear they are only counted.
-template <int N, typename Index>
-__device__ __forceinline__ void list_near(Shared& s, const bool (&has)[N], Index index) {
-    bool any = false;
+// Appends indices to s.near, N a lane at most: a wavefront takes 64 places at a time (a
+// count that all share for each vector is waited for: 600 of 50257 logits in 10.5 us, this
+// way in 8). Past kMostNear they are only counted.
+struct Near {
+    int base = 0, room = 0;   // the wavefront's next place, and how many it has
+    template <int N, typename Index>
+    __device__ __forceinline__ void list(Shared& s, const bool (&has)[N], Index index) {
+        bool any = false;
 #pragma unroll
-    for (int e = 0; e < N; ++e) any |= has[e];
-    if (!__any(any)) return;
-    int total = 0;
+        for (int e = 0; e < N; ++e) any |= has[e];
+        if (!__any(any)) return;
+        int total = 0;
 #pragma unroll
-    for (int e = 0; e < N; ++e) total += __builtin_popcountll(__ballot(has[e]));
-    int at = 0;
-    if ((threadIdx.x & 63) == 0) at = atomicAdd(&s.listed, total);
-    at = __builtin_amdgcn_readfirstlane(at);
+        for (int e = 0; e < N; ++e) total += __builtin_popcountll(__ballot(has[e]));
+        if (total > room) {
+            finish(s);
+            room = max(total, 64);
+            int at = 0;
+            if ((threadIdx.x & 63) == 0) at = atomicAdd(&s.listed, room);
+            base = __builtin_amdgcn_readfirstlane(at);
+        }
+        room -= total;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        const uint64_t who = __ballot(has[e]);
-        const int own = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-        if (has[e] && own < kMostNear) s.near[own] = index(e);
-        at += __builtin_popcountll(who);
+        for (int e = 0; e < N; ++e) {
+            const uint64_t who = __ballot(has[e]);
+            const int own =
+                base + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+            if (has[e] && own < kMostNear) s.near[own] = index(e);
+            base += __builtin_popcountll(who);
+        }
     }
-}
+    // places that stay empty, fewer than 64
+    __device__ __forceinline__ void finish(Shared& s) const {
+        const int lane = threadIdx.x & 63;
+        if (lane < room && base + lane < kMostNear) s.near[base + lane] = -1;
+    }
+};
 
 // The sum and the ties of a wavefront's group that ends with vector j.
 __device__ __forceinline__ void put_entry(Shared& s, int j, uint64_t sum, int equal) {
@@ -512,8 +528,8 @@ template <typename R>
 __device__ __forceinline__ void load_near(const Shared& s, const R& r, float (&x)[kMostNear / kThreads]) {
 #pragma unroll
     for (int i = 0; i < kMostNear / kThreads; ++i) {
-        const int at = (int)threadIdx.x + i * kThreads;
-        x[i] = at < s.listed ? r.at(s.near[at]) : -__builtin_inff();
+        const int at = (int)threadIdx.x + i * kThreads, index = at < s.listed ? s.near[at] : -1;
+        x[i] = index >= 0 ? r.at(index) : -__builtin_inff();
     }
 }
 
@@ -903,24 +919,27 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                     in_last = (uint64_t)top_k - f.before;
                     uint64_t rest = 0;
                     // few kept tokens are listed all, else those of the last bin
-                    const int from = top_k <= kMostNear * 7 / 8 ? 0 : last_bin;
+                    const int from = top_k <= kMostNear * 5 / 8 ? 0 : last_bin;
                     if (tid == 0) s.listed = 0;
                     __syncthreads();
-                    r.each([&](int j, const u32x4& v) {
+                    // (wider than the bins by a little)
+                    const Keys bounds = keys_of<R>(bins, from, last_bin);
+                    const float high = from > 0 ? R::of_key(bounds.high) : __builtin_inff();
+                    const float low = fmaxf(R::of_key(bounds.low), -3.4028234663852886e38f);
+                    Near listed;
+                    r.each4([&](int j, const u32x4& v) {
                         bool in[R::VE];
 #pragma unroll
-                        for (int e = 0; e < R::VE; ++e) {
-                            const int bin = bins.of(R::value(v, e));
-                            in[e] = bin >= from && bin <= last_bin;
-                        }
-                        list_near<R::VE>(s, in, [&](int e) { return r.index(j, e); });
+                        for (int e = 0; e < R::VE; ++e) in[e] = R::value(v, e) <= high && R::value(v, e) >= low;
+                        listed.list<R::VE>(s, in, [&](int e) { return r.index(j, e); });
                     });
+                    listed.finish(s);
                     __syncthreads();
                     const Keys keys = keys_of<R>(bins, last_bin, last_bin);
                     auto one = [](float) { return (uint64_t)1; };
-                    const int near = s.listed;
+                    const bool near = s.listed <= kMostNear;   // all are listed
                     float x[kMostNear / kThreads];
-                    if (near <= kMostNear) {
+                    if (near) {
                         load_near(s, r, x);
                         select<R>(s, keys, in_last, 0.0f, 0, [&](auto f) {
 #pragma unroll
@@ -937,7 +956,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                         }, one, limit.value, rest);
                     }
                     limit.ties = (int64_t)rest;
-                    if (from == 0 && near <= kMostNear) {   // all that follows is about the listed ones
+                    if (from == 0 && near) {   // all that follows is about the listed ones
                         limited = summed = true;
                         auto above = [&](auto f) {
 #pragma unroll
@@ -1019,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                                 w[e] = counts ? w[e] : 0.0;
                                 all += w[e];
                                 group += x[e] > high ? w[e] : 0.0;
-                                if (counts && x[e] <= high && x[e] >= low) {   // few
+                                if (counts && x[e] <= high && x[e] >= low) {   // few: one by one
                                     const int i = atomicAdd(&s.listed, 1);
                                     if (i < kMostNear) s.near[i] = r.index(j, e0 + e);
                                 }
@@ -1033,7 +1052,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                     uint64_t total = whole(all), sure = whole(above);
                     block_sums(s, total, sure);
                     total += beside;
-                    const int near = s.listed;
+                    const bool near = s.listed <= kMostNear;   // all are listed
                     const uint64_t target = needed_of(total);
                     uint64_t rest = 0;
                     float value = by_count.value;
@@ -1041,7 +1060,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                     auto amount = [&](float x) { return weights.of(x); };
                     float x[kMostNear / kThreads];
                     bool found = target > sure;
-                    if (near <= kMostNear) {
+                    if (near) {
                         load_near(s, r, x);
                         if (found)
                             found = select<R>(s, keys, target - sure, by_count.value, tied, [&](auto f) {
@@ -1069,7 +1088,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
                     const uint64_t w = max(weights.of(value), (uint64_t)1);
                     limit = {value, (int64_t)((rest + w - 1) / w)};
                     // of a value that ties at top_k none is listed
-                    if (near <= kMostNear && value != by_count.value && least <= value) {
+                    if (near && value != by_count.value && least <= value) {
                         summed = true;
                         __syncthreads();
 #pragma unroll

@@ -218,3 +218,13 @@ def test_min_p_beside_top_p(gpu, dtype, top_k, top_p, min_p):
     """Either of them the narrower one, by much and by little."""
     _check(_sample.logits(4, 20011, dtype, 91), _sample.numbers(4, 92), top_k=top_k, top_p=top_p, min_p=min_p,
            temperature=torch.tensor([0.5, 1.0, 1.6, 1e-3]))
+
+
+@pytest.mark.parametrize("falling", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sorted_rows(gpu, dtype, falling):
+    """Likely tokens side by side, as where vocabularies are in the order of frequency."""
+    logits = _sample.logits(6, 50257, dtype, 61).float().sort(dim=1, descending=falling).values.to(dtype)
+    for settings in ({}, {"top_k": 600, "top_p": 0.9}, {"top_k": 2500}, {"top_k": 2600}, {"top_k": 30000, "top_p": 0.99},
+                     {"top_p": 0.7}, {"top_p": 0.99}, {"top_p": 0.9999}, {"min_p": 0.001}):
+        _check(logits, _sample.numbers(6, 62), **settings)
