@@ -670,13 +670,13 @@ struct Places {
 // Bound: the instructions of one compute unit, as a row is a workgroup's: an
 // instruction for every logit is 0.85 us of 128000, and a weight takes about twenty,
 // most of them in 64 bits. One row of 32000 fp16 logits with top_k 50 and top_p:
-// 9.2 us, of which 1.5 read it. fp32 rows of 50257 logits: without limits 15 us, by
-// top_p 33 to 35 (2.5 to read, 4.5 to count, 2.5 for the bracket, 19 for the weights,
-// 4 near the limit), by a narrower min_p 20. bf16 rows by value: 16 of 32000 without
-// limits 15 us, 256 of 128000 by top_p 46 us (65 MB once: 13). Not kept: a row in
-// registers (their spills), weights eight at a time (the same), several workgroups a
-// row (their launches, or a wait for each other, cost what they save up to 50257
-// logits).
+// 9.3 us, of which 1.5 read it. fp32 rows of 50257 logits: without limits 18 us, by
+// top_p 37 (2.5 to read, 4.5 to count, 2.5 for the bracket, 19 for the weights, 4 near
+// the limit, 3 for the token), by a top_k of 600 31, by a narrower min_p 14 to 21. bf16
+// rows by value: 16 of 32000 without limits 12.5 us, 256 of 128000 by top_p 43 us (65
+// MB once: 13). Not kept: a row in registers (their spills), weights eight at a time
+// (the same), several workgroups a row (their launches, or a wait for each other, cost
+// what they save up to 50257 logits).
 // ---------------------------------------------------------------------------
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
