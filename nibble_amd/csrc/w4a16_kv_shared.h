@@ -25,13 +25,13 @@ namespace w4a16 {
 // the shares that were written.
 //
 // Bound: latency, of the lengths' chain of loads and one round of shares (2048 rows
-// of 11 shares of 128 dims, 11.5 MB: 6.0 us; 512 rows of 13 of 64 dims 4.3).
+// of 11 shares of 128 dims, 11.5 MB: 5.7 us; 512 rows of 13 of 64 dims 4.3).
 // ---------------------------------------------------------------------------
 template <int D, int TYPE, int W>
 __global__ void __launch_bounds__(256) join_kernel(const AttnArgs prefix, const AttnArgs own, int prefix_unit,
                                                    int own_unit, int own_rows, int64_t rows) {
     constexpr int E = D / 64;   // dims a lane
-    constexpr int F = W == 1 ? 8 : 4;   // shares of a wavefront in flight
+    constexpr int F = W == 1 ? 12 : 4;   // shares of a wavefront in flight
     __shared__ float parts[W][D];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W, lane = threadIdx.x & 63;
     const int64_t row = blockIdx.x * (int64_t)(4 / W) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
@@ -156,8 +156,8 @@ void launch_beside(const SharedCall& c) {   // own slots in the decode form
         const dim3 grid((unsigned)(c.prefix_grid + c.own_grid)), threads(64 * kDecodeWaves);
         hipLaunchKernelGGL((prompt_kernel<D, 4, 1, CODES, TYPE, Prefix, NTO, OwnArgs>), grid, threads, 0, c.stream,
                            c.prefix, (OwnArgs{c.own, (int)c.prefix_grid}));
-    } else if (p.column_tiles >= 3) {
-        if constexpr (D <= 128) launch_pair<D, D == 64 ? 4 : 3, NTO, CODES, TYPE>(c);
+    } else if (p.column_tiles == 3) {
+        if constexpr (D == 128) launch_pair<D, 3, NTO, CODES, TYPE>(c);
     } else if (p.column_tiles == 2) {
         launch_pair<D, 2, NTO, CODES, TYPE>(c);
     } else {

@@ -80,23 +80,29 @@ SharedPlan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int6
         p.own = plan_side(batch, rows, kv_heads, slots, dim, kMostOwnShares, 256, own);
         p.last = p.own.splits == 1;
     } else {
-        // One launch for both, and one that joins. The prefix in the decode form up
-        // to 64 rows, 128 over short prefixes (128 rows of 128 dims over 3000 slots: 19
-        // us, in the prompt form 23; over 8192 slots the other way round): of 48 rows a
-        // workgroup where these are the fewest (42 rows over 4 x 30001 slots: 41 us, of
-        // 32 rows 47), two of them a compute unit from 17 rows on over long prefixes
-        // (32 rows over 100000 slots: 52 us, one 54; 16 rows 53, one 47). In the prompt
-        // form, which has the matrix cores to do, fewer workgroups where the sequences'
-        // own slots, which have the memory, take as long (64 sequences of up to 1024
-        // slots behind 8192: 160 workgroups 37 us, 256 of them 44; of up to 64 behind
-        // 32768: 63, and 128 of them 95).
-        prefix.prompt = all > (dim == 128 && prefix_slots <= 4096 ? 128 : 64);
-        prefix.column_tiles = all <= 16 ? 1 : all <= 32 || dim == 256 ? 2 : dim == 64 ? 4 : all <= 48 ? 3 : 2;
+        // One launch for both, and one that joins. The prefix in the decode form up to 64
+        // rows; of 128 dims up to 128 over short prefixes (128 rows over 6000 slots: 22 us,
+        // in the prompt form 27; over 8192 slots the other way round); of 64 dims, whose
+        // codes are fewer to decode, until the products are many (128 rows over 1500 slots:
+        // 10.3 us, in the prompt form 11.8; 256 over 6000: 16.5 and 21; 192 over 50000: 45
+        // and 39). 32 rows a workgroup (64 of 64 dims over 8000 slots: 11.7 us, 64 rows a
+        // workgroup 14.8), 48 where these are all (42 of 128 dims over 4 x 30001: 41 us, of
+        // 32 rows 47). One workgroup a compute unit, two for 17 to 48 rows of 128 dims over
+        // long prefixes (32 rows over 100000 slots: 52 us, one 54; 16 rows 53, one 47). In
+        // the prompt form, which has the matrix cores to do, fewer workgroups where the
+        // sequences' own slots, which have the memory, take as long (64 sequences of up to
+        // 1024 slots behind 8192: 160 workgroups 37 us, 256 of them 44; of up to 64 behind
+        // 32768: 63, and 128 of them 95; 256 sequences of 8 rows, of up to 256 slots behind
+        // 8000: 81, and 256 of them 52).
+        prefix.prompt = dim == 64 ? all > 64 && (__int128)all * prefix_slots > (6 << 20)
+                                  : all > (dim == 128 && prefix_slots <= 6144 ? 128 : 64);
+        prefix.column_tiles = all <= 16 ? 1 : all > 32 && all <= 48 && dim == 128 ? 3 : 2;
         if (prefix.column_tiles < own.column_tiles) prefix.column_tiles = own.column_tiles;
         prefix.least = prefix.prompt ? 2 : 4;
         own.least = 4;
-        const int64_t workgroups = prefix.prompt ? (batch / groups * slots >= 4 * prefix_slots ? 160 : 256)
-                                   : prefix.column_tiles >= 2 && all <= 48 && dim <= 128 && prefix_slots >= 8192 ? 512 : 256;
+        const bool beside = batch / groups * slots >= 4 * prefix_slots && rows * prefix_slots < 64 * slots;
+        const int64_t workgroups = prefix.prompt ? (beside ? 160 : 256)
+                                   : prefix.column_tiles >= 2 && all <= 48 && dim == 128 && prefix_slots >= 8192 ? 512 : 256;
         p.prefix = plan_side(groups, all, kv_heads, prefix_slots, dim, kMostPrefixShares, workgroups, prefix);
         p.own = plan_side(batch, rows, kv_heads, slots, dim, kMostOwnShares, 256, own);
     }

@@ -83,6 +83,16 @@ def test_shares_of_long_prefixes(gpu, per, tokens, heads, dim):
     _check(q, prefix, [5001], own, [(b * 523) % 2099 for b in range(per)])
 
 
+@pytest.mark.parametrize("length", [0, 1, 700, 5000])
+@pytest.mark.parametrize("codes,dtype", [("int8", "fp16"), ("fp8", "bf16")])
+def test_many_rows_in_a_large_cache(gpu, codes, dtype, length):
+    """Tokens of many sequences behind a prefix cache of many slots, however few are held; padding among them."""
+    q, prefix, own = _shared.case(1, 20, 1, 16, 2, 64, 42000, 60, codes, dtype)
+    _check(q, prefix, [length], own, [(7 * b) % 60 for b in range(20)], [b % 3 for b in range(20)])
+    big = [x * 2.0 ** 16 if i == 1 else x for i, x in enumerate(prefix)]
+    _check(q, big, [length], own, [(7 * b) % 60 for b in range(20)])
+
+
 @pytest.mark.parametrize("groups,per,tokens", [(1, 3, 40), (2, 1, 90), (1, 20, 17)])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("codes,dtype", [("int8", "fp16"), ("fp8", "bf16")])
