@@ -86,10 +86,9 @@ NATIVE_PREFILL_MAX_ROWS = 256
 FUSED_PREFILL_NATIVE_MAX_ROWS = 1024
 # Most bytes of a layer's cache that `sample` fills with copies of the prompt, one
 # for each sequence; longer prompts are attended to once for all of them. Measured
-# on steps of the 1.1B model (graph, sequences x prompt): 16 x 1024 tokens 955 us
-# with copies, 1010 without; 16 x 3000 (25 MB) 1042 and 1046, 32 x 3000 1413 and
-# 1399.
-FORK_BYTES_MAX = 24 << 20
+# on steps of the 1.1B model (graph, sequences x prompt): 16 x 1024 tokens (8 MB) 957
+# us with copies, 977 without; 16 x 2000 (16 MB) 1005 and 977, 32 x 1024 1287 and 1275.
+FORK_BYTES_MAX = 12 << 20
 # Steps of `sample` between two looks at which sequences have ended.
 EOS_STRIDE = 16
 # Sequences times head_dim that `QuantizedKVCache.reorder` takes.
