@@ -174,7 +174,8 @@ int w4a16_kv_fork(const w4a16_kv_cache* from, const w4a16_kv_cache* to, const in
 /*
  * The same within one cache: every sequence b becomes what sequence source[b]
  * held before the call (beams that live on, finished sequences whose place
- * another takes). lengths [batch] are those before the call. At most 262144 /
+ * another takes). lengths [batch] are the slots that the sequences hold when it is
+ * called, those that the step before has written among them. At most 262144 /
  * head_dim sequences.
  */
 int w4a16_kv_reorder(const w4a16_kv_cache* cache, const int64_t* source, const int64_t* lengths, void* stream);

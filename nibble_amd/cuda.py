@@ -306,8 +306,8 @@ def kv_reorder_cuda(
 ) -> None:
     """The sequences of an 8-bit cache in another order, in place: every
     sequence b becomes what sequence source[b] held before, its first
-    lengths[source[b]] slots (int64 [batch]); one whose source is outside the
-    batch stays as it is."""
+    lengths[source[b]] slots (int64 [batch], the newest tokens' slots among
+    them); one whose source is outside the batch stays as it is."""
     _require_extension()
     torch.ops.w4a16.kv_reorder.default(k_codes, k_scales, v_codes, v_scales, source, lengths)
 

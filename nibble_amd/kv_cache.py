@@ -132,13 +132,16 @@ class QuantizedKVCache:
     def fork_from(self, other: QuantizedKVCache, source: torch.Tensor, lengths: torch.Tensor) -> None:
         """Every sequence b becomes what sequence source[b] of another cache
         holds, lengths[source[b]] slots of it (int64 tensors of this and of the
-        other cache's batch); a source outside the other leaves b as it is."""
+        other cache's batch), those written by the step before included; a
+        source outside the other leaves b as it is."""
         call = kv_fork_cuda if self.k_codes.is_cuda else kv_reference.kv_fork_reference
         call(*other.tensors(), *self.tensors(), source, lengths)
 
     def reorder(self, source: torch.Tensor, lengths: torch.Tensor) -> None:
         """Every sequence b becomes what sequence source[b] held before, its
-        first lengths[source[b]] slots (int64 [batch] both)."""
+        first lengths[source[b]] slots (int64 [batch] both). A step that wrote
+        its tokens at the slots ``start`` holds start + tokens: with `start`
+        alone the newest tokens stay where they are."""
         call = kv_reorder_cuda if self.k_codes.is_cuda else kv_reference.kv_reorder_reference
         call(*self.tensors(), source, lengths)
 
