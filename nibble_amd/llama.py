@@ -727,27 +727,32 @@ class LlamaDecoder(torch.nn.Module):
                 left -= 1
         return torch.cat(out)
 
-    def _check_sampling(self, prompt, new_tokens, sequences, random) -> None:
+    def _check_sampling(self, prompt, new_tokens, sequences, random, settings) -> None:
         if sequences < 1 or new_tokens < 1:
             raise ValueError("sequences and new_tokens must be greater than zero")
         if sequences > 1 and self.kv_caches is None:
             raise ValueError("several sequences need an 8-bit kv_cache")
         if random is not None and random.shape != (sequences, new_tokens):
             raise ValueError("random must have shape [sequences, new_tokens]")
+        for name, value in settings.items():
+            if isinstance(value, torch.Tensor) and value.shape != (sequences,):
+                raise ValueError(f"{name} must be a number or have shape [sequences]")
         slots = prompt.numel() + new_tokens - 1
         if slots > self.cfg.max_seq_len:
             raise IndexError(f"prompt and new tokens are longer than the key/value cache ({slots} slots of "
                              f"{self.cfg.max_seq_len})")
 
     @torch.inference_mode()
-    def sample(self, prompt: torch.Tensor, new_tokens: int, sequences: int = 1, temperature: float = 1.0,
-               top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, random: torch.Tensor | None = None,
-               generator: torch.Generator | None = None, eos: int | None = None,
+    def sample(self, prompt: torch.Tensor, new_tokens: int, sequences: int = 1,
+               temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0,
+               top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
+               random: torch.Tensor | None = None, generator: torch.Generator | None = None, eos: int | None = None,
                use_graph: bool = True) -> torch.Tensor:
         """Tokens drawn after the prompt (int64 [T]): int64 [sequences,
         new_tokens], each by one of the uniform numbers ``random`` (float32
         [sequences, new_tokens]; drawn with ``generator`` if None) and the
-        settings of ``nibble_amd.sample``.
+        settings of ``nibble_amd.sample``, each a number or a tensor of one
+        value a sequence.
 
         One sequence runs the decode step of ``generate`` (its captured graph
         with use_graph, if ``capture`` recorded one) and continues in the
@@ -760,10 +765,10 @@ class LlamaDecoder(torch.nn.Module):
         With ``eos`` a sequence that has drawn it is filled up with it. When half
         of the running ones have ended, the others move up and the step goes on
         with them alone (looked at every EOS_STRIDE tokens)."""
-        self._check_sampling(prompt, new_tokens, sequences, random)
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        self._check_sampling(prompt, new_tokens, sequences, random, settings)
         if random is None:
             random = torch.rand((sequences, new_tokens), device=self.token.device, generator=generator)
-        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         self.prefill(prompt)
         if sequences == 1:
             out = self._sample_one(random[0], settings, eos, use_graph).unsqueeze(0)
@@ -814,12 +819,12 @@ class LlamaDecoder(torch.nn.Module):
         first = 0 if fork else length       # the row of the rotary tables of the caches' first slot
         cos, sin = self.cos[first:], self.sin[first:]
         state = {"token": whole(0, n), "random": torch.empty((n,), dtype=torch.float32, device=device),
-                 "held": whole(length if fork else 0, n), "caches": caches}
+                 "held": whole(length if fork else 0, n), "caches": caches, "settings": settings}
 
         def step():
             logits = self._rows_forward(state["token"], state["caches"], state["held"], cos, sin,
                                         None if fork else lengths)
-            state["token"].copy_(sample(logits, state["random"], **settings))
+            state["token"].copy_(sample(logits, state["random"], **state["settings"]))
             state["held"].add_(1)
 
         out = torch.full((n, steps), 0 if eos is None else eos, dtype=torch.int64, device=device)
@@ -841,7 +846,9 @@ class LlamaDecoder(torch.nn.Module):
                         cache.reorder(source, state["held"])
                     rows = rows[keep]
                     state = {"token": state["token"][keep], "random": state["random"][:live].clone(),
-                             "held": state["held"][keep], "caches": [c.first(live) for c in state["caches"]]}
+                             "held": state["held"][keep], "caches": [c.first(live) for c in state["caches"]],
+                             "settings": {name: value[keep] if isinstance(value, torch.Tensor) else value
+                                          for name, value in state["settings"].items()}}
                     graph = None
             state["random"].copy_(random[rows, i])
             if graph is not None:
