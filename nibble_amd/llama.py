@@ -91,6 +91,13 @@ FUSED_PREFILL_NATIVE_MAX_ROWS = 1024
 FORK_BYTES_MAX = 12 << 20
 # Steps of `sample` between two looks at which sequences have ended.
 EOS_STRIDE = 16
+# Replays for which `sample` records its step in a graph. Recording takes 2.3 to 3 ms of
+# the 1.1B model; a step of up to 16 sequences takes 1.45 ms from the host and 0.78 to
+# 0.89 replayed (whole calls, ms: 16 sequences of 6 tokens, four replays, 10.2 recorded
+# and 9.7 not, of 8 tokens 11.8 and 12.4; 4 of 6 tokens 9.4 and 9.6). Where the step
+# itself takes as long as its launches, recording is not won back soon (64 sequences of
+# 16 tokens 27.8 and 25.8, of 64 tokens 100.7 and 101.1).
+GRAPH_REPLAYS_MIN = 6
 # Sequences times head_dim that `QuantizedKVCache.reorder` takes.
 REORDER_VALUES_MAX = 262144
 
@@ -758,9 +765,11 @@ class LlamaDecoder(torch.nn.Module):
         with use_graph, if ``capture`` recorded one) and continues in the
         decoder's own state. Several need an 8-bit cache. The prompt is run once;
         its keys and values are copied into each sequence's cache up to
-        FORK_BYTES_MAX in all and attended to by all sequences together from
-        there on; the decoder's own state stays at the end of the prompt. Their
-        step is recorded in a HIP graph with use_graph.
+        FORK_BYTES_MAX of a layer for all sequences, and attended to by all of
+        them together from there on; the decoder's own state stays at the end
+        of the prompt. With use_graph their step is recorded in a HIP graph,
+        and again when sequences have left, for GRAPH_REPLAYS_MIN replays or
+        more.
 
         With ``eos`` a sequence that has drawn it is filled up with it. When half
         of the running ones have ended, the others move up and the step goes on
@@ -855,7 +864,7 @@ class LlamaDecoder(torch.nn.Module):
                 graph.replay()
             else:
                 step()
-                if use_graph and self.fused and steps - i > 4:   # the steps from the next one on
+                if use_graph and self.fused and steps - 1 - i >= GRAPH_REPLAYS_MIN:   # the steps from the next one on
                     graph = torch.cuda.CUDAGraph()
                     with torch.cuda.graph(graph):
                         step()
