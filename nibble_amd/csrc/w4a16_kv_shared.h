@@ -129,6 +129,10 @@ struct SidePlan {
     int threads;
 };
 
+// Wavefronts of the prompt form on a prefix alone, and on own slots where these give many
+// workgroups (which then have one share, so that Last is their mode).
+constexpr int wide_waves(int dim) { return dim <= 128 ? 8 : 4; }
+
 struct SharedPlan {
     SidePlan prefix, own;
     bool last;          // the own slots' launch joins the prefix's shares, else a launch of its own does
@@ -165,13 +169,9 @@ void launch_beside(const SharedCall& c) {   // own slots in the decode form
     }
 }
 
-template <int D, int CODES, int TYPE, Mode MODE>
-void launch_prompt(const SidePlan& p, const AttnArgs& a, int64_t grid, hipStream_t st) {
-    const dim3 g((unsigned)grid), threads((unsigned)p.threads);
-    if (p.waves == 4)
-        hipLaunchKernelGGL((prompt_kernel<D, 4, 1, CODES, TYPE, MODE>), g, threads, 0, st, a);
-    else if constexpr (D <= 128)
-        hipLaunchKernelGGL((prompt_kernel<D, 8, 1, CODES, TYPE, MODE>), g, threads, 0, st, a);
+template <int D, int W, int CODES, int TYPE, Mode MODE>
+void launch_prompt(const AttnArgs& a, int64_t grid, hipStream_t st) {
+    hipLaunchKernelGGL((prompt_kernel<D, W, 1, CODES, TYPE, MODE>), dim3((unsigned)grid), dim3(64 * W), 0, st, a);
 }
 
 template <int D, int CODES, int TYPE>
@@ -182,12 +182,16 @@ void launch_codes(const SharedCall& c) {
         else
             launch_beside<D, 2, CODES, TYPE>(c);
     } else {
-        launch_prompt<D, CODES, TYPE, Prefix>(c.plan.prefix, c.prefix, c.prefix_grid, c.stream);
+        constexpr int WIDE = wide_waves(D);
+        launch_prompt<D, WIDE, CODES, TYPE, Prefix>(c.prefix, c.prefix_grid, c.stream);
         if (c.plan.last) {
-            launch_prompt<D, CODES, TYPE, Last>(c.plan.own, c.own, c.own_grid, c.stream);
+            if (c.plan.own.waves == WIDE)
+                launch_prompt<D, WIDE, CODES, TYPE, Last>(c.own, c.own_grid, c.stream);
+            else
+                launch_prompt<D, 4, CODES, TYPE, Last>(c.own, c.own_grid, c.stream);
             return;
         }
-        launch_prompt<D, CODES, TYPE, Own>(c.plan.own, c.own, c.own_grid, c.stream);
+        launch_prompt<D, 4, CODES, TYPE, Own>(c.own, c.own_grid, c.stream);
     }
     const dim3 threads(256);
     // a wavefront a row where there are many rows of few shares (2048 rows of 11: 37

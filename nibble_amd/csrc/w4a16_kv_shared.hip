@@ -70,14 +70,15 @@ SharedPlan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int6
         // tokens, 32/8 heads of 128, behind 6000: 196 us, of 128 rows 218), of a
         // sequence's own rows as attention over one cache has them (202 with 256).
         prefix.prompt = true;
-        prefix.waves = dim <= 128 ? 8 : 4;
-        own.waves = dim <= 128 && batch * kv_heads * ((rows + 255) / 256) >= 512 ? 8 : 4;
+        prefix.waves = wide_waves((int)dim);
+        const bool many = batch * kv_heads * ((rows + 255) / 256) >= 512;
+        own.waves = many ? prefix.waves : 4;
         prefix.least = own.least = 8;
         p.prefix = plan_side(groups, all, kv_heads, prefix_slots, dim, kMostPrefixShares,
                              prompt_workgroups(groups * kv_heads * ((all + 32 * prefix.waves - 1) / (32 * prefix.waves)),
                                                prefix_slots, dim),
                              prefix);
-        p.own = plan_side(batch, rows, kv_heads, slots, dim, kMostOwnShares, 256, own);
+        p.own = plan_side(batch, rows, kv_heads, slots, dim, many ? 1 : kMostOwnShares, 256, own);
         p.last = p.own.splits == 1;
     } else {
         // One launch for both, and one that joins. The prefix in the decode form up to 64
