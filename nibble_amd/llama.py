@@ -88,6 +88,10 @@ FUSED_PREFILL_NATIVE_MAX_ROWS = 1024
 # for each sequence; longer prompts are attended to once for all of them. Measured
 # on steps of the 1.1B model (graph, sequences x prompt): 16 x 1024 tokens (8 MB) 957
 # us with copies, 977 without; 16 x 2000 (16 MB) 1005 and 977, 32 x 1024 1287 and 1275.
+# The attention alone, 32/8 heads of 128: 4 x 1024 (8 MB) 11.1 us with copies, 11.7
+# without, 4 x 2048 14.2 and 11.7, 16 x 256 8.2 and 13.7, 16 x 1024 (32 MB) 16.2 and 13.4.
+# Copies would serve many sequences longer (64 x 256 of 32 MB 12.8 and 18.4, of 64 MB 18.6
+# and 17.8), but take that memory in every layer.
 FORK_BYTES_MAX = 12 << 20
 # Steps of `sample` between two looks at which sequences have ended.
 EOS_STRIDE = 16
@@ -98,6 +102,15 @@ EOS_STRIDE = 16
 # itself takes as long as its launches, recording is not won back soon (64 sequences of
 # 16 tokens 27.8 and 25.8, of 64 tokens 100.7 and 101.1).
 GRAPH_REPLAYS_MIN = 6
+# Up to MOVED_ROWS sequences a step takes about as long however many there are, but for
+# the keys and values that it reads. Where the step is fused, running sequences move up
+# from more than that, or where those that have ended would have MOVED_BYTES read until
+# the end: recording the step anew takes 3 ms, in which about so much is read. (Without a
+# graph the same, so that both draw the same tokens.) The 1.1B model, sequences that end
+# evenly over the tokens, ms without moves, with all, by this rule: 16 of 64 tokens 61.4,
+# 66.6, 61.6; 16 of 1500 1393, 1322, 1332; 32 of 256 303, 277, 271; 64 of 256 390, 353, 349.
+MOVED_ROWS = 16
+MOVED_BYTES = 12 << 30
 # Sequences times head_dim that `QuantizedKVCache.reorder` takes.
 REORDER_VALUES_MAX = 262144
 
@@ -773,7 +786,8 @@ class LlamaDecoder(torch.nn.Module):
 
         With ``eos`` a sequence that has drawn it is filled up with it. When half
         of the running ones have ended, the others move up and the step goes on
-        with them alone (looked at every EOS_STRIDE tokens)."""
+        with them alone (looked at every EOS_STRIDE tokens), where that is worth
+        recording the step anew."""
         settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         self._check_sampling(prompt, new_tokens, sequences, random, settings)
         if random is None:
@@ -840,7 +854,7 @@ class LlamaDecoder(torch.nn.Module):
         rows = torch.arange(n, device=device)     # which sequences run
         state["token"].copy_(sample(first_logits, random[:, 0].contiguous(), **settings))
         out[:, 0] = state["token"]
-        graph = None
+        graph, before = None, length if fork else 0
         for i in range(1, steps):
             if eos is not None and i % EOS_STRIDE == 0:
                 running = ~(out[rows, :i] == eos).any(dim=1)
@@ -848,7 +862,8 @@ class LlamaDecoder(torch.nn.Module):
                 if live == 0:
                     break
                 # the others move up (of no more sequences than a cache is reordered with)
-                if 2 * live <= rows.numel() <= REORDER_VALUES_MAX // cfg.head_dim:
+                if (2 * live <= rows.numel() <= REORDER_VALUES_MAX // cfg.head_dim
+                        and (not self.fused or self._moves_pay(rows.numel(), live, before + i, steps - i))):
                     keep = running.nonzero().squeeze(1)
                     source = torch.cat((keep, whole(-1, rows.numel() - live)))
                     for cache in state["caches"]:
@@ -870,6 +885,12 @@ class LlamaDecoder(torch.nn.Module):
                         step()
             out[rows, i] = state["token"]
         return out
+
+    def _moves_pay(self, n: int, live: int, held: int, left: int) -> bool:
+        """Whether `live` of n sequences are to go on alone, at the price of
+        recording their step, over caches of `held` tokens for `left` steps."""
+        spared = (n - live) * held * 2 * self.cfg.num_kv_heads * self.cfg.head_dim * self.cfg.num_layers
+        return n > MOVED_ROWS or spared * left >= MOVED_BYTES
 
     def _rows_forward(self, tokens: torch.Tensor, caches: list[QuantizedKVCache], held: torch.Tensor,
                       cos: torch.Tensor, sin: torch.Tensor, prefix_lengths: torch.Tensor | None) -> torch.Tensor:

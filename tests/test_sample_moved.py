@@ -40,6 +40,7 @@ def _run(monkeypatch, model, device, most):
     with monkeypatch.context() as patch:
         patch.setattr(llama, "EOS_STRIDE", 4)
         patch.setattr(llama, "REORDER_VALUES_MAX", most)
+        patch.setattr(llama, "MOVED_ROWS", 0)
         patch.setattr(llama, "sample", lambda x, random, **_: (random * 512).to(torch.int64))
         patch.setattr(LlamaDecoder, "_rows_forward", spy_forward)
         patch.setattr(llama.QuantizedKVCache, "reorder", spy_reorder)
@@ -90,6 +91,7 @@ def test_gpu_captured(gpu, codes, dim, shared, monkeypatch):
     """Steps captured anew once sequences have moved up draw what eager steps draw, to the end."""
     monkeypatch.setattr(llama, "FORK_BYTES_MAX", 0 if shared else 1 << 40)
     monkeypatch.setattr(llama, "EOS_STRIDE", 4)
+    monkeypatch.setattr(llama, "MOVED_ROWS", 0)
     moves = []
     reorder = llama.QuantizedKVCache.reorder
     monkeypatch.setattr(llama.QuantizedKVCache, "reorder", lambda self, *a: (moves.append(a), reorder(self, *a))[1])
@@ -104,3 +106,26 @@ def test_gpu_captured(gpu, codes, dim, shared, monkeypatch):
     captured = model.sample(prompt, 60, **kw)
     count = len(moves)
     assert count > 0 and torch.equal(captured, model.sample(prompt, 60, use_graph=False, **kw)) and len(moves) == 2 * count
+
+
+def test_what_a_move_is_worth():
+    """More than 16 sequences, or 12 GiB of keys and values that need not be read (2 layers of 256 bytes a token)."""
+    model = LlamaDecoder(_cfg(), device="cpu", seed=3)
+    assert model._moves_pay(17, 8, 1, 16) and not model._moves_pay(16, 8, 1, 16)
+    left = (12 << 30) // (8 * 1024 * 2 * 2 * 128)
+    assert model._moves_pay(16, 8, 1024, left) and not model._moves_pay(16, 8, 1024, left - 1)
+    assert not model._moves_pay(16, 9, 1024, left)
+
+
+@pytest.mark.gpu
+def test_gpu_few_short_ones_stay(gpu, monkeypatch):
+    """Eight sequences go on to their end, recorded or not: the draws are those of a run without eos."""
+    monkeypatch.setattr(llama, "EOS_STRIDE", 4)
+    monkeypatch.setattr(llama.QuantizedKVCache, "reorder", None)
+    model = LlamaDecoder(_cfg(), device="cuda", seed=3)
+    prompt, kw = _prompt(33, device="cuda"), dict(sequences=SEQUENCES, top_k=3, random=_numbers(SEQUENCES, 40, device="cuda"))
+    free = model.sample(prompt, 40, **kw)
+    eos = int(free.flatten().mode().values)
+    want = torch.where((free == eos).cumsum(dim=1) > 0, eos, free)
+    for graph in (True, False):
+        assert torch.equal(model.sample(prompt, 40, eos=eos, use_graph=graph, **kw), want)

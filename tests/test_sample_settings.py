@@ -69,6 +69,7 @@ def test_gpu_settings(gpu, shared, monkeypatch):
     """Captured steps draw what eager ones draw, also once sequences have moved up."""
     monkeypatch.setattr(llama, "FORK_BYTES_MAX", 0 if shared else 1 << 40)
     monkeypatch.setattr(llama, "EOS_STRIDE", 4)
+    monkeypatch.setattr(llama, "MOVED_ROWS", 0)
     model = LlamaDecoder(_cfg(), device="cuda", seed=3)
     prompt, numbers, settings = _prompt(33, device="cuda"), _numbers(7, 40, device="cuda"), _settings(7, "cuda")
     free = model.sample(prompt, 40, sequences=7, random=numbers, **settings)
