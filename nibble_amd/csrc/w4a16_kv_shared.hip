@@ -94,7 +94,11 @@ SharedPlan plan_shared(int64_t groups, int64_t prefix_slots, int64_t batch, int6
         // sequences' own slots, which have the memory, take as long (64 sequences of up to
         // 1024 slots behind 8192: 160 workgroups 37 us, 256 of them 44; of up to 64 behind
         // 32768: 63, and 128 of them 95; 256 sequences of 8 rows, of up to 256 slots behind
-        // 8000: 81, and 256 of them 52).
+        // 8000: 81, and 256 of them 52). Of 92 sizes (24 to 256 sequences, 2000 to 32768
+        // prefix slots, 64 to 4096 own ones, six layouts of heads of 64 to 256 dims), each
+        // with 96 to 320 workgroups, these two lie within 10% of the best number for 80; far
+        // from it are 24 sequences of 1024 slots behind 8192 (35 us, 160 workgroups 27) and
+        // of 4096 (41, 96 of them 34), 24 of 256 dims and 512 slots (55, 160 of them 45).
         prefix.prompt = dim == 64 ? all > 64 && (__int128)all * prefix_slots > (6 << 20)
                                   : all > (dim == 128 && prefix_slots <= 6144 ? 128 : 64);
         prefix.column_tiles = all <= 16 ? 1 : all > 32 && all <= 48 && dim == 128 ? 3 : 2;

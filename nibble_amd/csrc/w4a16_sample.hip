@@ -304,9 +304,10 @@ __device__ __forceinline__ double fma_scalar(double a, double b, double c) {
 struct Weights {
     double top, factor, lowest;   // lowest: -60 / factor
     // 2^y of y = (x - top) factor <= 0: the whole part joins the exponent, 2^f with
-    // |f| <= 1/2 is 1 + f times a polynomial through 8 points, off by 2^-38.7. What
-    // lies far below gives 2^-60. N of them step by step together, as each operation
-    // waits for the one before (a pass over 50257 logits 11.2 us, one by one 12).
+    // |f| <= 1/2 is 1 + f times the polynomial that meets (2^f - 1) / f at the 8 Chebyshev
+    // points of [-1/2, 1/2], off by 2^-38.7. What lies far below gives 2^-60. N of them step
+    // by step together, as each operation waits for the one before (a pass over 50257
+    // logits 11.2 us, one by one 12).
     template <int N>
     __device__ __forceinline__ void weights(const float (&x)[N], double (&w)[N]) const {
         constexpr double round = 0x1.8p52;
@@ -674,9 +675,11 @@ struct Places {
 // top_p 37 (2.5 to read, 4.5 to count, 2.5 for the bracket, 19 for the weights, 4 near
 // the limit, 3 for the token), by a top_k of 600 31, by a narrower min_p 14 to 21. bf16
 // rows by value: 16 of 32000 without limits 12.5 us, 256 of 128000 by top_p 43 us (65
-// MB once: 13). Not kept: a row in registers (their spills), weights eight at a time
-// (the same), several workgroups a row (their launches, or a wait for each other, cost
-// what they save up to 50257 logits).
+// MB once: 13). fp16 rows without a small top_k go the fp32 rows' way (32000 logits by
+// top_p 27 us, without limits 12; 50257: 37 and 17; 128000: 63 and 31). Not kept: a row in
+// registers (their spills), weights eight at a time (the same). Not tried: a row over
+// several workgroups, in launches that hand on the largest value, the sums and the limit
+// (they would divide the reading, the counting and the weights, 26 of the 37 us).
 // ---------------------------------------------------------------------------
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
