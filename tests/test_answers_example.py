@@ -1,4 +1,4 @@
-"""The documents' example of several answers to a prompt, run as it stands on the CPU."""
+"""The documented example of several answers to a prompt, run as it stands on the CPU."""
 
 import pathlib
 import re
@@ -12,9 +12,8 @@ from tests import _kv
 
 def _example() -> tuple[str, str]:
     """What the example does once, and what it does at each step."""
-    root = pathlib.Path(__file__).resolve().parent.parent
-    blocks = [b for path in sorted(root.glob("*.md")) for b in re.findall(r"```python\n(.*?)```", path.read_text(), re.S)
-              if "attend_shared(" in b]
+    text = (pathlib.Path(__file__).resolve().parent.parent / "INTEGRATION.md").read_text()
+    blocks = [b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "attend_shared(" in b]
     assert len(blocks) == 1
     once, step = re.split(r"(?=^q = )", blocks[0].replace('"cuda"', '"cpu"'), maxsplit=1, flags=re.M)
     return once, step
